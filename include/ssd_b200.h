@@ -367,6 +367,125 @@ int sattn_train_fwd(const sattn_train_params* p, void* stream);
 int sattn_train_bwd(const sattn_train_params* p, const void* dout, void* dq, void* dk, void* dv,
                     void* dselect_gate, void* stream);
 
+/*
+ * Served selective attention: a paged cache of keys and values in 8 bits for many requests, and
+ * attention over packed prompts. The reference's cache is dense, in full precision, with one
+ * capacity and one write index for the whole batch (inference/selective_attn_cache.py:10-42);
+ * these are its serving form, with grouped heads (Hq query heads, Hkv key heads, query
+ * head h reads key head h / (Hq / Hkv)).
+ *
+ * A page holds page_size consecutive tokens of one request for every key head. A slot is
+ * page * page_size + the token's place in the page. Values are code * scale of their page
+ * and key head:
+ *   k_codes, v_codes  (num_pages, Hkv, page_size, D)  8-bit, 16-byte aligned
+ *   k_scale, v_scale  (num_pages, Hkv)                fp32
+ *   log_gate          (num_pages, Hkv, page_size)     fp32, or NULL (no gates)
+ * page_size in {16, 32, 64, 128}, head_dim D in {32, 64, 128, 256}.
+ */
+typedef enum { SSD_CODE_INT8 = 0, SSD_CODE_E4M3 = 1 } ssd_code_t;
+
+typedef struct sattn_cache {
+  int64_t num_pages, nkv, page_size, head_dim;
+  int32_t code; /* SSD_CODE_INT8 (largest code 127) or SSD_CODE_E4M3 (448) */
+  void* k_codes;
+  void* v_codes;
+  float* k_scale;
+  float* v_scale;
+  float* log_gate;
+} sattn_cache;
+
+/*
+ * Block tables and slots for the next call's tokens, from request lengths alone (no host
+ * synchronisation). Request r holds lengths[r] tokens in the pages block_table[r, 0 ..
+ * ceil(lengths[r] / page_size)) and is to take new_lengths[r] more. Free pages are a ring:
+ * free_pages[i % num_free] for i in [free_state[0], free_state[1]) are free, handed out in that
+ * order to the requests in order. A request whose pages do not fit the table's width, or that
+ * asks for more than is left for it, is not served: its length stays, its slots are -1, and it
+ * and later ones that need a page get none (a request that needs no page is served).
+ *   lengths, new_lengths  (requests,)              int32
+ *   block_table           (requests, table_width)  int32, new entries written in place
+ *   free_pages            (num_free,)              int32
+ *   free_state            (2,)                     int64: handed out, returned (running counts)
+ *   lengths_out           (requests,)              int32: lengths after the tokens are written
+ *   cu_new                (requests + 1,)          int32: offsets of the requests' tokens
+ *   slots, positions      (num_tokens,)            int64, int32: of each token; -1 and 0 past cu_new's end
+ *   free_state_out        (2,)                     int64
+ * Outputs other than block_table do not overlap inputs.
+ */
+int sattn_paged_plan(const int32_t* lengths, const int32_t* new_lengths, int32_t* block_table,
+                     const int32_t* free_pages, const int64_t* free_state, int32_t* lengths_out, int32_t* cu_new,
+                     int64_t* slots, int32_t* positions, int64_t* free_state_out, int64_t requests,
+                     int64_t table_width, int64_t num_free, int64_t num_tokens, int64_t page_size, void* stream);
+
+/*
+ * Writes tokens into the cache at their slots (-1, or past the cache: not written). The tokens of
+ * one page follow one another in `slots`, in the page's order (as sattn_paged_plan gives them).
+ * For a page and key head, with `first` the place of the call's first token in it:
+ *   old = first > 0 ? scale : 0;  new = max(old, max|x| * (1 / largest code))   (fp32, finite x only)
+ *   codes of the call's tokens = round(x / new) (ties to even, saturated); the page's earlier codes
+ *   become round(code * (old / new)) where new > old.
+ * A NaN is held as 0 (int8) or NaN (e4m3), an infinity as the largest code.
+ *   k, v      (num_tokens, Hkv, D)  dtype, with token and head strides in elements
+ *   log_gate  (num_tokens, Hkv)     fp32; NULL exactly when the cache has none
+ */
+int sattn_paged_append(const sattn_cache* cache, const void* k, const void* v, const float* log_gate,
+                       const int64_t* slots, int64_t num_tokens, int64_t k_token_stride, int64_t k_head_stride,
+                       int64_t v_token_stride, int64_t v_head_stride, int32_t dtype, void* stream);
+
+/*
+ * Reads slots back as the values that they stand for: k_out, v_out (num_slots, Hkv, D) dtype,
+ * 16-byte aligned; zeros where a slot is not the cache's.
+ */
+int sattn_paged_read(const sattn_cache* cache, const int64_t* slots, int64_t num_slots, void* k_out, void* v_out,
+                     int32_t dtype, void* stream);
+
+/*
+ * One decode step's attention: for request r with n = lengths[r] cached tokens (its own last),
+ *   s_j = scale * q . k_j + (j < n-1 ? log_gate_j : 0),   out = softmax(s) . v
+ * (the pos-mode gated softmax of sattn_decode_step). A key with log-gate -inf drops out; n = 0 gives
+ * zeros; n is cut to the table's width.
+ *   q, out       (requests, nheads, D)    dtype, 16-byte aligned; nheads a multiple of Hkv
+ *   block_table  (requests, table_width)  int32        lengths  (requests,)  int32
+ * workspace: sattn_paged_decode_workspace_size() bytes (may be 0), 16-byte aligned; nothing in it
+ * needs to start at zero or outlives the call.
+ */
+size_t sattn_paged_decode_workspace_size(const sattn_cache* cache, int64_t requests, int64_t table_width,
+                                         int64_t nheads);
+int sattn_paged_decode(const sattn_cache* cache, const void* q, const int32_t* block_table, const int32_t* lengths,
+                       void* out, int64_t requests, int64_t table_width, int64_t nheads, float scale, int32_t dtype,
+                       void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Selective attention over packed prompts, causal: sequence r is the tokens [cu_seqlens[r],
+ * cu_seqlens[r+1]), and for its positions j <= i
+ *   s_ij = scale * q_i . k_j + (j < i ? log_gate_j : 0),   out_i = softmax_j(s_i) . v
+ * Keys with log-gate -inf drop out for later queries. What a query does not see changes nothing in
+ * its row, infinities and NaN included. Rows past cu_seqlens[R] are written as zeros.
+ *   q          (T, nheads, D)   dtype, token and head strides in elements
+ *   k, v       (T, nkv, D)      dtype, token and head strides in elements
+ *   log_gate   (T, nkv)         fp32 or NULL
+ *   cu_seqlens (R + 1,)         int32, from 0, not falling, at most T
+ *   out        (T, nheads, D)   dtype
+ * All base addresses 16-byte aligned, all strides multiples of 16 bytes; D in {16, 32, 64, 128}.
+ * impl: SSD_IMPL_AUTO takes the tcgen05 kernel for 16-bit types with D 64 or 128 and the
+ * CUDA-core kernel otherwise; SSD_IMPL_TC requires the former, SSD_IMPL_SIMT forces the latter.
+ */
+typedef struct sattn_packed_params {
+  int64_t num_tokens, num_seqs, nheads, nkv, head_dim;
+  int64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+  int32_t dtype;
+  int32_t impl;
+  float scale;
+  const void* q;
+  const void* k;
+  const void* v;
+  const float* log_gate;
+  const int32_t* cu_seqlens;
+  void* out;
+} sattn_packed_params;
+
+int sattn_prefill_packed(const sattn_packed_params* p, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -11,6 +11,9 @@ Public surface (mirrors the reference's ``selective_attention.ops`` and
   ``ssd_scan_backward``, ``ssu_forward``, ``ssm_conv_prefill`` / ``ssm_conv_decode``,
   ``sattn_decode_step`` / ``selective_attn_step`` / ``sattn_prefill``) over the C ABI of
   ``libssd_b200.so`` (``include/ssd_b200.h``).
+- ``paged``: served selective attention, a paged 8-bit cache for many requests
+  (``sattn_paged_plan``, ``sattn_paged_append``, ``sattn_paged_decode``, ``sattn_paged_read``) and
+  attention over packed prompts with grouped heads (``sattn_prefill_packed``).
 - ``HostStreamScan``: the SSD forward on inputs in pinned host memory, with the copies
   of row slices overlapped with the scan (no reference counterpart).
 - ``shim.install()``: make an installed reference package use these kernels.
@@ -36,11 +39,19 @@ from .kernels import (
     ssu_forward,
     state_passing_forward,
 )
+from .paged import (
+    sattn_paged_append,
+    sattn_paged_decode,
+    sattn_paged_plan,
+    sattn_paged_read,
+    sattn_prefill_packed,
+)
 
 __all__ = [
     "SSDScanFn", "SSUFn", "HostStreamScan", "ssd_scan_forward", "ssu_forward", "chunk_cumsum_forward",
     "chunk_state_forward", "state_passing_forward", "bmm_chunk_forward", "chunk_scan_forward",
     "ssd_scan_backward", "ssm_conv_prefill", "ssm_conv_decode", "sattn_decode_step", "selective_attn_step",
     "sattn_prefill", "sattn_train_forward", "sattn_train_backward", "SelectiveAttnTrainFn", "selective_attn_train",
+    "sattn_paged_plan", "sattn_paged_append", "sattn_paged_decode", "sattn_paged_read", "sattn_prefill_packed",
     "check_device_error", "device_error",
 ]

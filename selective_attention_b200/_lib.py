@@ -24,6 +24,7 @@ IMPL_AUTO, IMPL_TC, IMPL_SIMT, IMPL_TC_STAGED = 0, 1, 2, 3
 IMPLS = {"auto": IMPL_AUTO, "tc": IMPL_TC, "simt": IMPL_SIMT, "tc_staged": IMPL_TC_STAGED}
 FUSED_MIN_CHAINS = 128  # SSD_FUSED_MIN_CHAINS
 
+CACHE_CODES = {torch.int8: 0, torch.float8_e4m3fn: 1}  # ssd_code_t
 DTYPE_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 # Every symbol include/ssd_b200.h declares, with its ctypes signature.
@@ -52,6 +53,12 @@ EXPORTS = {
     "sattn_train_workspace_size": (c_size_t, [c_void_p]),
     "sattn_train_fwd": (c_int, [c_void_p, c_void_p]),
     "sattn_train_bwd": (c_int, [c_void_p] * 7),
+    "sattn_paged_plan": (c_int, [c_void_p] * 10 + [c_int64] * 5 + [c_void_p]),
+    "sattn_paged_append": (c_int, [c_void_p] * 5 + [c_int64] * 5 + [c_int32, c_void_p]),
+    "sattn_paged_read": (c_int, [c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int32, c_void_p]),
+    "sattn_paged_decode_workspace_size": (c_size_t, [c_void_p] + [c_int64] * 3),
+    "sattn_paged_decode": (c_int, [c_void_p] * 5 + [c_int64] * 3 + [c_float, c_int32, c_void_p, c_size_t, c_void_p]),
+    "sattn_prefill_packed": (c_int, [c_void_p, c_void_p]),
 }
 
 
@@ -91,6 +98,29 @@ class SattnTrainParams(ctypes.Structure):
         ("q_rot", c_void_p), ("k_rot", c_void_p), ("v", c_void_p), ("select_gate", c_void_p), ("lengths", c_void_p),
         ("out", c_void_p), ("lse", c_void_p), ("log_gate", c_void_p), ("stats", c_void_p),
         ("workspace", c_void_p), ("workspace_bytes", c_size_t),
+    ]
+
+
+class SattnCache(ctypes.Structure):
+    """Mirror of ``sattn_cache`` in include/ssd_b200.h."""
+
+    _fields_ = [
+        ("num_pages", c_int64), ("nkv", c_int64), ("page_size", c_int64), ("head_dim", c_int64), ("code", c_int32),
+        ("k_codes", c_void_p), ("v_codes", c_void_p), ("k_scale", c_void_p), ("v_scale", c_void_p),
+        ("log_gate", c_void_p),
+    ]
+
+
+class SattnPackedParams(ctypes.Structure):
+    """Mirror of ``sattn_packed_params`` in include/ssd_b200.h."""
+
+    _fields_ = [
+        ("num_tokens", c_int64), ("num_seqs", c_int64), ("nheads", c_int64), ("nkv", c_int64), ("head_dim", c_int64),
+        ("q_token_stride", c_int64), ("q_head_stride", c_int64), ("k_token_stride", c_int64),
+        ("k_head_stride", c_int64), ("v_token_stride", c_int64), ("v_head_stride", c_int64),
+        ("dtype", c_int32), ("impl", c_int32), ("scale", c_float),
+        ("q", c_void_p), ("k", c_void_p), ("v", c_void_p), ("log_gate", c_void_p), ("cu_seqlens", c_void_p),
+        ("out", c_void_p),
     ]
 
 

@@ -192,7 +192,8 @@ int ssd_b200_device_error(void* stream) {
   const unsigned int d = fetch_error_sattn(s);
   const unsigned int e = fetch_error_bwd_tc(s);
   const unsigned int f = fetch_error_split(s);
-  return (int)(a ? a : (b ? b : (c ? c : (d ? d : (e ? e : f)))));
+  const unsigned int g = fetch_error_packed(s);
+  return (int)(a ? a : (b ? b : (c ? c : (d ? d : (e ? e : (f ? f : g))))));
 }
 
 int ssd_scan_uses_tensor_cores(const ssd_params* p) {
@@ -662,6 +663,153 @@ int sattn_train_bwd(const sattn_train_params* p, const void* dout, void* dq, voi
   if (!dout || !dq || !dk || !dv || !dselect_gate) return SSD_ERR_INVALID_ARGUMENT;
   if (!aligned16(dout)) return SSD_ERR_INVALID_ARGUMENT;
   return cuda_status(launch_sattn_train_bwd(a, dout, dq, dk, dv, dselect_gate, reinterpret_cast<cudaStream_t>(stream)));
+}
+
+}  // extern "C"
+
+namespace {
+
+// Checks a paged cache's description; its device arrays are only checked for being there.
+int paged_cache(const sattn_cache* c, PagedCache* o) {
+  if (!c || c->num_pages <= 0 || c->nkv <= 0 || c->nkv > 65535 || c->num_pages > 0x7fffffffll)
+    return SSD_ERR_INVALID_ARGUMENT;
+  const int64_t p = c->page_size, d = c->head_dim;
+  if ((p != 16 && p != 32 && p != 64 && p != 128) || (d != 32 && d != 64 && d != 128 && d != 256))
+    return SSD_ERR_INVALID_ARGUMENT;
+  if (c->code != SSD_CODE_INT8 && c->code != SSD_CODE_E4M3) return SSD_ERR_UNSUPPORTED_DTYPE;
+  if (!c->k_codes || !c->v_codes || !c->k_scale || !c->v_scale || !aligned16(c->k_codes) || !aligned16(c->v_codes))
+    return SSD_ERR_INVALID_ARGUMENT;
+  o->k = reinterpret_cast<unsigned char*>(c->k_codes);
+  o->v = reinterpret_cast<unsigned char*>(c->v_codes);
+  o->ks = c->k_scale;
+  o->vs = c->v_scale;
+  o->gate = c->log_gate;
+  o->pages = c->num_pages;
+  o->nkv = (int)c->nkv;
+  o->page = (int)p;
+  o->page_shift = p == 16 ? 4 : (p == 32 ? 5 : (p == 64 ? 6 : 7));
+  o->D = (int)d;
+  o->code = c->code;
+  return SSD_OK;
+}
+
+bool decode_geometry_ok(const PagedCache& c, int64_t requests, int64_t width, int64_t nheads) {
+  return requests > 0 && requests <= 0x7fffffffll && width > 0 && nheads > 0 && nheads <= 65535 &&
+         nheads % c.nkv == 0 && width * c.page <= 0x7fffffffll;
+}
+
+}  // namespace
+
+extern "C" {
+
+int sattn_paged_plan(const int32_t* lengths, const int32_t* new_lengths, int32_t* block_table,
+                     const int32_t* free_pages, const int64_t* free_state, int32_t* lengths_out, int32_t* cu_new,
+                     int64_t* slots, int32_t* positions, int64_t* free_state_out, int64_t requests,
+                     int64_t table_width, int64_t num_free, int64_t num_tokens, int64_t page_size, void* stream) {
+  if (requests < 0 || table_width < 0 || num_free < 0 || num_tokens < 0 || requests > 0x7fffffffll ||
+      num_tokens > 0x7fffffffll || table_width * page_size > 0x7fffffffll || num_free > 0x7fffffffll)
+    return SSD_ERR_INVALID_ARGUMENT;
+  if (page_size != 16 && page_size != 32 && page_size != 64 && page_size != 128) return SSD_ERR_INVALID_ARGUMENT;
+  if (!free_state || !free_state_out || !cu_new || (num_tokens && (!slots || !positions)) ||
+      (requests && (!lengths || !new_lengths || !lengths_out || (table_width && !block_table))) ||
+      (num_free && !free_pages))
+    return SSD_ERR_INVALID_ARGUMENT;
+  const int shift = page_size == 16 ? 4 : (page_size == 32 ? 5 : (page_size == 64 ? 6 : 7));
+  return cuda_status(launch_paged_plan(lengths, new_lengths, block_table, free_pages,
+                                       reinterpret_cast<const long long*>(free_state), lengths_out, cu_new,
+                                       reinterpret_cast<long long*>(slots), positions,
+                                       reinterpret_cast<long long*>(free_state_out), (int)requests, (int)table_width,
+                                       num_free, num_tokens, shift, reinterpret_cast<cudaStream_t>(stream)));
+}
+
+int sattn_paged_append(const sattn_cache* cache, const void* k, const void* v, const float* log_gate,
+                       const int64_t* slots, int64_t num_tokens, int64_t k_token_stride, int64_t k_head_stride,
+                       int64_t v_token_stride, int64_t v_head_stride, int32_t dtype, void* stream) {
+  PagedCache c{};
+  const int st = paged_cache(cache, &c);
+  if (st) return st;
+  if (!dtype_ok(dtype)) return SSD_ERR_UNSUPPORTED_DTYPE;
+  if (num_tokens < 0 || num_tokens > 0x7fffffffll) return SSD_ERR_INVALID_ARGUMENT;
+  if ((log_gate != nullptr) != (c.gate != nullptr) && num_tokens) return SSD_ERR_INVALID_ARGUMENT;
+  if (num_tokens == 0) return SSD_OK;
+  if (!k || !v || !slots) return SSD_ERR_INVALID_ARGUMENT;
+  return cuda_status(launch_paged_append(c, k, v, log_gate, reinterpret_cast<const long long*>(slots), num_tokens,
+                                         k_token_stride, k_head_stride, v_token_stride, v_head_stride, dtype,
+                                         reinterpret_cast<cudaStream_t>(stream)));
+}
+
+int sattn_paged_read(const sattn_cache* cache, const int64_t* slots, int64_t num_slots, void* k_out, void* v_out,
+                     int32_t dtype, void* stream) {
+  PagedCache c{};
+  const int st = paged_cache(cache, &c);
+  if (st) return st;
+  if (!dtype_ok(dtype)) return SSD_ERR_UNSUPPORTED_DTYPE;
+  if (num_slots < 0 || num_slots > (1ll << 40)) return SSD_ERR_INVALID_ARGUMENT;
+  if (num_slots == 0) return SSD_OK;
+  if (!slots || !k_out || !v_out || !aligned16(k_out) || !aligned16(v_out)) return SSD_ERR_INVALID_ARGUMENT;
+  return cuda_status(launch_paged_read(c, reinterpret_cast<const long long*>(slots), num_slots, k_out, v_out, dtype,
+                                       reinterpret_cast<cudaStream_t>(stream)));
+}
+
+size_t sattn_paged_decode_workspace_size(const sattn_cache* cache, int64_t requests, int64_t table_width,
+                                         int64_t nheads) {
+  PagedCache c{};
+  if (paged_cache(cache, &c) || !decode_geometry_ok(c, requests, table_width, nheads)) return 0;
+  return paged_decode_workspace((int)requests, (int)table_width, (int)nheads, c.nkv, c.page_shift, c.D);
+}
+
+int sattn_paged_decode(const sattn_cache* cache, const void* q, const int32_t* block_table, const int32_t* lengths,
+                       void* out, int64_t requests, int64_t table_width, int64_t nheads, float scale, int32_t dtype,
+                       void* workspace, size_t workspace_bytes, void* stream) {
+  PagedCache c{};
+  const int st = paged_cache(cache, &c);
+  if (st) return st;
+  if (!dtype_ok(dtype)) return SSD_ERR_UNSUPPORTED_DTYPE;
+  if (!decode_geometry_ok(c, requests, table_width, nheads)) return SSD_ERR_INVALID_ARGUMENT;
+  if (!q || !block_table || !lengths || !out || !aligned16(q) || !aligned16(out)) return SSD_ERR_INVALID_ARGUMENT;
+  const size_t need = paged_decode_workspace((int)requests, (int)table_width, (int)nheads, c.nkv, c.page_shift, c.D);
+  if (need && (workspace_bytes < need || !workspace)) return SSD_ERR_WORKSPACE_TOO_SMALL;
+  if (need && !aligned16(workspace)) return SSD_ERR_INVALID_ARGUMENT;
+  return cuda_status(launch_paged_decode(c, q, block_table, lengths, out, (int)requests, (int)table_width, (int)nheads,
+                                         scale, dtype, workspace, reinterpret_cast<cudaStream_t>(stream)));
+}
+
+int sattn_prefill_packed(const sattn_packed_params* p, void* stream) {
+  if (!p) return SSD_ERR_INVALID_ARGUMENT;
+  if (p->num_tokens < 0 || p->num_tokens > 0x7fffffffll || p->num_seqs < 0 || p->num_seqs > 0x7fffffffll ||
+      p->nheads <= 0 || p->nkv <= 0 || p->nheads > 0x7fffffffll || p->nheads % p->nkv != 0)
+    return SSD_ERR_INVALID_ARGUMENT;
+  const int64_t D = p->head_dim;
+  if (D != 16 && D != 32 && D != 64 && D != 128) return SSD_ERR_INVALID_ARGUMENT;
+  if (!dtype_ok(p->dtype)) return SSD_ERR_UNSUPPORTED_DTYPE;
+  if (p->num_tokens == 0) return SSD_OK;
+  if (!p->q || !p->k || !p->v || !p->out || !p->cu_seqlens || !aligned16(p->q) || !aligned16(p->k) ||
+      !aligned16(p->v) || !aligned16(p->out))
+    return SSD_ERR_INVALID_ARGUMENT;
+  const int64_t es = p->dtype == SSD_F32 ? 4 : 2;
+  const int64_t strides[6] = {p->q_token_stride, p->q_head_stride, p->k_token_stride,
+                              p->k_head_stride,  p->v_token_stride, p->v_head_stride};
+  for (int64_t x : strides)
+    if (x < 0 || (x * es) % 16 != 0) return SSD_ERR_INVALID_ARGUMENT;
+  const bool tc_ok = sattn_packed_tc_supported((int)D, p->dtype);
+  if (p->impl == SSD_IMPL_TC && !tc_ok) return SSD_ERR_INVALID_ARGUMENT;
+  PackedArgs a{};
+  a.q = p->q;
+  a.k = p->k;
+  a.v = p->v;
+  a.log_gate = p->log_gate;
+  a.cu = p->cu_seqlens;
+  a.out = p->out;
+  a.R = (int)p->num_seqs;
+  a.T = (int)p->num_tokens;
+  a.Hq = (int)p->nheads;
+  a.Hk = (int)p->nkv;
+  a.D = (int)D;
+  a.dtype = p->dtype;
+  a.st = PackedStrides{strides[0], strides[1], strides[2], strides[3], strides[4], strides[5]};
+  a.scale = p->scale;
+  a.use_tc = p->impl != SSD_IMPL_SIMT && tc_ok;
+  return cuda_status(launch_sattn_packed(a, reinterpret_cast<cudaStream_t>(stream)));
 }
 
 }  // extern "C"

@@ -97,6 +97,46 @@ unsigned int fetch_error_sattn(cudaStream_t s);
 cudaError_t launch_sattn_attn_fa(const void* q, const void* k, const void* v, const float* lg, void* out, float* lse,
                                  int b, int H, int L, float scale, int dtype, int causal, cudaStream_t s);
 
+// paged.cu (the paged 8-bit key/value cache), paged_decode.cu (attention over it)
+struct PagedCache {
+  unsigned char *k, *v;  // codes (pages, nkv, page, D)
+  float *ks, *vs;        // scales (pages, nkv)
+  float* gate;           // log-gates (pages, nkv, page) or null
+  long long pages;
+  int nkv, page, page_shift, D, code;
+};
+cudaError_t launch_paged_plan(const int* lengths, const int* new_lengths, int* table, const int* free_pages,
+                              const long long* free_state, int* lengths_out, int* cu_new, long long* slots,
+                              int* positions, long long* free_state_out, int R, int W, long long F, long long T,
+                              int page_shift, cudaStream_t s);
+// Token and head strides in elements; gate (n, nkv) or null.
+cudaError_t launch_paged_append(const PagedCache& c, const void* k, const void* v, const float* gate,
+                                const long long* slots, long long n, long long k_ts, long long k_hs, long long v_ts,
+                                long long v_hs, int dtype, cudaStream_t s);
+cudaError_t launch_paged_read(const PagedCache& c, const long long* slots, long long n, void* ko, void* vo, int dtype,
+                              cudaStream_t s);
+size_t paged_decode_workspace(int R, int W, int Hq, int Hk, int page_shift, int D);
+cudaError_t launch_paged_decode(const PagedCache& c, const void* q, const int* table, const int* lengths, void* out,
+                                int R, int W, int Hq, float scale, int dtype, void* workspace, cudaStream_t s);
+
+// sattn_packed.cu (attention over packed prompts; grouped heads)
+struct PackedStrides {
+  long long q_ts, q_hs, k_ts, k_hs, v_ts, v_hs;  // token and head strides, elements
+};
+struct PackedArgs {
+  const void *q, *k, *v;
+  const float* log_gate;  // (T, Hk) or null
+  const int* cu;          // (R + 1,)
+  void* out;              // (T, Hq, D)
+  int R, T, Hq, Hk, D, dtype;
+  PackedStrides st;
+  float scale;
+  int use_tc;
+};
+bool sattn_packed_tc_supported(int D, int dtype);
+cudaError_t launch_sattn_packed(const PackedArgs& a, cudaStream_t s);
+unsigned int fetch_error_packed(cudaStream_t s);
+
 // sattn_train.cu (training-mode selective attention and its backward; CUDA cores)
 struct SattnTrainArgs {
   int B, H, L, D, dtype, causal;

@@ -1,0 +1,389 @@
+// paged.cu - the paged 8-bit key/value cache of served selective attention: block tables and
+// slot maps from request lengths (plan), quantised writes (append) and reads back (read).
+// The reference keeps a dense full-precision cache of one capacity per batch
+// (inference/selective_attn_cache.py:10-42); this is its form for many requests at once.
+//
+// A page holds page_size consecutive tokens of one request, for every key head:
+//   codes (num_pages, Hkv, page_size, D) 8-bit, scale (num_pages, Hkv) fp32, so that
+//   value = code * scale[page, head]; log-gates (num_pages, Hkv, page_size) fp32.
+// Slot s is token s % page_size of page s / page_size.
+#include <math.h>
+
+#include "common.cuh"
+#include "kernels.h"
+#include "paged.cuh"
+#include "sattn_tiles.cuh"
+
+namespace ssdb200 {
+namespace {
+
+// ---------------------------------------------------------------------------
+// plan
+// ---------------------------------------------------------------------------
+// One launch; a CTA writes the slots and positions of kPlanTokens new tokens. Each CTA sums all
+// requests' new tokens and pages by itself (a block scan over pairs packed in 64 bits), which
+// for some hundred requests costs less than a second launch or a wait between CTAs would; the
+// requests that begin in or reach into its tokens leave an entry at their first token there, and
+// a running maximum over the tokens finds each token's entry. A page's table entry is written by
+// the token at its first position, so no two threads write one entry and none is read that
+// another writes.
+constexpr int kPlanThreads = 256;
+constexpr int kPlanPer = 4;
+constexpr int kPlanTokens = kPlanThreads * kPlanPer;
+
+struct PlanEntry {
+  int r, len, cu, pages_before;  // request, cached tokens, its first new token, pages given before it
+  int served;
+};
+
+__device__ __forceinline__ unsigned long long warp_scan_add(unsigned long long v, int lane) {
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const unsigned long long o = __shfl_up_sync(0xffffffffu, v, off);
+    if (lane >= off) v += o;
+  }
+  return v;
+}
+
+__global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(
+    const int* __restrict__ lengths, const int* __restrict__ new_lengths, int* table, const int* __restrict__ free_pages,
+    const long long* __restrict__ free_state, int* __restrict__ lengths_out, int* __restrict__ cu_new,
+    long long* __restrict__ slots, int* __restrict__ positions, long long* __restrict__ free_state_out, int R, int W,
+    long long F, long long T, int page_shift) {
+  __shared__ PlanEntry ent[kPlanTokens];
+  __shared__ short start[kPlanTokens];
+  __shared__ unsigned long long wsum[kPlanThreads / 32];
+  __shared__ int wmax[kPlanThreads / 32];
+  __shared__ long long s_given;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const long long t0 = (long long)blockIdx.x * kPlanTokens;
+  const long long t1 = min(t0 + kPlanTokens, T);
+  const int page = 1 << page_shift;
+  const long long head = free_state[0], tail = free_state[1];
+  const long long avail = min(tail - head, F);
+#pragma unroll
+  for (int i = 0; i < kPlanPer; ++i) start[tid + i * kPlanThreads] = -1;
+  if (tid == 0) s_given = 0;
+  __syncthreads();
+  unsigned long long carry = 0;  // low word: new tokens, high word: pages
+  for (int r0 = 0; r0 < R; r0 += kPlanThreads) {
+    const int r = r0 + tid;
+    int len = 0, add = 0, need = 0;
+    bool fits = true;
+    if (r < R) {
+      len = max(lengths[r], 0);
+      add = max(new_lengths[r], 0);
+      const long long end = ((long long)len + add + page - 1) >> page_shift;
+      fits = end <= W;
+      need = fits ? (int)(end - (((long long)len + page - 1) >> page_shift)) : 0;
+    }
+    const unsigned long long mine = ((unsigned long long)(unsigned)need << 32) | (unsigned)add;
+    unsigned long long incl = warp_scan_add(mine, lane);
+    if (lane == 31) wsum[warp] = incl;
+    __syncthreads();
+    unsigned long long before = carry, all = carry;
+#pragma unroll
+    for (int w = 0; w < kPlanThreads / 32; ++w) {
+      const unsigned long long x = wsum[w];
+      if (w < warp) before += x;
+      all += x;
+    }
+    carry = all;
+    incl += before;
+    const long long upto = (long long)(incl >> 32);
+    const int cu = (int)((unsigned)incl - (unsigned)add);
+    const bool served = r < R && fits && (need == 0 || upto <= avail);
+    if (r < R) {
+      if (add > 0 && cu < t1 && cu + (long long)add > t0) {
+        const int at = (int)(max((long long)cu, t0) - t0);
+        ent[at] = PlanEntry{r, len, cu, (int)(upto - need), served};
+        start[at] = (short)at;
+      }
+      if (blockIdx.x == 0) {
+        lengths_out[r] = served ? len + add : lengths[r];
+        cu_new[r + 1] = cu + add;
+        if (served && need > 0) atomicMax((unsigned long long*)&s_given, (unsigned long long)upto);
+      }
+    }
+    __syncthreads();  // wsum is rewritten, ent and start are read
+  }
+  if (blockIdx.x == 0 && tid == 0) {
+    cu_new[0] = 0;
+    free_state_out[0] = head + s_given;
+    free_state_out[1] = tail;
+  }
+  // the entry of each token: running maximum of start over kPlanPer tokens a thread
+  int own[kPlanPer], m = -1;
+#pragma unroll
+  for (int i = 0; i < kPlanPer; ++i) {
+    m = max(m, (int)start[tid * kPlanPer + i]);
+    own[i] = m;
+  }
+  int incl = m;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const int o = __shfl_up_sync(0xffffffffu, incl, off);
+    if (lane >= off) incl = max(incl, o);
+  }
+  if (lane == 31) wmax[warp] = incl;
+  __syncthreads();
+  int prev = __shfl_up_sync(0xffffffffu, incl, 1);
+  if (lane == 0) prev = -1;
+  for (int w = 0; w < warp; ++w) prev = max(prev, wmax[w]);
+  const long long total = (long long)(unsigned)carry;
+#pragma unroll
+  for (int i = 0; i < kPlanPer; ++i) {
+    const long long t = t0 + tid * kPlanPer + i;
+    if (t >= T) break;
+    const int at = max(own[i], prev);
+    long long slot = -1;
+    int pos = 0;
+    if (t < total && at >= 0) {
+      const PlanEntry e = ent[at];
+      pos = e.len + (int)(t - e.cu);
+      if (e.served) {
+        const int pg = pos >> page_shift, has = (e.len + page - 1) >> page_shift, in = pos & (page - 1);
+        int id;
+        if (pg < has) {
+          id = table[(long long)e.r * W + pg];
+        } else {
+          id = free_pages[(head + e.pages_before + (pg - has)) % F];
+          if (in == 0) table[(long long)e.r * W + pg] = id;
+        }
+        slot = (long long)id * page + in;
+      }
+    }
+    slots[t] = slot;
+    positions[t] = pos;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// append
+// ---------------------------------------------------------------------------
+// CTA = (block of `per` tokens, key head, K or V). A segment is a run of tokens with consecutive
+// slots in one page; the CTA in whose block it begins writes all of it (up to page - 1 tokens
+// past its block), so each page and head has one writer. Three steps: the largest finite
+// magnitude of each row; the segment's scale from its rows and the page's old scale; the codes
+// of the rows, and, where the scale grew, of the page's older rows. x is read twice, the
+// second time from L1/L2.
+constexpr int kAppThreads = 256;
+constexpr int kAppRows = 256;  // rows of one CTA: per + page - 1 <= 255
+
+template <typename T, bool VEC>
+__device__ __forceinline__ void load_row8(const T* p, float (&x)[8]) {
+  if constexpr (VEC) {
+    load8<T>(p, x);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = Ld<T>::f(p + e);
+  }
+}
+
+template <typename T, typename C, bool VEC>
+__global__ void __launch_bounds__(kAppThreads) paged_append_kernel(
+    const T* __restrict__ kx, const T* __restrict__ vx, const float* __restrict__ gate,
+    const long long* __restrict__ slots, unsigned char* kc, unsigned char* vc, float* ks, float* vs, float* gc,
+    long long num_pages, int H, int page_shift, int D, long long Tn, long long k_ts, long long k_hs, long long v_ts,
+    long long v_hs, int per) {
+  __shared__ float rmax[kAppRows];    // per row; the segment's new scale after step 2
+  __shared__ float ratio[kAppRows];   // at a segment's first row: old / new scale where it grew, else 0
+  __shared__ short head_of[kAppRows]; // row -> its segment's first row, -1 if the row is not this CTA's
+  __shared__ int s_rows;
+  const int tid = threadIdx.x, page = 1 << page_shift;
+  const int h = blockIdx.y;
+  const bool is_v = blockIdx.z != 0;
+  const T* x = is_v ? vx + h * v_hs : kx + h * k_hs;
+  const long long ts = is_v ? v_ts : k_ts;
+  unsigned char* codes = is_v ? vc : kc;
+  float* scale = is_v ? vs : ks;
+  const long long t0 = (long long)blockIdx.x * per;
+  const long long nslots = num_pages << page_shift;
+  const int most = (int)min((long long)per + page - 1, Tn - t0);  // rows that can be this CTA's
+  if (tid == 0) s_rows = 0;
+  auto slot_of = [&](long long t) -> long long {
+    const long long s = slots[t];
+    return s >= 0 && s < nslots ? s : -1;
+  };
+  // a row's segment begins at the row or at most page - 1 rows before it
+  for (int i = tid; i < most; i += kAppThreads) {
+    const long long s = slot_of(t0 + i);
+    int first = -1;
+    if (s >= 0) {
+      const int back = (int)(s & (page - 1));
+      int b = 0;
+      while (b < back && t0 + i - b > 0 && slots[t0 + i - b - 1] == s - b - 1) ++b;
+      first = i - b;
+      if (first < 0 || first >= per) first = -1;  // another CTA's
+    }
+    head_of[i] = (short)first;
+    rmax[i] = 0.f;
+    if (first >= 0) atomicMax(&s_rows, i + 1);
+  }
+  __syncthreads();
+  const int rows = s_rows;
+  if (rows == 0) return;
+  const int lpr = D >> 3;                   // lanes per row, 8 elements each
+  const int sub = tid % lpr, grp = tid / lpr, ngrp = kAppThreads / lpr;
+  for (int i0 = 0; i0 < rows; i0 += ngrp) {
+    const int i = i0 + grp;
+    const bool live = i < rows && head_of[i] >= 0;
+    float m = 0.f;
+    if (live) {
+      float v[8];
+      load_row8<T, VEC>(x + (t0 + i) * ts + sub * 8, v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float a = fabsf(v[e]);
+        m = fmaxf(m, a < INFINITY ? a : 0.f);  // infinities and NaN do not set the scale
+      }
+    }
+    for (int off = 1; off < lpr; off <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+    if (live && sub == 0) rmax[i] = m;
+  }
+  __syncthreads();
+  for (int i = tid; i < rows; i += kAppThreads) {
+    if (head_of[i] != i) continue;
+    float m = 0.f;
+    for (int j = i; j < rows && j < i + page && head_of[j] == i; ++j) m = fmaxf(m, rmax[j]);
+    const long long s = slots[t0 + i];
+    float* sp = scale + (s >> page_shift) * H + h;
+    const float was = (s & (page - 1)) ? *sp : 0.f;  // a page that begins here has no older rows
+    const float now = fmaxf(was, m * Code<C>::kPerMost);
+    ratio[i] = now > was ? __fdiv_rn(was, now) : -1.f;
+    *sp = now;
+    // the rows' step reads it below; other segments' rows are apart
+    rmax[i] = now;
+  }
+  __syncthreads();
+  for (int i0 = 0; i0 < rows; i0 += ngrp) {
+    const int i = i0 + grp;
+    const int first = i < rows ? head_of[i] : -1;
+    if (first < 0) continue;
+    const long long s = slots[t0 + i];
+    const long long row = ((s >> page_shift) * H + h) * page + (s & (page - 1));
+    float v[8];
+    load_row8<T, VEC>(x + (t0 + i) * ts + sub * 8, v);
+    const float sc = rmax[first];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = sc > 0.f ? __fdiv_rn(v[e], sc) : 0.f;
+    *reinterpret_cast<uint2*>(codes + row * D + sub * 8) = Code<C>::pack8(v);
+    if (!is_v && gate && sub == 0) gc[row] = gate[(t0 + i) * H + h];
+  }
+  // older rows of the pages whose scale grew
+  for (int i = 0; i < min(rows, per); ++i) {
+    if (head_of[i] != i || ratio[i] < 0.f) continue;
+    const long long s = slots[t0 + i];
+    const int older = (int)(s & (page - 1));
+    unsigned char* base = codes + ((s >> page_shift) * H + h) * (long long)page * D;
+    for (int j = grp; j < older; j += ngrp) {
+      uint2* p = reinterpret_cast<uint2*>(base + (long long)j * D + sub * 8);
+      float v[8];
+      Code<C>::unpack8(*p, v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] *= ratio[i];
+      *p = Code<C>::pack8(v);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// read: values of the given slots, (N, H, D) for K and V; slots outside the cache give zeros.
+// One thread reads 8 codes and writes 8 values; bound by writing them.
+// ---------------------------------------------------------------------------
+template <typename T, typename C>
+__global__ void __launch_bounds__(256) paged_read_kernel(const long long* __restrict__ slots,
+                                                         const unsigned char* __restrict__ kc,
+                                                         const unsigned char* __restrict__ vc,
+                                                         const float* __restrict__ ks, const float* __restrict__ vs,
+                                                         T* __restrict__ ko, T* __restrict__ vo, long long num_pages,
+                                                         int H, int page_shift, int D, long long n8) {
+  const int lpr = D >> 3, page = 1 << page_shift;
+  const bool is_v = blockIdx.y != 0;
+  const unsigned char* codes = is_v ? vc : kc;
+  const float* scale = is_v ? vs : ks;
+  T* out = is_v ? vo : ko;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n8; i += (long long)gridDim.x * 256) {
+    const long long rh = i / lpr;
+    const int sub = (int)(i - rh * lpr);
+    const long long t = rh / H;
+    const int h = (int)(rh - t * H);
+    const long long s = slots[t];
+    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (s >= 0 && s < (num_pages << page_shift)) {
+      const long long ph = (s >> page_shift) * H + h;
+      Code<C>::unpack8(*reinterpret_cast<const uint2*>(codes + (ph * page + (s & (page - 1))) * D + sub * 8), v);
+      const float sc = scale[ph];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] *= sc;
+    }
+    store8<T>(out + i * 8, v);
+  }
+}
+
+template <typename T, typename C>
+cudaError_t append_t(const PagedCache& c, const void* k, const void* v, const float* gate, const long long* slots,
+                     long long n, long long k_ts, long long k_hs, long long v_ts, long long v_hs, cudaStream_t s) {
+  // Few tokens: small blocks, so that many CTAs share them. Many: a block is a page (each CTA then
+  // has one segment or two, and few CTAs find none).
+  const int per = n * c.nkv <= 2048 ? 4 : (c.page < 16 ? 16 : c.page);
+  const bool vec = (reinterpret_cast<uintptr_t>(k) % 16 == 0) && (reinterpret_cast<uintptr_t>(v) % 16 == 0) &&
+                   (k_ts * sizeof(T)) % 16 == 0 && (k_hs * sizeof(T)) % 16 == 0 && (v_ts * sizeof(T)) % 16 == 0 &&
+                   (v_hs * sizeof(T)) % 16 == 0;
+  const long long blocks = (n + per - 1) / per;
+  if (blocks > 0x7fffffffll) return cudaErrorInvalidValue;
+  dim3 grid((unsigned)blocks, (unsigned)c.nkv, 2);
+  auto fn = vec ? paged_append_kernel<T, C, true> : paged_append_kernel<T, C, false>;
+  fn<<<grid, kAppThreads, 0, s>>>((const T*)k, (const T*)v, gate, slots, c.k, c.v, c.ks, c.vs, c.gate, c.pages,
+                                  c.nkv, c.page_shift, c.D, n, k_ts, k_hs, v_ts, v_hs, per);
+  return cudaGetLastError();
+}
+
+template <typename T, typename C>
+cudaError_t read_t(const PagedCache& c, const long long* slots, long long n, void* ko, void* vo, cudaStream_t s) {
+  const long long n8 = n * c.nkv * (c.D >> 3);
+  const long long blocks = (n8 + 255) / 256;
+  dim3 grid((unsigned)(blocks < 148 * 64 ? blocks : 148 * 64), 2);
+  paged_read_kernel<T, C><<<grid, 256, 0, s>>>(slots, c.k, c.v, c.ks, c.vs, (T*)ko, (T*)vo, c.pages, c.nkv,
+                                               c.page_shift, c.D, n8);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_paged_plan(const int* lengths, const int* new_lengths, int* table, const int* free_pages,
+                              const long long* free_state, int* lengths_out, int* cu_new, long long* slots,
+                              int* positions, long long* free_state_out, int R, int W, long long F, long long T,
+                              int page_shift, cudaStream_t s) {
+  long long blocks = (T + kPlanTokens - 1) / kPlanTokens;
+  if (blocks < 1) blocks = 1;
+  if (blocks > 0x7fffffffll) return cudaErrorInvalidValue;
+  paged_plan_kernel<<<(unsigned)blocks, kPlanThreads, 0, s>>>(lengths, new_lengths, table, free_pages, free_state,
+                                                              lengths_out, cu_new, slots, positions, free_state_out, R,
+                                                              W, F, T, page_shift);
+  return cudaGetLastError();
+}
+
+#define PAGED_DISPATCH(fn, ...)                                                     \
+  do {                                                                              \
+    const bool e4m3 = c.code == SSD_CODE_E4M3;                                      \
+    switch (dtype) {                                                                \
+      case SSD_F32: return e4m3 ? fn<float, E4M3>(__VA_ARGS__) : fn<float, Int8>(__VA_ARGS__); \
+      case SSD_BF16: return e4m3 ? fn<__nv_bfloat16, E4M3>(__VA_ARGS__) : fn<__nv_bfloat16, Int8>(__VA_ARGS__); \
+      case SSD_F16: return e4m3 ? fn<__half, E4M3>(__VA_ARGS__) : fn<__half, Int8>(__VA_ARGS__); \
+    }                                                                               \
+    return cudaErrorInvalidValue;                                                   \
+  } while (0)
+
+cudaError_t launch_paged_append(const PagedCache& c, const void* k, const void* v, const float* gate,
+                                const long long* slots, long long n, long long k_ts, long long k_hs, long long v_ts,
+                                long long v_hs, int dtype, cudaStream_t s) {
+  PAGED_DISPATCH(append_t, c, k, v, gate, slots, n, k_ts, k_hs, v_ts, v_hs, s);
+}
+
+cudaError_t launch_paged_read(const PagedCache& c, const long long* slots, long long n, void* ko, void* vo, int dtype,
+                              cudaStream_t s) {
+  PAGED_DISPATCH(read_t, c, slots, n, ko, vo, s);
+}
+
+}  // namespace ssdb200
