@@ -379,7 +379,7 @@ int sattn_train_bwd(const sattn_train_params* p, const void* dout, void* dq, voi
  * and key head:
  *   k_codes, v_codes  (num_pages, Hkv, page_size, D)  8-bit, 16-byte aligned
  *   k_scale, v_scale  (num_pages, Hkv)                fp32
- *   log_gate          (num_pages, Hkv, page_size)     fp32, or NULL (no gates)
+ *   log_gate          (num_pages, Hkv, page_size)     fp32, 16-byte aligned, or NULL (no gates)
  * page_size in {16, 32, 64, 128}, head_dim D in {32, 64, 128, 256}.
  */
 typedef enum { SSD_CODE_INT8 = 0, SSD_CODE_E4M3 = 1 } ssd_code_t;

@@ -677,7 +677,8 @@ int paged_cache(const sattn_cache* c, PagedCache* o) {
   if ((p != 16 && p != 32 && p != 64 && p != 128) || (d != 32 && d != 64 && d != 128 && d != 256))
     return SSD_ERR_INVALID_ARGUMENT;
   if (c->code != SSD_CODE_INT8 && c->code != SSD_CODE_E4M3) return SSD_ERR_UNSUPPORTED_DTYPE;
-  if (!c->k_codes || !c->v_codes || !c->k_scale || !c->v_scale || !aligned16(c->k_codes) || !aligned16(c->v_codes))
+  if (!c->k_codes || !c->v_codes || !c->k_scale || !c->v_scale || !aligned16(c->k_codes) || !aligned16(c->v_codes) ||
+      !aligned16(c->log_gate))
     return SSD_ERR_INVALID_ARGUMENT;
   o->k = reinterpret_cast<unsigned char*>(c->k_codes);
   o->v = reinterpret_cast<unsigned char*>(c->v_codes);

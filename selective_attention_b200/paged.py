@@ -102,8 +102,8 @@ def _cache(k_cache, v_cache, k_scale, v_scale, log_gate_cache) -> _lib.SattnCach
                  (log_gate_cache, "log_gate_cache")):
         if t is not None and not t.is_contiguous():
             raise ValueError(f"[{n}] must be contiguous (it is used in place)")
-    for t, n in ((k_cache, "k_cache"), (v_cache, "v_cache")):
-        if t.data_ptr() % 16:
+    for t, n in ((k_cache, "k_cache"), (v_cache, "v_cache"), (log_gate_cache, "log_gate_cache")):
+        if t is not None and t.data_ptr() % 16:
             raise ValueError(f"[{n}] must start on a 16-byte boundary")
     return _lib.SattnCache(num_pages=P, nkv=H, page_size=page, head_dim=D, code=_lib.CACHE_CODES[k_cache.dtype],
                            k_codes=_lib.ptr(k_cache), v_codes=_lib.ptr(v_cache), k_scale=_lib.ptr(k_scale),
