@@ -193,7 +193,8 @@ int ssd_b200_device_error(void* stream) {
   const unsigned int e = fetch_error_bwd_tc(s);
   const unsigned int f = fetch_error_split(s);
   const unsigned int g = fetch_error_packed(s);
-  return (int)(a ? a : (b ? b : (c ? c : (d ? d : (e ? e : (f ? f : g))))));
+  const unsigned int h = fetch_error_paged(s);
+  return (int)(a ? a : (b ? b : (c ? c : (d ? d : (e ? e : (f ? f : (g ? g : h)))))));
 }
 
 int ssd_scan_uses_tensor_cores(const ssd_params* p) {
@@ -756,7 +757,7 @@ size_t sattn_paged_decode_workspace_size(const sattn_cache* cache, int64_t reque
                                          int64_t nheads) {
   PagedCache c{};
   if (paged_cache(cache, &c) || !decode_geometry_ok(c, requests, table_width, nheads)) return 0;
-  return paged_decode_workspace((int)requests, (int)table_width, (int)nheads, c.nkv, c.page_shift, c.D);
+  return paged_decode_workspace((int)nheads, c.nkv, c.D);
 }
 
 int sattn_paged_decode(const sattn_cache* cache, const void* q, const int32_t* block_table, const int32_t* lengths,
@@ -768,7 +769,7 @@ int sattn_paged_decode(const sattn_cache* cache, const void* q, const int32_t* b
   if (!dtype_ok(dtype)) return SSD_ERR_UNSUPPORTED_DTYPE;
   if (!decode_geometry_ok(c, requests, table_width, nheads)) return SSD_ERR_INVALID_ARGUMENT;
   if (!q || !block_table || !lengths || !out || !aligned16(q) || !aligned16(out)) return SSD_ERR_INVALID_ARGUMENT;
-  const size_t need = paged_decode_workspace((int)requests, (int)table_width, (int)nheads, c.nkv, c.page_shift, c.D);
+  const size_t need = paged_decode_workspace((int)nheads, c.nkv, c.D);
   if (need && (workspace_bytes < need || !workspace)) return SSD_ERR_WORKSPACE_TOO_SMALL;
   if (need && !aligned16(workspace)) return SSD_ERR_INVALID_ARGUMENT;
   return cuda_status(launch_paged_decode(c, q, block_table, lengths, out, (int)requests, (int)table_width, (int)nheads,

@@ -115,7 +115,8 @@ cudaError_t launch_paged_append(const PagedCache& c, const void* k, const void* 
                                 long long v_hs, int dtype, cudaStream_t s);
 cudaError_t launch_paged_read(const PagedCache& c, const long long* slots, long long n, void* ko, void* vo, int dtype,
                               cudaStream_t s);
-size_t paged_decode_workspace(int R, int W, int Hq, int Hk, int page_shift, int D);
+unsigned int fetch_error_paged(cudaStream_t s);
+size_t paged_decode_workspace(int Hq, int Hk, int D);
 cudaError_t launch_paged_decode(const PagedCache& c, const void* q, const int* table, const int* lengths, void* out,
                                 int R, int W, int Hq, float scale, int dtype, void* workspace, cudaStream_t s);
 

@@ -8,11 +8,14 @@
 // The step reads every code once and computes 4 operations a code for each of the g = Hq / Hk
 // query heads that share it, so it should run at the memory's rate. What decides that is the
 // work between a code's arrival and its product; this layout keeps it low:
-//   - a warp takes 16 tokens at a time through its own ring of cp.async stages in shared memory
-//     (no barrier between warps, several KB in flight for each warp);
+//   - one warp of a CTA fetches (TMA, 16 tokens of K or V a box, a ring of stages of 64 tokens), four
+//     warps compute, 16 tokens of a stage each; the fetching warp runs ahead from one request to the
+//     next, so that memory stays busy where the others join their results;
 //   - both products are m16n8k16 tensor-core products with the codes as the 16-row operand A and
 //     up to 8 query heads as the 8 columns: S^T = K Q^T has tokens as rows, O^T = V^T P^T has
-//     dimensions as rows, so heads pad to 8 and not to 16. The codes become fp16 in registers, exactly
+//     dimensions as rows, so heads pad to 8 and not to 16 (tcgen05 would pad them to 16 columns too,
+//     but takes its 128-row operand from shared memory, where the codes would have to be written
+//     back as 16-bit values first). The codes become fp16 in registers, exactly
 //     (int8: a byte permute builds 1024 + code + 128, one subtraction; e4m3: a conversion);
 //   - within a product the contraction index and the rows of A may come in any order that both
 //     operands share. A lane takes 16 consecutive bytes of a token's K for four k-steps, and 16
@@ -24,7 +27,6 @@
 // offset by 2^7 so that products down to 2^-21 of the row's largest keep all bits. q enters
 // as fp16 after scaling its row by a power of two, which is exact for fp16 and for bf16 (8 bits)
 // down to 2^-29 of the row's largest element; an fp32 q and its P are split into two fp16 parts (22 bits).
-#include <cuda_pipeline_primitives.h>
 #include <math.h>
 
 #include <type_traits>
@@ -32,12 +34,18 @@
 #include "common.cuh"
 #include "kernels.h"
 #include "paged.cuh"
+#include "sm100.cuh"
+#include "tmap.cuh"
 
 namespace ssdb200 {
 namespace {
 
-constexpr int kDecWarps = 4;
-constexpr int kMinTiles = 8;       // 16-token tiles that a split has at least
+using namespace sm100;
+
+constexpr int kDecWarps = 4;                        // computing warps
+constexpr int kDecThreads = (kDecWarps + 1) * 32;   // and one that fetches
+constexpr int kMinTiles = 8;                        // 16-token tiles that a CTA's share has at least
+constexpr unsigned int kSiteDecLoad = 0x401, kSiteDecUse = 0x402;
 constexpr float kDecLog2e = 1.4426950408889634f;
 constexpr float kGrow = 8.0f;      // log2: O is rescaled when a row's maximum grows by more
 constexpr float kOffset = 7.0f;    // log2: P = 2^(s - m + 7) <= 2^15
@@ -84,457 +92,700 @@ __device__ __forceinline__ void expand4(uint32_t w, uint32_t& lo, uint32_t& hi) 
   }
 }
 
-// Where 16-byte chunk `ch` of token row `row` lies in a stage's K and V tile (bytes). The reads of
-// one 16-byte phase touch two rows x four chunks (K) and four row pairs x two chunks (V); the
-// exchanges below spread either over all banks.
-template <int D> __device__ __forceinline__ int k_at(int row, int ch) {
-  return row * D + ((D >= 128 ? ch ^ ((row & 1) << 2) : ch) << 4);
-}
-template <int D> __device__ __forceinline__ int v_at(int row, int ch) {
-  return row * D + ((D >= 128 ? ch ^ (((row >> 1) & 3) << 1) : (D == 64 ? ch ^ (((row >> 1) & 1) << 1) : ch)) << 4);
+// Where 16-byte chunk `ch` of token row `row` lies in a 16-token tile of K or V (bytes): rows of up
+// to 128 bytes, swizzled by the TMA; head_dim 256 is two tiles of 128 columns.
+template <int D> __device__ __forceinline__ int tile_at(int row, int ch) {
+  if constexpr (D >= 128) return (ch >> 3) * 2048 + row * 128 + (((ch & 7) ^ (row & 7)) << 4);
+  if constexpr (D == 64) return row * 64 + ((ch ^ ((row >> 1) & 3)) << 4);
+  return row * 32 + ((ch ^ ((row >> 2) & 1)) << 4);
 }
 
-template <int D> constexpr int dec_stages() { return D == 256 ? 3 : 4; }
-template <int D> constexpr int dec_stage_bytes() { return 32 * D + 128; }  // K, V, 16 gates, k_scale, v_scale
+template <int D> constexpr int dec_stages() { return D == 256 ? 2 : (D == 128 ? 3 : 4); }
+template <int D> constexpr int dec_stage_bytes() { return kDecWarps * 32 * D; }  // K tiles, V tiles
+constexpr int kInfoFloats = 24;                                                  // 16 gates, k_scale, v_scale, live
+// Results of two warps on their way to two others: m, l and O of a lane.
+template <int D, int NG> constexpr int dec_xchg_words() { return NG * (D / 16 * 4 + 4); }
 template <int D, int NG> constexpr size_t dec_smem() {
-  const size_t ring = (size_t)kDecWarps * dec_stages<D>() * dec_stage_bytes<D>();
-  const size_t merge = (size_t)kDecWarps * NG * 8 * (D + 2) * 4;
-  return ring > merge ? ring : merge;
+  return 1024 + (size_t)dec_stages<D>() * (dec_stage_bytes<D>() + kDecWarps * kInfoFloats * 4) +
+         2 * 32 * dec_xchg_words<D, NG>() * 4 + 128;
 }
 
 struct DecodeArgs {
   const void* q;
-  const unsigned char *kc, *vc;
   const float *ks, *vs, *gc;
   const int *table, *lengths;
   void* out;
-  float *part, *part_ml;  // (request, head, split) partial O and (m, l)
+  float *part, *part_ml;  // (2 parts of a CTA, 8 NG heads) partial O and (m, l)
   long long pages;
-  int W, Hq, Hk, g, page_shift, splits;
+  int R, W, Hq, Hk, g, ngrp, page_shift, ctas;
   float scale;
 };
 
-// Splits of a request that have work, and their tiles each.
-__device__ __forceinline__ int dec_split_tiles(int tiles, int splits) {
-  return max((tiles + splits - 1) / splits, kMinTiles);
-}
 __device__ __forceinline__ int dec_length(const DecodeArgs& a, int r) {
   return (int)min((long long)max(a.lengths[r], 0), (long long)a.W << a.page_shift);
 }
+__device__ __forceinline__ int dec_tiles(const DecodeArgs& a, int r) { return (dec_length(a, r) + 15) >> 4; }
 
-// CTA = (split of the request's tokens, key head and group of 8 NG query heads, request).
+// All requests' tiles, request by request and, within one, row group by row group (a row group:
+// the up to 8 NG query heads that share one reading of a key head), are one line; CTA i works on
+// [i * per, (i + 1) * per) of it. So every CTA has the same share whatever the lengths are, and one
+// long request is spread over all of them. A row group that crosses from one CTA into the next
+// leaves a part in each, which paged_decode_join_kernel joins in their order.
+__device__ __forceinline__ long long dec_share(long long units, int ctas) {
+  const long long per = (units + ctas - 1) / ctas;
+  return per < kMinTiles ? kMinTiles : per;
+}
+
+// Called by a whole CTA of N threads: the tiles of all requests (returned), and those before
+// request `upto` (before). sums: 2 * N / 32 words of shared memory.
+template <int N>
+__device__ __forceinline__ long long dec_count(const DecodeArgs& a, int upto, long long& before, long long* sums) {
+  const int tid = threadIdx.x;
+  long long all = 0, pre = 0;
+  for (int r = tid; r < a.R; r += N) {
+    const int t = dec_tiles(a, r);
+    all += t;
+    if (r < upto) pre += t;
+  }
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) {
+    all += __shfl_xor_sync(0xffffffffu, all, off);
+    pre += __shfl_xor_sync(0xffffffffu, pre, off);
+  }
+  if ((tid & 31) == 0) sums[tid >> 5] = all, sums[N / 32 + (tid >> 5)] = pre;
+  __syncthreads();
+  all = pre = 0;
+#pragma unroll
+  for (int w = 0; w < N / 32; ++w) all += sums[w], pre += sums[N / 32 + w];
+  before = pre;
+  return all;
+}
+
+// (kept in step with dec_ctas, which sizes the workspace)
+template <int D, int NG> constexpr int dec_ctas_per_sm() {
+  return D == 256 || NG == 2 ? 2 : (D == 128 ? 3 : 4);
+}
+
+// A run of tiles of one row group.
+struct DecSegment {
+  int r, n, tiles, group, first, last;
+};
+// The segment at `at` of the line, r and r_at (the request and its first tile on the line) moved on to it.
+__device__ __forceinline__ DecSegment dec_segment(const DecodeArgs& a, int groups, long long at, long long end, int& r,
+                                                  long long& r_at) {
+  DecSegment s;
+  for (;;) {
+    s.n = dec_length(a, r);
+    s.tiles = (s.n + 15) >> 4;
+    const long long all = (long long)s.tiles * groups;
+    if (at < r_at + all) break;
+    r_at += all;
+    ++r;
+  }
+  s.r = r;
+  const long long in = at - r_at;
+  s.group = (int)(in / s.tiles);
+  s.first = (int)(in - (long long)s.group * s.tiles);
+  s.last = (int)min((long long)s.tiles, s.first + (end - at));
+  return s;
+}
+
 template <typename T, typename C, int D, int NG>
-__global__ void __launch_bounds__(kDecWarps * 32, (NG == 2 || D == 256 || std::is_same<T, float>::value) ? 2 : 3)
-    paged_decode_kernel(const DecodeArgs a) {
+__global__ void __launch_bounds__(kDecThreads, dec_ctas_per_sm<D, NG>())
+    paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                        const DecodeArgs a) {
   constexpr bool SPLIT = std::is_same<T, float>::value;
-  constexpr int NST = dec_stages<D>(), STAGE = dec_stage_bytes<D>();
+  constexpr int NST = dec_stages<D>(), STAGE = dec_stage_bytes<D>(), TILE = 16 * D;
   constexpr int KW = D / 16;                 // K words of a lane and row = k-steps
   constexpr int MT = D / 16;                 // 16-row tiles of O^T
   constexpr int VWORDS = D / 32;             // V words of a lane and token
-  constexpr int CPR = D / 16;                // 16-byte chunks of a row
-  extern __shared__ __align__(16) unsigned char dsm[];
-  const int r = blockIdx.z, split = blockIdx.x;
-  const int ngrp = (a.g + 8 * NG - 1) / (8 * NG);
-  const int hk = blockIdx.y / ngrp, hg = blockIdx.y - hk * ngrp;
+  extern __shared__ uint8_t dsm_raw[];
+  __shared__ long long s_sums[2 * (kDecWarps + 1)];
+  __shared__ int s_req;
+  __shared__ long long s_at;
+  uint8_t* ring = align1024_shared(dsm_raw);
+  float* infos = reinterpret_cast<float*>(ring + NST * STAGE);
+  float* xchg = infos + NST * kDecWarps * kInfoFloats;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(xchg + 2 * 32 * dec_xchg_words<D, NG>());
+  auto full = [&](int s) { return smem_u32(&bars[s]); };
+  auto empty = [&](int s) { return smem_u32(&bars[NST + s]); };
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, lr = lane >> 2, lc = lane & 3;
-  const int n = dec_length(a, r);
-  const int tiles = (n + 15) >> 4, per = dec_split_tiles(tiles, a.splits);
-  const int first = split * per, last = min(first + per, tiles);
-  const int h0 = hk * a.g + hg * 8 * NG, nh = min(a.g - hg * 8 * NG, 8 * NG);
   T* out = reinterpret_cast<T*>(a.out);
-  if (n == 0 && split == 0) {
-    for (int i = tid; i < nh * D; i += kDecWarps * 32) out[((long long)r * a.Hq + h0) * D + i] = from_f32<T>(0.f);
+  asm volatile("griddepcontrol.launch_dependents;");  // the join may be put in place now (it waits for this grid)
+  if (tid == 0) {
+    prefetch_tmap(&tm_k);
+    prefetch_tmap(&tm_v);
+#pragma unroll
+    for (int i = 0; i < NST; ++i) {
+      mbar_init(full(i), 1);
+      mbar_init(empty(i), kDecWarps);
+    }
+    fence_mbar_init();
   }
-  if (first >= last) return;
-
-  // q as the B operand of S^T: lane (lr, lc) holds head lr, dimensions of its k slots
-  uint32_t qb[NG][KW][2], ql[SPLIT ? NG : 1][SPLIT ? KW : 1][2];
-  float qf[NG][2];  // per score column 2 lc, 2 lc + 1: scale * log2(e) / the row's power of two
+  const int groups = a.Hk * a.ngrp;
+  long long unused;
+  const long long units = dec_count<kDecThreads>(a, 0, unused, s_sums) * groups;
+  const long long per = dec_share(units, (int)gridDim.x);
+  const long long begin = blockIdx.x * per, end = min(begin + per, units);
+  for (int r = blockIdx.x; r < a.R; r += gridDim.x) {  // requests without tokens
+    if (dec_length(a, r) == 0)
+      for (int i = tid; i < a.Hq * D; i += kDecThreads) out[(long long)r * a.Hq * D + i] = from_f32<T>(0.f);
+  }
+  if (begin >= end) return;
+  // the request that holds tile `begin` of the line, by a scan of one warp
+  if (warp == 0) {
+    long long base = 0;
+    for (int r0 = 0; r0 < a.R; r0 += 32) {
+      const int t = r0 + lane < a.R ? dec_tiles(a, r0 + lane) : 0;
+      long long incl = (long long)t * groups;
 #pragma unroll
-  for (int x = 0; x < NG; ++x) {
-    const int h = 8 * x + lr;
-    const T* qp = reinterpret_cast<const T*>(a.q) + ((long long)r * a.Hq + h0 + h) * D;
-    float v[KW][4], m = 0.f;
-#pragma unroll
-    for (int k = 0; k < KW; ++k) {
-      const int d = D == 32 ? 8 * lc + 4 * k : 64 * (k >> 2) + 16 * lc + 4 * (k & 3);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        v[k][e] = h < nh ? to_f32<T>(qp[d + e]) : 0.f;
-        m = fmaxf(m, fabsf(v[k][e]));
+      for (int off = 1; off < 32; off <<= 1) {
+        const long long x = __shfl_up_sync(0xffffffffu, incl, off);
+        if (lane >= off) incl += x;
       }
+      const long long hi = base + incl, lo = hi - (long long)t * groups;
+      if (lo <= begin && begin < hi) s_req = r0 + lane, s_at = lo;
+      base = __shfl_sync(0xffffffffu, hi, 31);
+      if (base > begin) break;
     }
-    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-    // the largest element goes to [2^14, 2^15); fp16 queries need no scaling
-    float up = 1.f, down = 1.f;
-    if (!std::is_same<T, __half>::value && m > 0.f && m < INFINITY) {
-      const int e = min(max(14 - ilogbf(m), -126), 126);
-      up = ldexpf(1.f, e);
-      down = ldexpf(1.f, -e);
-    }
-#pragma unroll
-    for (int k = 0; k < KW; ++k) {
-#pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        const float x0 = v[k][2 * b] * up, x1 = v[k][2 * b + 1] * up;
-        qb[x][k][b] = half2_bits(x0, x1);
-        if constexpr (SPLIT) {
-          const float2 hi = __half22float2(*reinterpret_cast<const __half2*>(&qb[x][k][b]));
-          ql[x][k][b] = half2_bits(x0 - hi.x, x1 - hi.y);
+  }
+  __syncthreads();
+  int r = s_req;
+  long long r_at = s_at;
+  int step = 0;  // stages used so far
+  const int tiles_page = a.page_shift - 4;  // log2 of a page's tiles
+
+  if (warp == kDecWarps) {
+    // ---------------------------------------------------------------- fetch
+    // Lanes take the four tiles of a stage in turn: lanes 0-3 their K, 4-7 V, 8-11 gates, 12-15 scales,
+    // 16-23 the second column halves of head_dim 256. Page numbers and scales come 32 tiles at a time,
+    // one batch ahead.
+    bool dead = false;
+    for (long long at = begin; at < end;) {
+      const DecSegment sg = dec_segment(a, groups, at, end, r, r_at);
+      const int hk = sg.group / a.ngrp;
+      const int* row = a.table + (long long)sg.r * a.W;
+      auto page_of = [&](int t) { return t < sg.last ? row[t >> tiles_page] : -1; };
+      auto valid = [&](int id) { return id >= 0 && id < a.pages; };
+      int id = page_of(sg.first + lane), id_next = -1;
+      float ksc = 0.f, vsc = 0.f, ksc_next = 0.f, vsc_next = 0.f;
+      if (valid(id)) ksc = a.ks[(long long)id * a.Hk + hk], vsc = a.vs[(long long)id * a.Hk + hk];
+      for (int t = sg.first, i = 0; t < sg.last; t += kDecWarps, ++i, ++step) {
+        const int in = i & 7;  // eight steps a batch
+        if (in == 0) {
+          if (i > 0) id = id_next, ksc = ksc_next, vsc = vsc_next;
+          id_next = page_of(t + 32 + lane);
+        } else if (in == 4) {
+          ksc_next = vsc_next = 0.f;
+          if (valid(id_next))
+            ksc_next = a.ks[(long long)id_next * a.Hk + hk], vsc_next = a.vs[(long long)id_next * a.Hk + hk];
+        }
+        const int st = step % NST, w = lane & 3, mt = t + w;
+        if (step >= NST && !dead) dead = !mbar_wait_sleep(empty(st), ((step / NST) - 1) & 1, kSiteDecLoad);
+        dead = __any_sync(0xffffffffu, dead);
+        const int my = __shfl_sync(0xffffffffu, id, 4 * in + w);
+        const float mk = __shfl_sync(0xffffffffu, ksc, 4 * in + w), mv = __shfl_sync(0xffffffffu, vsc, 4 * in + w);
+        const bool live = mt < sg.last && valid(my) && !dead;
+        const long long ph = live ? (long long)my * a.Hk + hk : 0;
+        const int row0 = (mt & ((1 << tiles_page) - 1)) << 4;
+        float* info = infos + (st * kDecWarps + w) * kInfoFloats;
+        const int role = lane >> 2;
+        if (role == 3) info[16] = mk, info[17] = mv, info[18] = live ? 1.f : 0.f;
+        const int n_live = __popc(__ballot_sync(0xffffffffu, live) & 0xfu);
+        __syncwarp();
+        if (lane == 0) mbar_expect_tx(full(st), (uint32_t)(n_live * (2 * TILE + (a.gc ? 64 : 0))));
+        __syncwarp();
+        if (live) {
+          const uint32_t kd = smem_u32(ring + st * STAGE + w * TILE), vd = kd + kDecWarps * TILE;
+          if (role == 0) tma_load_3d(kd, &tm_k, 0, row0, (int)ph, full(st));
+          if (role == 1) tma_load_3d(vd, &tm_v, 0, row0, (int)ph, full(st));
+          if (role == 2 && a.gc) bulk_load(smem_u32(info), a.gc + (ph << a.page_shift) + row0, 64, full(st));
+          if (D == 256 && role == 4) tma_load_3d(kd + 2048, &tm_k, 128, row0, (int)ph, full(st));
+          if (D == 256 && role == 5) tma_load_3d(vd + 2048, &tm_v, 128, row0, (int)ph, full(st));
         }
       }
+      at += sg.last - sg.first;
     }
-    const float f = a.scale * kDecLog2e * down;
-    qf[x][0] = __shfl_sync(0xffffffffu, f, (2 * lc) * 4);
-    qf[x][1] = __shfl_sync(0xffffffffu, f, (2 * lc + 1) * 4);
+    // no copy may be in flight when the CTA exits
+    if (lane == 0)
+      for (int d = 1; d <= NST && d <= step; ++d)
+        mbar_wait(full((step - d) % NST), ((step - d) / NST) & 1, kSiteDecLoad);
+    return;
   }
 
-  unsigned char* ring = dsm + warp * NST * STAGE;
-  const int mine = (last - first - warp + kDecWarps - 1) / kDecWarps;  // this warp's tiles
-  const int tiles_page = a.page_shift - 4;                              // log2 of a page's tiles
-  int ids = -1;  // page of tile `lane` of the current 32
-  auto issue = [&](int it) {
-    if ((it & 31) == 0) {
-      const int t = first + warp + (it + lane) * kDecWarps;
-      ids = t < last ? a.table[(long long)r * a.W + (t >> tiles_page)] : -1;
-    }
-    const int id = __shfl_sync(0xffffffffu, ids, it & 31);
-    if (it < mine) {
-      const int t = first + warp + it * kDecWarps;
-      unsigned char* st = ring + (it % NST) * STAGE;
-      float* info = reinterpret_cast<float*>(st + 32 * D);
-      const bool ok = id >= 0 && id < a.pages;
-      const long long ph = ok ? (long long)id * a.Hk + hk : 0;
-      const int row0 = (t & ((1 << tiles_page) - 1)) << 4;
-      const long long tok = (ph << a.page_shift) + row0;
-      const size_t zero = ok ? 0 : 16;
-#pragma unroll
-      for (int i = 0; i < D / 32; ++i) {
-        const int c = lane + 32 * i, row = c / CPR, ch = c % CPR;
-        __pipeline_memcpy_async(st + k_at<D>(row, ch), a.kc + tok * D + c * 16, 16, zero);
-        __pipeline_memcpy_async(st + 16 * D + v_at<D>(row, ch), a.vc + tok * D + c * 16, 16, zero);
-      }
-      if (lane < 4) {
-        // without gates the 16 floats are unused
-        if (a.gc) __pipeline_memcpy_async(info + 4 * lane, a.gc + tok + 4 * lane, 16, zero);
-      } else if (lane == 4) {
-        __pipeline_memcpy_async(info + 16, a.ks + ph, 4, ok ? 0 : 4);
-      } else if (lane == 5) {
-        __pipeline_memcpy_async(info + 17, a.vs + ph, 4, ok ? 0 : 4);
-      } else if (lane == 6) {
-        info[18] = ok ? 1.f : 0.f;
-      }
-    }
-    __pipeline_commit();
-  };
+  // ------------------------------------------------------------------ compute
+  // A wait that ran out sets the error flag; the warp then waits for no more stages but takes every step,
+  // so that the barriers below always have their warps.
+  bool dead = false;
+  for (long long at = begin; at < end;) {
+    const DecSegment sg = dec_segment(a, groups, at, end, r, r_at);
+    const int hk = sg.group / a.ngrp, hg = sg.group - hk * a.ngrp;
+    const int h0 = hk * a.g + hg * 8 * NG, nh = min(a.g - hg * 8 * NG, 8 * NG);
+    const int n = sg.n;
 
-  float o[NG][MT][4], m[NG][2], l[NG][2], unit = 0.f;  // O in units of the v_scale `unit`
-#pragma unroll
-  for (int x = 0; x < NG; ++x) {
-    m[x][0] = m[x][1] = -INFINITY;
-    l[x][0] = l[x][1] = 0.f;
-#pragma unroll
-    for (int i = 0; i < MT; ++i) o[x][i][0] = o[x][i][1] = o[x][i][2] = o[x][i][3] = 0.f;
-  }
-#pragma unroll
-  for (int i = 0; i < NST - 1; ++i) issue(i);
-  for (int it = 0; it < mine; ++it) {
-    __pipeline_wait_prior(NST - 2);
-    __syncwarp();
-    issue(it + NST - 1);  // into the stage that the whole warp has read in the last step
-    const unsigned char* st = ring + (it % NST) * STAGE;
-    const float* info = reinterpret_cast<const float*>(st + 32 * D);
-    const int t0 = (first + warp + it * kDecWarps) * 16 + lr, t1 = t0 + 8;
-    // ---- S^T = K Q^T
-    float s[NG][4], s2[NG][4];
-#pragma unroll
-    for (int x = 0; x < NG; ++x)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) s[x][e] = s2[x][e] = 0.f;
-    uint32_t kw[2][KW];
-#pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      if constexpr (D == 32) {
-        const uint2 w = *reinterpret_cast<const uint2*>(st + (lr + 8 * b) * D + lc * 8);
-        kw[b][0] = w.x, kw[b][1] = w.y;
-      } else {
-#pragma unroll
-        for (int j = 0; j < D / 64; ++j) {
-          const uint4 w = *reinterpret_cast<const uint4*>(st + k_at<D>(lr + 8 * b, lc + 4 * j));
-          kw[b][4 * j] = w.x, kw[b][4 * j + 1] = w.y, kw[b][4 * j + 2] = w.z, kw[b][4 * j + 3] = w.w;
-        }
-      }
-    }
-#pragma unroll
-    for (int k = 0; k < KW; ++k) {
-      uint32_t a0, a1, a2, a3;
-      expand4<C>(kw[0][k], a0, a2);
-      expand4<C>(kw[1][k], a1, a3);
-#pragma unroll
-      for (int x = 0; x < NG; ++x) {
-        mma16816(k & 1 ? s2[x] : s[x], a0, a1, a2, a3, qb[x][k][0], qb[x][k][1]);
-        if constexpr (SPLIT) mma16816(k & 1 ? s[x] : s2[x], a0, a1, a2, a3, ql[x][k][0], ql[x][k][1]);
-      }
-    }
-    // ---- scores in log2 units
-    const float ksc = info[16], vsc = info[17];
-    bool in0 = t0 < n, in1 = t1 < n;
-    float g0 = 0.f, g1 = 0.f;
-    if (a.gc) {
-      g0 = t0 < n - 1 ? info[lr] * kDecLog2e : 0.f;
-      g1 = t1 < n - 1 ? info[lr + 8] * kDecLog2e : 0.f;
-      in0 = in0 && g0 != -INFINITY;
-      in1 = in1 && g1 != -INFINITY;
-    }
-    const bool live = info[18] != 0.f;
-    in0 = in0 && live;
-    in1 = in1 && live;
-    bool grow = false;
-#pragma unroll
-    for (int x = 0; x < NG; ++x)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float y = fmaf(s[x][e] + s2[x][e], qf[x][e & 1] * ksc, e < 2 ? g0 : g1);
-        s[x][e] = (e < 2 ? in0 : in1) ? y : -INFINITY;
-        grow |= s[x][e] > m[x][e & 1] + kGrow;
-      }
-    if (__any_sync(0xffffffffu, grow)) {
-#pragma unroll
-      for (int x = 0; x < NG; ++x)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float t = fmaxf(s[x][e], s[x][e + 2]);
-          t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 4));
-          t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 8));
-          t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 16));
-          const float mn = fmaxf(m[x][e], t);
-          const float f = m[x][e] == -INFINITY ? 0.f : dec_ex2(m[x][e] - mn);
-          if (mn == m[x][e]) continue;  // (uniform over the lanes of a column: no collective below)
-          m[x][e] = mn;
-          l[x][e] *= f;
-#pragma unroll
-          for (int i = 0; i < MT; ++i) o[x][i][e] *= f, o[x][i][e + 2] *= f;
-        }
-    }
-    if (vsc > unit) {
-      const float f = unit / vsc;
-      unit = vsc;
-#pragma unroll
-      for (int x = 0; x < NG; ++x)
-#pragma unroll
-        for (int i = 0; i < MT; ++i)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[x][i][e] *= f;
-    }
-    const float ratio = unit > 0.f ? __fdividef(vsc, unit) : 0.f;
-    // ---- P, as the B operand of O^T (heads as columns, tokens as the contraction)
-    uint32_t pb[NG][2], pl[SPLIT ? NG : 1][2];
+    // q as the B operand of S^T: lane (lr, lc) holds head lr, dimensions of its k slots
+    uint32_t qb[NG][KW][2], ql[SPLIT ? NG : 1][SPLIT ? KW : 1][2];
+    float qf[NG][2];  // per score column 2 lc, 2 lc + 1: scale * log2(e) / the row's power of two
 #pragma unroll
     for (int x = 0; x < NG; ++x) {
-      const float m0 = m[x][0] == -INFINITY ? 0.f : m[x][0] - kOffset;
-      const float m1 = m[x][1] == -INFINITY ? 0.f : m[x][1] - kOffset;
-      float p[4];
+      const int h = 8 * x + lr;
+      const T* qp = reinterpret_cast<const T*>(a.q) + ((long long)sg.r * a.Hq + h0 + h) * D;
+      float v[KW][4], m = 0.f;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) p[e] = dec_ex2(s[x][e] - (e & 1 ? m1 : m0));
-      l[x][0] += p[0] + p[2];
-      l[x][1] += p[1] + p[3];
+      for (int k = 0; k < KW; ++k) {
+        const int d = D == 32 ? 8 * lc + 4 * k : 64 * (k >> 2) + 16 * lc + 4 * (k & 3);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          v[k][e] = h < nh ? to_f32<T>(qp[d + e]) : 0.f;
+          m = fmaxf(m, fabsf(v[k][e]));
+        }
+      }
+      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+      // the largest element goes to [2^14, 2^15); fp16 queries need no scaling
+      float up = 1.f, down = 1.f;
+      if (!std::is_same<T, __half>::value && m > 0.f && m < INFINITY) {
+        const int e = min(max(14 - ilogbf(m), -126), 126);
+        up = ldexpf(1.f, e);
+        down = ldexpf(1.f, -e);
+      }
+#pragma unroll
+      for (int k = 0; k < KW; ++k) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          const float x0 = v[k][2 * b] * up, x1 = v[k][2 * b + 1] * up;
+          qb[x][k][b] = half2_bits(x0, x1);
+          if constexpr (SPLIT) {
+            const float2 hi = __half22float2(*reinterpret_cast<const __half2*>(&qb[x][k][b]));
+            ql[x][k][b] = half2_bits(x0 - hi.x, x1 - hi.y);
+          }
+        }
+      }
+      const float f = a.scale * kDecLog2e * down;
+      qf[x][0] = __shfl_sync(0xffffffffu, f, (2 * lc) * 4);
+      qf[x][1] = __shfl_sync(0xffffffffu, f, (2 * lc + 1) * 4);
+    }
+
+    float o[NG][MT][4], m[NG][2], l[NG][2], unit = 0.f;  // O in units of the v_scale `unit`
+#pragma unroll
+    for (int x = 0; x < NG; ++x) {
+      m[x][0] = m[x][1] = -INFINITY;
+      l[x][0] = l[x][1] = 0.f;
+#pragma unroll
+      for (int i = 0; i < MT; ++i) o[x][i][0] = o[x][i][1] = o[x][i][2] = o[x][i][3] = 0.f;
+    }
+    for (int t = sg.first; t < sg.last; t += kDecWarps, ++step) {
+      const int st = step % NST;
+      if (!dead) dead = !__all_sync(0xffffffffu, mbar_wait_sleep(full(st), (step / NST) & 1, kSiteDecUse));
+      if (t + warp < sg.last) {
+      const uint8_t* kt = ring + st * STAGE + warp * TILE;
+      const uint8_t* vt = kt + kDecWarps * TILE;
+      const float* info = infos + (st * kDecWarps + warp) * kInfoFloats;
+      const int t0 = (t + warp) * 16 + lr, t1 = t0 + 8;
+      // ---- S^T = K Q^T
+      float s[NG][4], s2[NG][4];
+#pragma unroll
+      for (int x = 0; x < NG; ++x)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[x][e] = s2[x][e] = 0.f;
+      uint32_t kw[2][KW];
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
-        const float p0 = p[2 * b] * ratio, p1 = p[2 * b + 1] * ratio;
-        const uint32_t w = half2_bits(p0, p1);
-        pb[x][b] = transpose8x8(w);
-        if constexpr (SPLIT) {
-          const float2 hi = __half22float2(*reinterpret_cast<const __half2*>(&w));
-          pl[x][b] = transpose8x8(half2_bits(p0 - hi.x, p1 - hi.y));
+        if constexpr (D == 32) {
+          const uint2 w = *reinterpret_cast<const uint2*>(kt + tile_at<D>(lr + 8 * b, lc >> 1) + (lc & 1) * 8);
+          kw[b][0] = w.x, kw[b][1] = w.y;
+        } else {
+#pragma unroll
+          for (int j = 0; j < D / 64; ++j) {
+            const uint4 w = *reinterpret_cast<const uint4*>(kt + tile_at<D>(lr + 8 * b, lc + 4 * j));
+            kw[b][4 * j] = w.x, kw[b][4 * j + 1] = w.y, kw[b][4 * j + 2] = w.z, kw[b][4 * j + 3] = w.w;
+          }
         }
       }
-    }
-    // ---- O^T += V^T P^T
-    uint32_t vw[4][VWORDS];  // tokens 2 lc, 2 lc + 1, 2 lc + 8, 2 lc + 9
 #pragma unroll
-    for (int b = 0; b < 4; ++b) {
-      const int row = 2 * lc + (b & 1) + (b >> 1) * 8;
-      const unsigned char* vp = st + 16 * D;
-      if constexpr (D == 32) {
-        vw[b][0] = *reinterpret_cast<const uint32_t*>(vp + row * D + lr * 4);
-      } else if constexpr (D == 64) {
-        const uint2 w = *reinterpret_cast<const uint2*>(vp + v_at<D>(row, lr >> 1) + (lr & 1) * 8);
-        vw[b][0] = w.x, vw[b][1] = w.y;
-      } else {
-#pragma unroll
-        for (int j = 0; j < D / 128; ++j) {
-          const uint4 w = *reinterpret_cast<const uint4*>(vp + v_at<D>(row, lr + 8 * j));
-          vw[b][4 * j] = w.x, vw[b][4 * j + 1] = w.y, vw[b][4 * j + 2] = w.z, vw[b][4 * j + 3] = w.w;
-        }
-      }
-    }
-    if constexpr (std::is_same<C, E4M3>::value) {
-      // a NaN code of a token that does not count must not meet its zero weight
-      const unsigned b0 = __ballot_sync(0xffffffffu, in0), b1 = __ballot_sync(0xffffffffu, in1);
-      if ((b0 & b1) != 0xffffffffu) {
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          const bool in = ((b < 2 ? b0 : b1) >> (4 * (2 * lc + (b & 1)))) & 1u;
-#pragma unroll
-          for (int j = 0; j < VWORDS; ++j) vw[b][j] = in ? vw[b][j] : 0u;
-        }
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < VWORDS; ++j) {
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const uint32_t sel = half ? 0x7362 : 0x5140;
+      for (int k = 0; k < KW; ++k) {
         uint32_t a0, a1, a2, a3;
-        expand4<C>(__byte_perm(vw[0][j], vw[1][j], sel), a0, a1);
-        expand4<C>(__byte_perm(vw[2][j], vw[3][j], sel), a2, a3);
+        expand4<C>(kw[0][k], a0, a2);
+        expand4<C>(kw[1][k], a1, a3);
 #pragma unroll
         for (int x = 0; x < NG; ++x) {
-          mma16816(o[x][2 * j + half], a0, a1, a2, a3, pb[x][0], pb[x][1]);
-          if constexpr (SPLIT) mma16816(o[x][2 * j + half], a0, a1, a2, a3, pl[x][0], pl[x][1]);
+          mma16816(k & 1 ? s2[x] : s[x], a0, a1, a2, a3, qb[x][k][0], qb[x][k][1]);
+          if constexpr (SPLIT) mma16816(k & 1 ? s[x] : s2[x], a0, a1, a2, a3, ql[x][k][0], ql[x][k][1]);
         }
       }
+      // ---- scores in log2 units
+      const float ksc = info[16], vsc = info[17];
+      bool in0 = t0 < n, in1 = t1 < n;
+      float g0 = 0.f, g1 = 0.f;
+      if (a.gc) {
+        g0 = t0 < n - 1 ? info[lr] * kDecLog2e : 0.f;
+        g1 = t1 < n - 1 ? info[lr + 8] * kDecLog2e : 0.f;
+        in0 = in0 && g0 != -INFINITY;
+        in1 = in1 && g1 != -INFINITY;
+      }
+      const bool live = info[18] != 0.f;
+      in0 = in0 && live;
+      in1 = in1 && live;
+      bool grow = false;
+#pragma unroll
+      for (int x = 0; x < NG; ++x)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float y = fmaf(s[x][e] + s2[x][e], qf[x][e & 1] * ksc, e < 2 ? g0 : g1);
+          s[x][e] = (e < 2 ? in0 : in1) ? y : -INFINITY;
+          grow |= s[x][e] > m[x][e & 1] + kGrow;
+        }
+      if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+        for (int x = 0; x < NG; ++x)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float t = fmaxf(s[x][e], s[x][e + 2]);
+            t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 4));
+            t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 8));
+            t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 16));
+            const float mn = fmaxf(m[x][e], t);
+            const float f = m[x][e] == -INFINITY ? 0.f : dec_ex2(m[x][e] - mn);
+            if (mn == m[x][e]) continue;  // (uniform over the lanes of a column: no collective below)
+            m[x][e] = mn;
+            l[x][e] *= f;
+#pragma unroll
+            for (int i = 0; i < MT; ++i) o[x][i][e] *= f, o[x][i][e + 2] *= f;
+          }
+      }
+      if (vsc > unit) {
+        const float f = unit / vsc;
+        unit = vsc;
+#pragma unroll
+        for (int x = 0; x < NG; ++x)
+#pragma unroll
+          for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[x][i][e] *= f;
+      }
+      const float ratio = unit > 0.f ? __fdividef(vsc, unit) : 0.f;
+      // ---- P, as the B operand of O^T (heads as columns, tokens as the contraction)
+      uint32_t pb[NG][2], pl[SPLIT ? NG : 1][2];
+#pragma unroll
+      for (int x = 0; x < NG; ++x) {
+        const float m0 = m[x][0] == -INFINITY ? 0.f : m[x][0] - kOffset;
+        const float m1 = m[x][1] == -INFINITY ? 0.f : m[x][1] - kOffset;
+        float p[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) p[e] = dec_ex2(s[x][e] - (e & 1 ? m1 : m0));
+        l[x][0] += p[0] + p[2];
+        l[x][1] += p[1] + p[3];
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          const float p0 = p[2 * b] * ratio, p1 = p[2 * b + 1] * ratio;
+          const uint32_t w = half2_bits(p0, p1);
+          pb[x][b] = transpose8x8(w);
+          if constexpr (SPLIT) {
+            const float2 hi = __half22float2(*reinterpret_cast<const __half2*>(&w));
+            pl[x][b] = transpose8x8(half2_bits(p0 - hi.x, p1 - hi.y));
+          }
+        }
+      }
+      // ---- O^T += V^T P^T
+      uint32_t vw[4][VWORDS];  // tokens 2 lc, 2 lc + 1, 2 lc + 8, 2 lc + 9
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        const int row = 2 * lc + (b & 1) + (b >> 1) * 8;
+        if constexpr (D == 32) {
+          vw[b][0] = *reinterpret_cast<const uint32_t*>(vt + tile_at<D>(row, lr >> 2) + (lr & 3) * 4);
+        } else if constexpr (D == 64) {
+          const uint2 w = *reinterpret_cast<const uint2*>(vt + tile_at<D>(row, lr >> 1) + (lr & 1) * 8);
+          vw[b][0] = w.x, vw[b][1] = w.y;
+        } else {
+#pragma unroll
+          for (int j = 0; j < D / 128; ++j) {
+            const uint4 w = *reinterpret_cast<const uint4*>(vt + tile_at<D>(row, lr + 8 * j));
+            vw[b][4 * j] = w.x, vw[b][4 * j + 1] = w.y, vw[b][4 * j + 2] = w.z, vw[b][4 * j + 3] = w.w;
+          }
+        }
+      }
+      if constexpr (std::is_same<C, E4M3>::value) {
+        // a NaN code of a token that does not count must not meet its zero weight
+        const unsigned b0 = __ballot_sync(0xffffffffu, in0), b1 = __ballot_sync(0xffffffffu, in1);
+        if ((b0 & b1) != 0xffffffffu) {
+#pragma unroll
+          for (int b = 0; b < 4; ++b) {
+            const bool in = ((b < 2 ? b0 : b1) >> (4 * (2 * lc + (b & 1)))) & 1u;
+#pragma unroll
+            for (int j = 0; j < VWORDS; ++j) vw[b][j] = in ? vw[b][j] : 0u;
+          }
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < VWORDS; ++j) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const uint32_t sel = half ? 0x7362 : 0x5140;
+          uint32_t a0, a1, a2, a3;
+          expand4<C>(__byte_perm(vw[0][j], vw[1][j], sel), a0, a1);
+          expand4<C>(__byte_perm(vw[2][j], vw[3][j], sel), a2, a3);
+#pragma unroll
+          for (int x = 0; x < NG; ++x) {
+            mma16816(o[x][2 * j + half], a0, a1, a2, a3, pb[x][0], pb[x][1]);
+            if constexpr (SPLIT) mma16816(o[x][2 * j + half], a0, a1, a2, a3, pl[x][0], pl[x][1]);
+          }
+        }
+      }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(empty(st));
     }
-  }
-  __pipeline_wait_prior(0);
-  __syncthreads();  // the ring becomes the warps' results
 
-  // ---- merge the warps
-  float* so = reinterpret_cast<float*>(dsm);                    // [warp][head][D]
-  float* sml = so + kDecWarps * NG * 8 * D;                     // [warp][head][2]
+    // ---- join the warps: 2 and 3 hand their results to 0 and 1, then 1 to 0; lanes hold the same places
 #pragma unroll
-  for (int x = 0; x < NG; ++x)
+    for (int x = 0; x < NG; ++x)
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      float t = l[x][e];
-      t += __shfl_xor_sync(0xffffffffu, t, 4);
-      t += __shfl_xor_sync(0xffffffffu, t, 8);
-      t += __shfl_xor_sync(0xffffffffu, t, 16);
-      const int h = warp * NG * 8 + 8 * x + 2 * lc + e;
-      if (lr == 0) sml[2 * h] = m[x][e], sml[2 * h + 1] = t;
+      for (int e = 0; e < 2; ++e) {
+        l[x][e] += __shfl_xor_sync(0xffffffffu, l[x][e], 4);
+        l[x][e] += __shfl_xor_sync(0xffffffffu, l[x][e], 8);
+        l[x][e] += __shfl_xor_sync(0xffffffffu, l[x][e], 16);
 #pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        const int d = D == 32 ? 4 * lr + 2 * i : (D == 64 ? 8 * lr + 2 * i : 128 * (i >> 3) + 16 * lr + 2 * (i & 7));
-        *reinterpret_cast<float2*>(so + h * D + d) = make_float2(o[x][i][e] * unit, o[x][i][e + 2] * unit);
+        for (int i = 0; i < MT; ++i) o[x][i][e] *= unit, o[x][i][e + 2] *= unit;
+      }
+    auto put = [&](float* to) {
+      float4* p = reinterpret_cast<float4*>(to) + lane;
+#pragma unroll
+      for (int x = 0; x < NG; ++x) {
+        *p = make_float4(m[x][0], m[x][1], l[x][0], l[x][1]);
+        p += 32;
+#pragma unroll
+        for (int i = 0; i < MT; ++i, p += 32) *p = make_float4(o[x][i][0], o[x][i][1], o[x][i][2], o[x][i][3]);
+      }
+    };
+    auto take = [&](const float* from) {
+      const float4* p = reinterpret_cast<const float4*>(from) + lane;
+#pragma unroll
+      for (int x = 0; x < NG; ++x) {
+        const float4 ml = *p;
+        p += 32;
+        const float n0 = fmaxf(m[x][0], ml.x), n1 = fmaxf(m[x][1], ml.y);
+        const float f0 = m[x][0] == -INFINITY ? 0.f : dec_ex2(m[x][0] - n0), g0 = ml.x == -INFINITY ? 0.f : dec_ex2(ml.x - n0);
+        const float f1 = m[x][1] == -INFINITY ? 0.f : dec_ex2(m[x][1] - n1), g1 = ml.y == -INFINITY ? 0.f : dec_ex2(ml.y - n1);
+        m[x][0] = n0, m[x][1] = n1;
+        l[x][0] = l[x][0] * f0 + ml.z * g0;  // (a NaN stays one, also times 0)
+        l[x][1] = l[x][1] * f1 + ml.w * g1;
+#pragma unroll
+        for (int i = 0; i < MT; ++i, p += 32) {
+          const float4 y = *p;
+          o[x][i][0] = o[x][i][0] * f0 + y.x * g0;
+          o[x][i][1] = o[x][i][1] * f1 + y.y * g1;
+          o[x][i][2] = o[x][i][2] * f0 + y.z * g0;
+          o[x][i][3] = o[x][i][3] * f1 + y.w * g1;
+        }
+      }
+    };
+    float* x0 = xchg + (warp & 1) * 32 * dec_xchg_words<D, NG>();
+    named_bar_sync(1, kDecWarps * 32);  // the last segment's results have been taken
+    if (warp >= 2) put(x0);
+    named_bar_sync(1, kDecWarps * 32);
+    if (warp < 2) {
+      take(x0);
+      if (warp == 1) put(x0);
+      named_bar_sync(2, 64);
+      if (warp == 0) {
+        take(xchg + 32 * dec_xchg_words<D, NG>());
+        const bool whole = sg.first == 0 && sg.last == sg.tiles;
+        // parts of a row group: the first of a CTA's share in place 0, a later one (its last) in place 1
+        const long long part = (2ll * blockIdx.x + (at == begin ? 0 : 1)) * (8 * NG);
+#pragma unroll
+        for (int x = 0; x < NG; ++x)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int h = 8 * x + 2 * lc + e;
+            if (h >= nh) continue;
+            const float inv = 1.0f / l[x][e];
+            constexpr int RUN = D >= 128 ? 8 : MT;  // row pairs of consecutive dimensions
+#pragma unroll
+            for (int i0 = 0; i0 < MT; i0 += RUN) {
+              const int d0 = (i0 ? 128 : 0) + 2 * RUN * lr;
+              if (whole) {
+                T* op = out + ((long long)sg.r * a.Hq + h0 + h) * D + d0;
+#pragma unroll
+                for (int i = 0; i < RUN; ++i) {
+                  const float y0 = o[x][i0 + i][e] * inv, y1 = o[x][i0 + i][e + 2] * inv;
+                  if constexpr (SPLIT) {
+                    *reinterpret_cast<float2*>(op + 2 * i) = make_float2(y0, y1);
+                  } else {
+                    *reinterpret_cast<uint32_t*>(op + 2 * i) = pack2<T>(y0, y1);
+                  }
+                }
+              } else {
+                float* op = a.part + (part + h) * D + d0;
+#pragma unroll
+                for (int i = 0; i < RUN; ++i)
+                  *reinterpret_cast<float2*>(op + 2 * i) = make_float2(o[x][i0 + i][e], o[x][i0 + i][e + 2]);
+              }
+            }
+            if (!whole && lr == 0)
+              *reinterpret_cast<float2*>(a.part_ml + 2 * (part + h)) = make_float2(m[x][e], l[x][e]);
+          }
       }
     }
-  __syncthreads();
-  const bool whole = per >= tiles;  // this split is all of the request
-  for (int i = tid; i < nh * D; i += kDecWarps * 32) {
-    const int h = i / D, d = i - h * D;
-    float mm = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < kDecWarps; ++w) mm = fmaxf(mm, sml[2 * (w * NG * 8 + h)]);
-    float acc = 0.f, ll = 0.f;
-#pragma unroll
-    for (int w = 0; w < kDecWarps; ++w) {
-      const float mw = sml[2 * (w * NG * 8 + h)];
-      const float f = mw == -INFINITY ? 0.f : dec_ex2(mw - mm);
-      ll = fmaf(sml[2 * (w * NG * 8 + h) + 1], f, ll);  // (a NaN stays one)
-      acc = fmaf(so[(w * NG * 8 + h) * D + d], f, acc);
-    }
-    const long long row = (long long)r * a.Hq + h0 + h;
-    if (whole) {
-      out[row * D + d] = from_f32<T>(acc / ll);
-    } else {
-      a.part[(row * a.splits + split) * D + d] = acc;
-      if (d == 0) {
-        a.part_ml[2 * (row * a.splits + split)] = mm;
-        a.part_ml[2 * (row * a.splits + split) + 1] = ll;
-      }
-    }
+    at += sg.last - sg.first;
   }
 }
 
-// Joins the splits of a request; thread = dimension.
-template <typename T>
-__global__ void paged_decode_join_kernel(const DecodeArgs a, int D) {
-  const int h = blockIdx.x, r = blockIdx.y, d = threadIdx.x;
-  const int tiles = (dec_length(a, r) + 15) >> 4, per = dec_split_tiles(tiles, a.splits);
-  if (per >= tiles) return;
-  const int used = (tiles + per - 1) / per;
-  const long long row = (long long)r * a.Hq + h;
-  const float* ml = a.part_ml + 2 * row * a.splits;
-  const float* p = a.part + row * a.splits * D + d;
-  float mm = -INFINITY, ll = 0.f, acc = 0.f;
-  for (int s = 0; s < used; ++s) mm = fmaxf(mm, ml[2 * s]);
+// Joins the parts of the row groups that several CTAs worked on. CTA = (request, query head); a warp
+// takes every kJoinWarps-th part, a lane four dimensions.
+constexpr int kJoinWarps = 8;
+
+template <typename T, int D, int NG>
+__global__ void __launch_bounds__(kJoinWarps * 32) paged_decode_join_kernel(const DecodeArgs a) {
+  constexpr int VEC = D >= 128 ? 4 : D / 32, COLS = D / (32 * VEC);  // D = 32: 1 x 1, 64: 2 x 1, 128: 4 x 1, 256: 4 x 2
+  __shared__ long long s_sums[2 * kJoinWarps];
+  __shared__ float s_m[kJoinWarps], s_l[kJoinWarps];
+  __shared__ __align__(16) float s_o[kJoinWarps][D];
+  const int h = blockIdx.x, r = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tiles = dec_tiles(a, r);
+  const int hk = h / a.g, hg = (h - hk * a.g) / (8 * NG), groups = a.Hk * a.ngrp;
+  long long before;
+  const long long units = dec_count<kJoinWarps * 32>(a, r, before, s_sums) * groups;
+  const long long per = dec_share(units, a.ctas);
+  const long long lo = before * groups + (long long)(hk * a.ngrp + hg) * tiles, hi = lo + tiles;
+  const int c0 = (int)(lo / per), c1 = (int)((hi - 1) / per);
+  const int hl = h - hk * a.g - hg * 8 * NG;
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // every CTA waits: this grid must not end before the first one
+  if (tiles == 0 || c0 == c1) return;                 // one CTA had all of it
+  float m = -INFINITY, l = 0.f, o[COLS][VEC];
+#pragma unroll
+  for (int j = 0; j < COLS; ++j)
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) o[j][e] = 0.f;
 #pragma unroll 4
-  for (int s = 0; s < used; ++s) {
-    const float mw = ml[2 * s];
-    const float f = mw == -INFINITY ? 0.f : dec_ex2(mw - mm);
-    ll = fmaf(ml[2 * s + 1], f, ll);
-    acc = fmaf(p[(long long)s * D], f, acc);
+  for (int c = c0 + warp; c <= c1; c += kJoinWarps) {
+    const long long p = (2ll * c + (c * per >= lo ? 0 : 1)) * (8 * NG) + hl;
+    const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * p);
+    const float mn = fmaxf(m, ml.x);
+    const float f = m == -INFINITY ? 0.f : dec_ex2(m - mn), g = ml.x == -INFINITY ? 0.f : dec_ex2(ml.x - mn);
+    l = l * f + ml.y * g;
+    m = mn;
+#pragma unroll
+    for (int j = 0; j < COLS; ++j) {
+      const float* src = a.part + p * D + j * 128 + lane * VEC;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) o[j][e] = o[j][e] * f + src[e] * g;
+    }
   }
-  reinterpret_cast<T*>(a.out)[row * D + d] = from_f32<T>(acc / ll);
+  if (lane == 0) s_m[warp] = m, s_l[warp] = l;
+#pragma unroll
+  for (int j = 0; j < COLS; ++j)
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) s_o[warp][j * 128 + lane * VEC + e] = o[j][e];
+  __syncthreads();
+  for (int d = tid; d < D; d += kJoinWarps * 32) {
+    float mm = -INFINITY, ll = 0.f, acc = 0.f;
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w) mm = fmaxf(mm, s_m[w]);
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w) {
+      const float f = s_m[w] == -INFINITY ? 0.f : dec_ex2(s_m[w] - mm);
+      ll = fmaf(s_l[w], f, ll);
+      acc = fmaf(s_o[w][d], f, acc);
+    }
+    reinterpret_cast<T*>(a.out)[((long long)r * a.Hq + h) * D + d] = from_f32<T>(acc / ll);
+  }
 }
 
-// Splits of each request: enough CTAs to fill the 148 SMs several times over, so that requests of
-// different lengths even out.
-int dec_splits(int R, int W, int Hk, int ngrp, int page_shift) {
-  const long long pairs = (long long)R * Hk * ngrp;
-  const long long tiles = ((long long)W << page_shift) / 16;
-  long long s = (2048 + pairs - 1) / pairs;
-  const long long most = (tiles + kMinTiles - 1) / kMinTiles;
-  if (s > most) s = most;
-  if (s > 128) s = 128;
-  return s < 1 ? 1 : (int)s;
+// Tensor map over the codes of K or V as (D, page, pages * heads), boxes of 16 tokens.
+bool make_map_codes(CUtensorMap* map, const void* base, int D, int page, uint64_t rows) {
+  auto enc = tensor_map_encoder();
+  if (!enc) return false;
+  const int inner = D < 128 ? D : 128;
+  cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)page, rows};
+  cuuint64_t strides[2] = {(cuuint64_t)D, (cuuint64_t)D * page};
+  cuuint32_t box[3] = {(cuuint32_t)inner, 16, 1};
+  cuuint32_t es[3] = {1, 1, 1};
+  const CUtensorMapSwizzle sw = inner == 128 ? CU_TENSOR_MAP_SWIZZLE_128B
+                                             : (inner == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B);
+  return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, es,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, sw, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
-int dec_groups(int g, int D) { return g > 8 && D < 256 ? (g + 15) / 16 : (g + 7) / 8; }
+
+// Query heads of one row group: 16 where more than 8 share a key head (one reading serves twice as
+// many; with head_dim 256 the registers hold 8), else 8.
+int dec_ng(int g, int D) { return g > 8 && D < 256 ? 2 : 1; }
+int dec_ctas(int g, int D) {
+  const int per = D == 256 || dec_ng(g, D) == 2 ? 2 : (D == 128 ? 3 : 4);
+  return 148 * per;
+}
 
 template <typename T, typename C, int D, int NG>
-cudaError_t decode_launch(const DecodeArgs& a, int R, cudaStream_t s) {
+cudaError_t decode_launch(DecodeArgs a, const PagedCache& c, cudaStream_t s) {
   constexpr size_t smem = dec_smem<D, NG>();
+  CUtensorMap mk, mv;
+  if (!make_map_codes(&mk, c.k, D, c.page, (uint64_t)c.pages * c.nkv) ||
+      !make_map_codes(&mv, c.v, D, c.page, (uint64_t)c.pages * c.nkv))
+    return cudaErrorInvalidValue;
   cudaError_t e = cudaFuncSetAttribute(paged_decode_kernel<T, C, D, NG>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        (int)smem);
   if (e != cudaSuccess) return e;
-  const int ngrp = (a.g + 8 * NG - 1) / (8 * NG);
-  dim3 grid((unsigned)a.splits, (unsigned)(a.Hk * ngrp), (unsigned)R);
-  paged_decode_kernel<T, C, D, NG><<<grid, kDecWarps * 32, smem, s>>>(a);
-  if ((e = cudaGetLastError()) != cudaSuccess || a.splits == 1) return e;
-  paged_decode_join_kernel<T><<<dim3((unsigned)a.Hq, (unsigned)R), D, 0, s>>>(a, D);
-  return cudaGetLastError();
+  a.ngrp = (a.g + 8 * NG - 1) / (8 * NG);
+  // no more CTAs than the table has tiles for
+  const long long units = (((long long)a.W << a.page_shift) + 15) / 16 * a.R * a.Hk * a.ngrp;
+  const long long want = (units + kMinTiles - 1) / kMinTiles;
+  a.ctas = 148 * dec_ctas_per_sm<D, NG>();
+  if (want < a.ctas) a.ctas = (int)want;
+  paged_decode_kernel<T, C, D, NG><<<a.ctas, kDecThreads, smem, s>>>(mk, mv, a);
+  if ((e = cudaGetLastError()) != cudaSuccess || a.ctas == 1) return e;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)a.Hq, (unsigned)a.R);
+  cfg.blockDim = dim3(kJoinWarps * 32);
+  cfg.stream = s;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, paged_decode_join_kernel<T, D, NG>, a);
 }
 
 template <typename T, typename C>
-cudaError_t decode_t(const DecodeArgs& a, int R, int D, cudaStream_t s) {
-  const bool wide = a.g > 8;
+cudaError_t decode_t(const DecodeArgs& a, const PagedCache& c, cudaStream_t s) {
+  const int D = c.D;
+  const bool wide = dec_ng(a.g, D) == 2;
   switch (D) {
-    case 32: return wide ? decode_launch<T, C, 32, 2>(a, R, s) : decode_launch<T, C, 32, 1>(a, R, s);
-    case 64: return wide ? decode_launch<T, C, 64, 2>(a, R, s) : decode_launch<T, C, 64, 1>(a, R, s);
-    case 128: return wide ? decode_launch<T, C, 128, 2>(a, R, s) : decode_launch<T, C, 128, 1>(a, R, s);
-    case 256: return decode_launch<T, C, 256, 1>(a, R, s);
+    case 32: return wide ? decode_launch<T, C, 32, 2>(a, c, s) : decode_launch<T, C, 32, 1>(a, c, s);
+    case 64: return wide ? decode_launch<T, C, 64, 2>(a, c, s) : decode_launch<T, C, 64, 1>(a, c, s);
+    case 128: return wide ? decode_launch<T, C, 128, 2>(a, c, s) : decode_launch<T, C, 128, 1>(a, c, s);
+    case 256: return decode_launch<T, C, 256, 1>(a, c, s);
   }
   return cudaErrorInvalidValue;
 }
 
 }  // namespace
 
-size_t paged_decode_workspace(int R, int W, int Hq, int Hk, int page_shift, int D) {
-  const int splits = dec_splits(R, W, Hk, dec_groups(Hq / Hk, D), page_shift);
-  return splits == 1 ? 0 : (size_t)R * Hq * splits * (D + 2) * sizeof(float);
+size_t paged_decode_workspace(int Hq, int Hk, int D) {
+  const int g = Hq / Hk;
+  return (size_t)dec_ctas(g, D) * 2 * 8 * dec_ng(g, D) * (D + 2) * sizeof(float);
 }
 
 cudaError_t launch_paged_decode(const PagedCache& c, const void* q, const int* table, const int* lengths, void* out,
                                 int R, int W, int Hq, float scale, int dtype, void* workspace, cudaStream_t s) {
-  if (R > 65535) return cudaErrorInvalidValue;
+  // the join's grid, and the tensor maps' coordinate over (page, head)
+  if (R > 65535 || c.pages * c.nkv > 0x7fffffffll) return cudaErrorInvalidValue;
   DecodeArgs a{};
   a.q = q;
-  a.kc = c.k, a.vc = c.v, a.ks = c.ks, a.vs = c.vs, a.gc = c.gate;
+  a.ks = c.ks, a.vs = c.vs, a.gc = c.gate;
   a.table = table, a.lengths = lengths, a.out = out;
   a.pages = c.pages;
-  a.W = W, a.Hq = Hq, a.Hk = c.nkv, a.g = Hq / c.nkv, a.page_shift = c.page_shift, a.scale = scale;
-  a.splits = dec_splits(R, W, c.nkv, dec_groups(a.g, c.D), c.page_shift);
+  a.R = R, a.W = W, a.Hq = Hq, a.Hk = c.nkv, a.g = Hq / c.nkv, a.page_shift = c.page_shift, a.scale = scale;
   a.part = reinterpret_cast<float*>(workspace);
-  a.part_ml = a.part + (size_t)R * Hq * a.splits * c.D;
+  a.part_ml = a.part + (size_t)dec_ctas(a.g, c.D) * 2 * 8 * dec_ng(a.g, c.D) * c.D;
   const bool e4m3 = c.code == SSD_CODE_E4M3;
   switch (dtype) {
-    case SSD_F32: return e4m3 ? decode_t<float, E4M3>(a, R, c.D, s) : decode_t<float, Int8>(a, R, c.D, s);
-    case SSD_BF16:
-      return e4m3 ? decode_t<__nv_bfloat16, E4M3>(a, R, c.D, s) : decode_t<__nv_bfloat16, Int8>(a, R, c.D, s);
-    case SSD_F16: return e4m3 ? decode_t<__half, E4M3>(a, R, c.D, s) : decode_t<__half, Int8>(a, R, c.D, s);
+    case SSD_F32: return e4m3 ? decode_t<float, E4M3>(a, c, s) : decode_t<float, Int8>(a, c, s);
+    case SSD_BF16: return e4m3 ? decode_t<__nv_bfloat16, E4M3>(a, c, s) : decode_t<__nv_bfloat16, Int8>(a, c, s);
+    case SSD_F16: return e4m3 ? decode_t<__half, E4M3>(a, c, s) : decode_t<__half, Int8>(a, c, s);
   }
   return cudaErrorInvalidValue;
 }
+
+SSDB200_DEFINE_ERROR_FETCH(fetch_error_paged)
 
 }  // namespace ssdb200
