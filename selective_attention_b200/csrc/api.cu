@@ -793,7 +793,8 @@ int sattn_prefill_packed(const sattn_packed_params* p, void* stream) {
                               p->k_head_stride,  p->v_token_stride, p->v_head_stride};
   for (int64_t x : strides)
     if (x < 0 || (x * es) % 16 != 0) return SSD_ERR_INVALID_ARGUMENT;
-  const bool tc_ok = sattn_packed_tc_supported((int)D, p->dtype);
+  bool tc_ok = sattn_packed_tc_supported((int)D, p->dtype);
+  for (int64_t x : strides) tc_ok = tc_ok && x > 0;  // (tensor maps have no stride of 0)
   if (p->impl == SSD_IMPL_TC && !tc_ok) return SSD_ERR_INVALID_ARGUMENT;
   PackedArgs a{};
   a.q = p->q;

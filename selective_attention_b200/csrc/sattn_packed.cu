@@ -7,10 +7,14 @@
 // there changes nothing. Rows past the last sequence are written as zeros.
 #include <math.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 #include "kernels.h"
 #include "packed_tiles.cuh"
 #include "sattn_tiles.cuh"
+#include "sm100.cuh"
+#include "tmap.cuh"
 
 namespace ssdb200 {
 namespace {
@@ -193,14 +197,565 @@ cudaError_t packed_simt_t(const PackedArgs& a, cudaStream_t s) {
   return cudaGetLastError();
 }
 
-}  // namespace
+// ===========================================================================
+// Tensor-core kernel (16-bit types, head_dim 64 or 128). CTA = two 128-query tiles, w = 0 and 1:
+// the same positions of two query heads that share a key head, or (heads that cannot be paired)
+// two neighbouring tiles of one head. With two heads both tiles have the same keys, and
+// a prompt is cut at 128 positions instead of 256. Warp roles (12 warps):
+//   warp 0            loads: the Q tiles once, then 128-key tiles of K and V by TMA into two rings;
+//   warp 1 (lane 0)   products: S_w = Q_w K_j^T into TMEM; once softmax w has written P_w(j) over
+//                     S_w(j): O_w += P_w V_j (A from TMEM), then S_w(j + 1). The tiles alternate, so
+//                     that the tensor core works on one while the other's softmax runs;
+//   warps 4-7, 8-11   softmax of tile w, thread = query row = TMEM lane, a tile's 128 scores in
+//                     registers: running maximum in log2 units (O is rescaled only when it grows
+//                     by more than e^8), P = 2^(s - m) rounded to the type, fp32 sums;
+//   warps 2-3         what no query may meet: a product multiplies by zero where it should leave
+//                     out, which is wrong for infinities and NaN. In the last key tiles (own, later
+//                     and other sequences' positions) they set non-finite elements of V to zero, and
+//                     the rows that do see one add it at the end (`odd`); with gates, they write the
+//                     tile's gates and set the K and V rows of dropped keys to zero.
+// The bound is the tensor core (4 D operations a score) together with the special-function unit
+// (one exponential a score: 16 a clock and SM, just as long as the products of head_dim 128), so
+// every kPolyEvery-th pair of exponentials is a cubic on the FMA pipes.
+// TMEM columns: S_0 [0, 128) S_1 [128, 256) (P_w in the first 64 of S_w) O_0 [256, 256 + D) O_1 [384, 384 + D).
+// Every wait is bounded; a role that gives up records a site code, raises the CTA's abort flag and
+// leaves its loop.
+// ===========================================================================
+using namespace sm100;
 
-bool sattn_packed_tc_supported(int D, int dtype) {
-  (void)D, (void)dtype;
-  return false;
+constexpr int kPkThreads = 384;
+constexpr int kPkStages = 2;
+constexpr int kGateSlots = 4;  // a slot is rewritten when the softmaxes are two tiles further
+constexpr float kPkLog2e = 1.4426950408889634f;
+constexpr float kPkRescale = 8.0f * kPkLog2e;
+constexpr unsigned int kSitePkLoad = 0x411, kSitePkMma = 0x412, kSitePkSoft = 0x413, kSitePkClean = 0x414;
+#ifndef SSD_PK_POLY_EVERY
+#define SSD_PK_POLY_EVERY 4
+#endif
+constexpr int kPolyEvery = SSD_PK_POLY_EVERY;
+
+template <int D> constexpr int pk_tile_bytes() { return 128 * D * 2; }
+template <int D> constexpr size_t pk_smem() {
+  return 1024 + (size_t)(2 + 2 * kPkStages) * pk_tile_bytes<D>() + kGateSlots * 128 * 4 + 512;
 }
 
+__device__ __forceinline__ float pk_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// (a NaN stays one)
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+// Packed fp32 pairs.
+__device__ __forceinline__ uint64_t pk2(float a, float b) {
+  return (uint64_t)__float_as_uint(a) | ((uint64_t)__float_as_uint(b) << 32);
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ float lo2(uint64_t x) { return __uint_as_float((uint32_t)x); }
+__device__ __forceinline__ float hi2(uint64_t x) { return __uint_as_float((uint32_t)(x >> 32)); }
+// 2^d for a pair on the FMA pipes: d = n + f, n the nearest integer (left in the low mantissa bits by
+// adding 1.5 * 2^23), 2^f by a cubic least-squares fit on [-0.5, 0.5] (relative error below 8e-5,
+// against 4.9e-4 or more of the 16-bit rounding that follows), n added to the exponent. d is held
+// at -125 or above, so that the exponent stays normal: 2^-125 stands for 0.
+__device__ __forceinline__ uint64_t ex2_fma(uint64_t x) {
+  constexpr float kMagic = 12582912.0f;
+  const uint64_t d = pk2(fmaxf(lo2(x), -125.f), fmaxf(hi2(x), -125.f));
+  const uint64_t r = add2(d, pk2(kMagic, kMagic));
+  const uint64_t f = add2(d, add2(pk2(kMagic, kMagic), r ^ 0x8000000080000000ull));
+  uint64_t p = fma2(f, pk2(0.055171605f, 0.055171605f), pk2(0.24261111f, 0.24261111f));
+  p = fma2(p, f, pk2(0.69326097f, 0.69326097f));
+  p = fma2(p, f, pk2(0.99992806f, 0.99992806f));
+  return (uint64_t)((uint32_t)p + ((uint32_t)r << 23)) |
+         ((uint64_t)((uint32_t)(p >> 32) + ((uint32_t)(r >> 32) << 23)) << 32);
+}
+
+struct PackedTcArgs {
+  const float* lg;
+  const int* cu;
+  const void* v;
+  void* out;
+  int R, T, Hq, Hk, pair;  // pair: a CTA's tiles are two heads
+  long long v_ts, v_hs;
+  float scale;
+};
+
+template <typename T, int D, bool GATED>
+__global__ void __launch_bounds__(kPkThreads, 1)
+    sattn_packed_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                           const __grid_constant__ CUtensorMap tm_v, const PackedTcArgs a) {
+  constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
+  constexpr int NS = kPkStages, TILE = pk_tile_bytes<D>(), NB = D / 64;  // 64-column blocks of 16 KB
+  extern __shared__ uint8_t smraw[];
+  __shared__ PackedTile s_tile;
+  uint8_t* base = align1024_shared(smraw);
+  uint8_t* sQ = base;
+  auto sK = [&](int s) { return base + (2 + s) * TILE; };
+  auto sV = [&](int s) { return base + (2 + NS + s) * TILE; };
+  float* gates = reinterpret_cast<float*>(base + (2 + 2 * NS) * TILE);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(gates + kGateSlots * 128);
+  enum {
+    Q_FULL = 0, K_FULL = 1, V_FULL = K_FULL + NS, K_EMPTY = V_FULL + NS, V_EMPTY = K_EMPTY + NS,
+    CLEAN = V_EMPTY + NS, CARE_V = CLEAN + NS, CARE = CARE_V + 2, S_FULL = CARE + 2, P_FULL = S_FULL + 2, O_DONE = P_FULL + 2,
+    DRAIN = O_DONE + 2, NBARS = DRAIN + 1
+  };
+  static_assert(NBARS * 8 + 16 <= 512, "barrier area");
+  uint32_t* tslot = reinterpret_cast<uint32_t*>(bars + NBARS);
+  volatile int* s_abort = reinterpret_cast<volatile int*>(tslot + 1);
+  volatile int* s_odd = reinterpret_cast<volatile int*>(tslot + 2);
+  auto bar = [&](int i) { return smem_u32(&bars[i]); };
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (warp == 0) {
+    find_packed_tile(a.cu, a.R, a.T, (int)blockIdx.y, a.pair ? 128 : 256, &s_tile);
+  } else if (warp == 1) {
+    tmem_alloc(smem_u32(tslot), 512);
+  } else if (tid == 64) {
+    prefetch_tmap(&tm_q);
+    prefetch_tmap(&tm_k);
+    prefetch_tmap(&tm_v);
+    mbar_init(bar(Q_FULL), 1);
+    for (int s = 0; s < NS; ++s) {
+      mbar_init(bar(K_FULL + s), 1);
+      mbar_init(bar(V_FULL + s), 1);
+      mbar_init(bar(K_EMPTY + s), 1);
+      mbar_init(bar(V_EMPTY + s), 1);
+      mbar_init(bar(CLEAN + s), 2);
+    }
+    for (int w = 0; w < 2; ++w) {
+      mbar_init(bar(CARE_V + w), 1);
+      mbar_init(bar(CARE + w), 2);
+      mbar_init(bar(S_FULL + w), 1);
+      mbar_init(bar(P_FULL + w), 4);
+      mbar_init(bar(O_DONE + w), 1);
+    }
+    mbar_init(bar(DRAIN), 1);
+    *s_abort = 0;
+    *s_odd = 0;
+    fence_mbar_init();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tslot;
+  const PackedTile tile = s_tile;
+  T* out = reinterpret_cast<T*>(a.out);
+  if (tile.seq < 0) {  // nothing, or rows of no sequence
+    const int nh = a.pair ? 2 : 1, row = nh * D;
+    for (int i = tid; i < tile.rows * row; i += kPkThreads)
+      out[((long long)(tile.tok0 + i / row) * a.Hq + blockIdx.x * nh) * D + i % row] = from_f32<T>(0.f);
+    if (warp == 1) tmem_dealloc(tmem, 512);
+    return;
+  }
+  const int seq0 = tile.tok0 - tile.q0;  // the sequence's first token
+  const int q0[2] = {tile.q0, a.pair ? tile.q0 : tile.q0 + 128};
+  const int head[2] = {(int)blockIdx.x * (a.pair ? 2 : 1), (int)blockIdx.x * (a.pair ? 2 : 1) + (a.pair ? 1 : 0)};
+  const int hk = head[0] / (a.Hq / a.Hk);
+  const int nkw[2] = {q0[0] / 128 + 1, q0[1] < tile.n ? q0[1] / 128 + 1 : 0};
+  const int nk = max(nkw[0], nkw[1]);
+  const int care = nkw[0] - 1;  // key tiles from here on hold positions that some row does not see
+  constexpr uint32_t T_S = 0, T_O = 256;
+  // Registers: launched with 168 a thread (384 x 168 = 64512); warpgroup 0 keeps 56 and the two softmax
+  // warpgroups take 208 each: 128 x 56 + 256 x 208 = 60416 <= 64512.
+  static_assert(kPkThreads == 384, "register split assumes three warpgroups");
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ loads
+    regs_dec<56>();
+    if (lane == 0) {
+      const int nq = nkw[1] > 0 ? 2 : 1;
+      mbar_expect_tx(bar(Q_FULL), (uint32_t)(nq * TILE));
+      for (int w = 0; w < nq; ++w)
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+          tma_load_3d(smem_u32(sQ + w * TILE + b * 16384), &tm_q, 64 * b, seq0 + q0[w], head[w], bar(Q_FULL));
+      // the barrier and its parity that tile j of V arrives on
+      auto v_full = [&](int j) { return bar(j >= care ? CARE_V + j - care : V_FULL + j % NS); };
+      auto v_parity = [&](int j) { return j >= care ? 0 : (j / NS) & 1; };
+      int ks = 0, vs = 0;  // tiles asked for
+      while (vs < nk) {
+        const int s = ks % NS;
+        if (ks >= NS && (!mbar_wait(bar(K_EMPTY + s), ((ks / NS) - 1) & 1, kSitePkLoad) || *s_abort)) break;
+        mbar_expect_tx(bar(K_FULL + s), (uint32_t)TILE);
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+          tma_load_3d(smem_u32(sK(s) + b * 16384), &tm_k, 64 * b, seq0 + 128 * ks, hk, bar(K_FULL + s));
+        ++ks;
+        if (vs >= NS && (!mbar_wait(bar(V_EMPTY + s), ((vs / NS) - 1) & 1, kSitePkLoad) || *s_abort)) break;
+        mbar_expect_tx(v_full(vs), (uint32_t)TILE);
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+          tma_load_3d(smem_u32(sV(s) + b * 16384), &tm_v, 64 * b, seq0 + 128 * vs, hk, v_full(vs));
+        ++vs;
+      }
+      if (vs < nk) *s_abort = 1;
+      // no copy may still be in flight when the CTA exits
+      mbar_wait(bar(Q_FULL), 0, kSitePkLoad);
+      for (int jj = max(ks - NS, 0); jj < ks; ++jj) mbar_wait(bar(K_FULL + jj % NS), (jj / NS) & 1, kSitePkLoad);
+      for (int jj = max(vs - NS, 0); jj < vs; ++jj) mbar_wait(v_full(jj), v_parity(jj), kSitePkLoad);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ products
+    regs_dec<56>();
+    if (lane == 0) {
+      constexpr uint32_t ID_S = idesc_f16(128, 128, BF16, false, false);
+      constexpr uint32_t ID_O = idesc_f16(128, D, BF16, false, true);
+      const uint32_t qa = smem_u32(sQ);
+      bool issued = false;
+      auto ready = [&](int jj, int full) {  // tile jj of K or V, clean where it has to be
+        if (jj >= care && full == V_FULL) return mbar_wait(bar(CARE + jj - care), 0, kSitePkMma);
+        if (GATED && jj < care) return mbar_wait(bar(CLEAN + jj % NS), (jj / NS) & 1, kSitePkMma);
+        return mbar_wait(bar(full + jj % NS), (jj / NS) & 1, kSitePkMma);
+      };
+      auto issue_s = [&](int w, int jj) {
+        const uint32_t qb = qa + (uint32_t)(w * TILE), kb = smem_u32(sK(jj % NS));
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) {
+          const uint32_t off = (uint32_t)((ks >> 2) * 16384 + (ks & 3) * 32);
+          umma_f16(tmem + T_S + 128 * w, sdesc_sw128(qb + off, 16, 1024), sdesc_sw128(kb + off, 16, 1024), ID_S,
+                   ks > 0 ? 1u : 0u);
+        }
+        umma_commit(bar(S_FULL + w));
+        issued = true;
+      };
+      bool fail = !mbar_wait(bar(Q_FULL), 0, kSitePkMma) || !ready(0, K_FULL);
+      if (!fail) {
+        tc_fence_after();
+        issue_s(0, 0);
+        if (nkw[1] > 0) issue_s(1, 0);
+        umma_commit(bar(K_EMPTY));
+      }
+      for (int j = 0; j < nk && !fail && !*s_abort; ++j) {
+        const int s = j % NS;
+        const uint32_t vb = smem_u32(sV(s));
+        bool have_v = false, have_k = false;
+        for (int w = 0; w < 2 && !fail; ++w) {
+          if (j >= nkw[w]) continue;
+          if ((!have_v && !ready(j, V_FULL)) || !mbar_wait(bar(P_FULL + w), j & 1, kSitePkMma)) {
+            fail = true;
+            break;
+          }
+          have_v = true;
+          tc_fence_after();
+#pragma unroll
+          for (int ks = 0; ks < 8; ++ks)
+            umma_f16_ts(tmem + T_O + 128 * w, tmem + T_S + 128 * w + 8 * ks, sdesc_sw128(vb + 2048 * ks, 16384, 1024),
+                        ID_O, (j > 0 || ks > 0) ? 1u : 0u);
+          if (j + 1 < nkw[w]) {
+            if (!have_k && !ready(j + 1, K_FULL)) {
+              fail = true;
+              break;
+            }
+            have_k = true;
+            tc_fence_after();
+            issue_s(w, j + 1);  // over P_w(j): the products run in the order of their issue
+          } else {
+            umma_commit(bar(O_DONE + w));
+          }
+        }
+        if (fail) break;
+        umma_commit(bar(V_EMPTY + s));
+        if (have_k) umma_commit(bar(K_EMPTY + (j + 1) % NS));
+      }
+      if (fail) *s_abort = 1;
+      // every product has completed before TMEM is released
+      if (issued) {
+        umma_commit(bar(DRAIN));
+        mbar_wait(bar(DRAIN), 0, kSitePkMma);
+      }
+    }
+    __syncwarp();
+  } else if (warp < 4) {
+    // ------------------------------------------------------------ clean tiles
+    regs_dec<56>();
+    const int t = tid - 64;  // 0 .. 63: keys t and t + 64 of a tile
+    auto gate_at = [&](int key) {
+      if constexpr (!GATED) return 0.f;
+      return key < tile.n ? a.lg[(long long)(seq0 + key) * a.Hk + hk] * kPkLog2e : 0.f;
+    };
+    bool ok = true;
+    int j = GATED ? 0 : care;
+    float g0 = gate_at(128 * j + t), g1 = gate_at(128 * j + t + 64);
+    for (; j < nk; ++j) {
+      const int s = j % NS;
+      ok = ok && !*s_abort;
+      if (j < care)
+        ok = ok && mbar_wait_sleep(bar(K_FULL + s), (j / NS) & 1, kSitePkClean) &&
+             mbar_wait_sleep(bar(V_FULL + s), (j / NS) & 1, kSitePkClean);
+      else
+        ok = ok && mbar_wait_sleep(bar(CARE_V + j - care), 0, kSitePkClean);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      if constexpr (GATED) {
+        gates[(j % kGateSlots) * 128 + t] = g0;
+        gates[(j % kGateSlots) * 128 + t + 64] = g1;
+        if (j < care) {
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            if ((half ? g1 : g0) != -INFINITY) continue;
+            const int key = t + 64 * half;
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+              for (int c = 0; c < 8; ++c) {
+                *reinterpret_cast<uint4*>(sK(s) + b * 16384 + key * 128 + c * 16) = make_uint4(0u, 0u, 0u, 0u);
+                *reinterpret_cast<uint4*>(sV(s) + b * 16384 + key * 128 + c * 16) = make_uint4(0u, 0u, 0u, 0u);
+              }
+          }
+        }
+        g0 = gate_at(128 * (j + 1) + t);
+        g1 = gate_at(128 * (j + 1) + t + 64);
+      }
+      if (j >= care) {
+        constexpr uint32_t EXP = BF16 ? 0x7f80u : 0x7c00u;
+        uint4* vt = reinterpret_cast<uint4*>(sV(s));
+        bool odd = false;
+#pragma unroll 4
+        for (int i = t; i < TILE / 16; i += 64) {
+          uint4 x = vt[i];
+          auto bad = [&](uint32_t w) {
+            return (w & EXP) == EXP || (w & (EXP << 16)) == (EXP << 16);
+          };
+          if (bad(x.x) || bad(x.y) || bad(x.z) || bad(x.w)) {
+            odd = true;
+            auto fix = [&](uint32_t w) {
+              if ((w & EXP) == EXP) w &= 0xffff0000u;
+              if ((w & (EXP << 16)) == (EXP << 16)) w &= 0xffffu;
+              return w;
+            };
+            vt[i] = make_uint4(fix(x.x), fix(x.y), fix(x.z), fix(x.w));
+          }
+        }
+        if (odd) *s_odd = 1;
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(j >= care ? CARE + j - care : CLEAN + s));
+    }
+    if (!ok) *s_abort = 1;
+  } else {
+    // ------------------------------------------------------------ softmax of tile w
+    regs_inc<208>();
+    const int w = (warp - 4) >> 2;
+    const int r = (warp & 3) * 32 + lane;
+    const uint32_t tl = (uint32_t)((warp & 3) * 32) << 16;
+    const int my_nk = w ? nkw[1] : nkw[0];
+    const int qi = (w ? q0[1] : q0[0]) + r;
+    const uint32_t ts = tmem + tl + T_S + 128 * w, to = tmem + tl + T_O + 128 * w;
+    const float scale2 = a.scale * kPkLog2e;
+    float m_used = -INFINITY, lsum = 0.f;
+    bool not_a_number = false;  // the row has a score of NaN or +inf
+    bool wfail = false;
+    auto warp_wait = [&](uint32_t b, uint32_t parity) {
+      if (!wfail) wfail = !__all_sync(0xffffffffu, mbar_wait(b, parity, kSitePkSoft));
+      return !wfail;
+    };
+    for (int j = 0; j < my_nk; ++j) {
+      if (!warp_wait(bar(S_FULL + w), j & 1)) break;
+      if (GATED && !warp_wait(j >= care ? bar(CARE + j - care) : bar(CLEAN + j % NS), j >= care ? 0 : (j / NS) & 1)) break;
+      tc_fence_after();
+      uint32_t sv[4][32];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_ld32(ts + 32 * c, sv[c]);
+      tmem_wait_ld();
+      const float* g = gates + (j % kGateSlots) * 128;
+      float mp[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      float mul = scale2;  // what the scores are still to be multiplied by
+      if (j < care && (GATED || scale2 > 0.f)) {
+        if constexpr (GATED) {
+          const uint64_t sc2 = pk2(scale2, scale2);
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int e = 0; e < 32; e += 4) {
+              const float4 gg = *reinterpret_cast<const float4*>(g + 32 * c + e);
+              const uint64_t x0 = fma2(pk2(__uint_as_float(sv[c][e]), __uint_as_float(sv[c][e + 1])), sc2, pk2(gg.x, gg.y));
+              const uint64_t x1 = fma2(pk2(__uint_as_float(sv[c][e + 2]), __uint_as_float(sv[c][e + 3])), sc2, pk2(gg.z, gg.w));
+              sv[c][e] = (uint32_t)x0, sv[c][e + 1] = (uint32_t)(x0 >> 32);
+              sv[c][e + 2] = (uint32_t)x1, sv[c][e + 3] = (uint32_t)(x1 >> 32);
+            }
+          mul = 1.f;
+        }
+      } else {
+        // own position, later ones and dropped keys
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            const int key = 128 * j + 32 * c + e;
+            const float gg = GATED ? g[32 * c + e] : 0.f;
+            const float x = fmaf(__uint_as_float(sv[c][e]), scale2, key < qi ? gg : 0.f);
+            sv[c][e] = __float_as_uint(key == qi || (key < qi && gg != -INFINITY) ? x : -INFINITY);
+          }
+        mul = 1.f;
+      }
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+#pragma unroll
+        for (int e = 0; e < 32; e += 4)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) mp[q] = max_nan(mp[q], __uint_as_float(sv[c][e + q]));
+      const float mt = max_nan(max_nan(mp[0], mp[1]), max_nan(mp[2], mp[3])) * mul;
+      if (!(mt < INFINITY)) not_a_number = true;
+      float f = 1.f;
+      bool resc = false;
+      if (mt < INFINITY && mt > m_used + kPkRescale) {
+        if (m_used != -INFINITY) {  // O and the sum hold earlier tiles: rescale them
+          f = pk_ex2(m_used - mt);
+          lsum *= f;
+          resc = true;
+        }
+        m_used = mt;
+      }
+      // S_w(j) is complete, and with it the products before it: O_w holds the tiles up to j - 1
+      if (__any_sync(0xffffffffu, resc)) {
+#pragma unroll
+        for (int c = 0; c < D / 16; ++c) {
+          uint32_t o[16];
+          tmem_ld16(to + 16 * c, o);
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+          tmem_st16(to + 16 * c, o);
+        }
+      }
+      const float mb = m_used == -INFINITY ? 0.f : -m_used;
+      const uint64_t mul2 = pk2(mul, mul), mb2 = pk2(mb, mb);
+      uint64_t ls[2] = {0ull, 0ull};
+      auto weights = [&](auto cubic) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int q = 0; q < 16; ++q) {
+            const uint64_t d = fma2(pk2(__uint_as_float(sv[c][2 * q]), __uint_as_float(sv[c][2 * q + 1])), mul2, mb2);
+            uint64_t p;
+            if (decltype(cubic)::value && kPolyEvery > 0 && q % (kPolyEvery > 0 ? kPolyEvery : 1) == 0) {
+              p = ex2_fma(d);
+            } else {
+              p = pk2(pk_ex2(lo2(d)), pk_ex2(hi2(d)));
+            }
+            ls[q & 1] = add2(ls[q & 1], p);
+            pk[q] = pack2<T>(lo2(p), hi2(p));
+          }
+          tmem_st16(ts + 16 * c, pk);  // (the scores of these columns are in registers)
+        }
+      };
+      // 2^-125 is no 0 to a large V: where positions are masked every exponential is the hardware's
+      if (j < care)
+        weights(std::true_type{});
+      else
+        weights(std::false_type{});
+      const uint64_t l2 = add2(ls[0], ls[1]);
+      lsum += lo2(l2) + hi2(l2);
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(P_FULL + w));
+    }
+    if (!wfail && my_nk > 0 && warp_wait(bar(O_DONE + w), 0)) {
+      tc_fence_after();
+      const float inv = not_a_number ? __uint_as_float(0x7fffffffu) : 1.0f / lsum;
+      const bool odd = *s_odd != 0;
+      T* op = out + ((long long)(seq0 + qi) * a.Hq + (w ? head[1] : head[0])) * D;
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t o[32];
+        tmem_ld32(to + 32 * c, o);
+        tmem_wait_ld();
+        if (qi < tile.n) {
+          if (odd) {
+            // the elements of V that were set to zero, for the rows that see them
+            for (int key = 128 * care; key <= qi; ++key) {
+              if (GATED && key < qi && a.lg[(long long)(seq0 + key) * a.Hk + hk] == -INFINITY) continue;
+              const T* vp = reinterpret_cast<const T*>(a.v) + (seq0 + key) * a.v_ts + hk * a.v_hs + 32 * c;
+#pragma unroll
+              for (int e = 0; e < 32; ++e) {
+                const float x = to_f32<T>(vp[e]);
+                if (!(fabsf(x) < INFINITY)) o[e] = __float_as_uint(__uint_as_float(o[e]) + x);
+              }
+            }
+          }
+#pragma unroll
+          for (int e = 0; e < 32; e += 8) {
+            uint4 y;
+            y.x = pack2<T>(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv);
+            y.y = pack2<T>(__uint_as_float(o[e + 2]) * inv, __uint_as_float(o[e + 3]) * inv);
+            y.z = pack2<T>(__uint_as_float(o[e + 4]) * inv, __uint_as_float(o[e + 5]) * inv);
+            y.w = pack2<T>(__uint_as_float(o[e + 6]) * inv, __uint_as_float(o[e + 7]) * inv);
+            *reinterpret_cast<uint4*>(op + 32 * c + e) = y;
+          }
+        }
+      }
+    }
+    if (wfail) *s_abort = 1;
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) tmem_dealloc(tmem, 512);
+}
+
+// Tensor map over (D, tokens, heads) of a packed tensor, boxes of 64 columns x 128 tokens.
+bool make_map_packed(CUtensorMap* map, const void* base, bool bf16, int D, int T, int H, long long ts, long long hs) {
+  auto enc = tensor_map_encoder();
+  if (!enc) return false;
+  cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)T, (cuuint64_t)H};
+  cuuint64_t strides[2] = {(cuuint64_t)ts * 2, (cuuint64_t)hs * 2};
+  cuuint32_t box[3] = {64, 128, 1};
+  cuuint32_t es[3] = {1, 1, 1};
+  return enc(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(base),
+             dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, int D, bool GATED>
+cudaError_t packed_tc_t(const PackedArgs& a, cudaStream_t s) {
+  const bool bf16 = std::is_same<T, __nv_bfloat16>::value;
+  CUtensorMap mq, mk, mv;
+  if (!make_map_packed(&mq, a.q, bf16, D, a.T, a.Hq, a.st.q_ts, a.st.q_hs) ||
+      !make_map_packed(&mk, a.k, bf16, D, a.T, a.Hk, a.st.k_ts, a.st.k_hs) ||
+      !make_map_packed(&mv, a.v, bf16, D, a.T, a.Hk, a.st.v_ts, a.st.v_hs))
+    return cudaErrorInvalidValue;
+  PackedTcArgs k{};
+  k.lg = a.log_gate, k.cu = a.cu, k.v = a.v, k.out = a.out;
+  k.R = a.R, k.T = a.T, k.Hq = a.Hq, k.Hk = a.Hk;
+  k.pair = (a.Hq / a.Hk) % 2 == 0;
+  k.v_ts = a.st.v_ts, k.v_hs = a.st.v_hs;
+  k.scale = a.scale;
+  const long long tiles = packed_tile_bound(a.T, a.R, k.pair ? 128 : 256);
+  if (tiles > 65535) return cudaErrorInvalidValue;
+  cudaError_t e = cudaFuncSetAttribute(sattn_packed_tc_kernel<T, D, GATED>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       (int)pk_smem<D>());
+  if (e != cudaSuccess) return e;
+  sattn_packed_tc_kernel<T, D, GATED>
+      <<<dim3((unsigned)(k.pair ? a.Hq / 2 : a.Hq), (unsigned)tiles), kPkThreads, pk_smem<D>(), s>>>(mq, mk, mv, k);
+  return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t packed_tc(const PackedArgs& a, cudaStream_t s) {
+  if (a.D == 64) return a.log_gate ? packed_tc_t<T, 64, true>(a, s) : packed_tc_t<T, 64, false>(a, s);
+  return a.log_gate ? packed_tc_t<T, 128, true>(a, s) : packed_tc_t<T, 128, false>(a, s);
+}
+
+}  // namespace
+
+bool sattn_packed_tc_supported(int D, int dtype) { return (D == 64 || D == 128) && dtype != SSD_F32; }
+
 cudaError_t launch_sattn_packed(const PackedArgs& a, cudaStream_t s) {
+  if (a.use_tc) return a.dtype == SSD_BF16 ? packed_tc<__nv_bfloat16>(a, s) : packed_tc<__half>(a, s);
   switch (a.dtype) {
     case SSD_F32: return packed_simt_t<float>(a, s);
     case SSD_BF16: return packed_simt_t<__nv_bfloat16>(a, s);
