@@ -202,8 +202,8 @@ cudaError_t packed_simt_t(const PackedArgs& a, cudaStream_t s) {
 // the same positions of two query heads that share a key head, or (heads that cannot be paired)
 // two neighbouring tiles of one head. With two heads both tiles have the same keys, and
 // a prompt is cut at 128 positions instead of 256. Warp roles (12 warps):
-//   warp 0            loads: the Q tiles once, then 128-key tiles of K and V by TMA into two rings;
-//   warp 1 (lane 0)   products: S_w = Q_w K_j^T into TMEM; once softmax w has written P_w(j) over
+//   warp 0            loads: the Q tiles once, then 128-key tiles of K and V by TMA into a ring;
+//   warp 1            products: S_w = Q_w K_j^T into TMEM; once softmax w has written P_w(j) over
 //                     S_w(j): O_w += P_w V_j (A from TMEM), then S_w(j + 1). The tiles alternate, so
 //                     that the tensor core works on one while the other's softmax runs;
 //   warps 4-7, 8-11   softmax of tile w, thread = query row = TMEM lane, a tile's 128 scores in
@@ -224,8 +224,7 @@ cudaError_t packed_simt_t(const PackedArgs& a, cudaStream_t s) {
 using namespace sm100;
 
 constexpr int kPkThreads = 384;
-constexpr int kPkStages = 2;
-constexpr int kGateSlots = 4;  // a slot is rewritten when the softmaxes are two tiles further
+constexpr int kCleanSlots = 4;
 constexpr float kPkLog2e = 1.4426950408889634f;
 constexpr float kPkRescale = 8.0f * kPkLog2e;
 constexpr unsigned int kSitePkLoad = 0x411, kSitePkMma = 0x412, kSitePkSoft = 0x413, kSitePkClean = 0x414;
@@ -235,9 +234,17 @@ constexpr unsigned int kSitePkLoad = 0x411, kSitePkMma = 0x412, kSitePkSoft = 0x
 constexpr int kPolyEvery = SSD_PK_POLY_EVERY;
 
 template <int D> constexpr int pk_tile_bytes() { return 128 * D * 2; }
-template <int D> constexpr size_t pk_smem() {
-  return 1024 + (size_t)(2 + 2 * kPkStages) * pk_tile_bytes<D>() + kGateSlots * 128 * 4 + 512;
+// One ring for the tiles of K and V in the order of their use, K_0 V_0 K_1 V_1 ...: what shared memory
+// holds beside the two Q tiles.
+template <int D> constexpr int pk_slots() { return D == 128 ? 5 : 8; }
+// Gates of tile j + G may take the place of tile j's: V_{j + G} is loaded when element
+// 2 (j + G) + 1 - slots has been used, K_{j + 1} or V_j, that is after the softmaxes of tile j.
+template <int D> constexpr int pk_gate_slots() { return D == 128 ? 3 : 4; }
+template <int D> constexpr int pk_bar_bytes() { return D == 128 ? 256 : 320; }
+template <int D, bool GATED> constexpr size_t pk_smem() {
+  return 1024 + (size_t)(2 + pk_slots<D>()) * pk_tile_bytes<D>() + (GATED ? pk_gate_slots<D>() * 128 * 4 : 0) + pk_bar_bytes<D>();
 }
+static_assert(pk_smem<128, true>() + sizeof(PackedTile) + 16 <= 227 * 1024, "shared memory of a CTA");
 
 __device__ __forceinline__ float pk_ex2(float x) {
   float y;
@@ -282,6 +289,34 @@ __device__ __forceinline__ uint64_t ex2_fma(uint64_t x) {
          ((uint64_t)((uint32_t)(p >> 32) + ((uint32_t)(r >> 32) << 23)) << 32);
 }
 
+// Low word of a 128-byte-swizzled operand's descriptor; the high word is the same for all of them (8-row
+// groups 1024 bytes apart, descriptor version, swizzle). Addresses below 2^18 only move the low 14 bits.
+__device__ __forceinline__ uint32_t desc_lo(uint32_t addr, uint32_t lbo) {
+  return ((addr >> 4) & 0x3fffu) | ((lbo >> 4) << 16);
+}
+constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 x, y;\n\tsetp.ne.b32 p, %5, 0;\n\t"
+      "mov.b64 x, {%1, %3};\n\tmov.b64 y, {%2, %3};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %4, p;\n\t}\n" ::"r"(d),
+      "r"(a), "r"(b), "r"(kDescHi), "r"(idesc), "r"((uint32_t)accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 y;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b64 y, {%2, %3};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %4, p;\n\t}\n" ::"r"(d),
+      "r"(a), "r"(b), "r"(kDescHi), "r"(idesc), "r"((uint32_t)accumulate)
+      : "memory");
+}
+// One lane of the (whole) warp, always the same.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t x;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(x));
+  return x != 0;
+}
+
 struct PackedTcArgs {
   const float* lg;
   const int* cu;
@@ -297,21 +332,20 @@ __global__ void __launch_bounds__(kPkThreads, 1)
     sattn_packed_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                            const __grid_constant__ CUtensorMap tm_v, const PackedTcArgs a) {
   constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
-  constexpr int NS = kPkStages, TILE = pk_tile_bytes<D>(), NB = D / 64;  // 64-column blocks of 16 KB
+  constexpr int NS = pk_slots<D>(), TILE = pk_tile_bytes<D>(), NB = D / 64;  // 64-column blocks of 16 KB
+  constexpr int GS = pk_gate_slots<D>();
   extern __shared__ uint8_t smraw[];
   __shared__ PackedTile s_tile;
   uint8_t* base = align1024_shared(smraw);
   uint8_t* sQ = base;
-  auto sK = [&](int s) { return base + (2 + s) * TILE; };
-  auto sV = [&](int s) { return base + (2 + NS + s) * TILE; };
-  float* gates = reinterpret_cast<float*>(base + (2 + 2 * NS) * TILE);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(gates + kGateSlots * 128);
+  auto slot_at = [&](int i) { return base + (2 + i % NS) * TILE; };  // of element i: K_j is 2 j, V_j 2 j + 1
+  float* gates = reinterpret_cast<float*>(base + (2 + NS) * TILE);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(gates + (GATED ? pk_gate_slots<D>() * 128 : 0));
   enum {
-    Q_FULL = 0, K_FULL = 1, V_FULL = K_FULL + NS, K_EMPTY = V_FULL + NS, V_EMPTY = K_EMPTY + NS,
-    CLEAN = V_EMPTY + NS, CARE_V = CLEAN + NS, CARE = CARE_V + 2, S_FULL = CARE + 2, P_FULL = S_FULL + 2, O_DONE = P_FULL + 2,
+    Q_FULL = 0, FULL = 1, EMPTY = FULL + NS, CLEAN = EMPTY + NS, CARE_V = CLEAN + kCleanSlots, CARE = CARE_V + 2, S_FULL = CARE + 2, P_FULL = S_FULL + 2, O_DONE = P_FULL + 2,
     DRAIN = O_DONE + 2, NBARS = DRAIN + 1
   };
-  static_assert(NBARS * 8 + 16 <= 512, "barrier area");
+  static_assert(NBARS * 8 + 16 <= pk_bar_bytes<D>(), "barrier area");
   uint32_t* tslot = reinterpret_cast<uint32_t*>(bars + NBARS);
   volatile int* s_abort = reinterpret_cast<volatile int*>(tslot + 1);
   volatile int* s_odd = reinterpret_cast<volatile int*>(tslot + 2);
@@ -327,12 +361,10 @@ __global__ void __launch_bounds__(kPkThreads, 1)
     prefetch_tmap(&tm_v);
     mbar_init(bar(Q_FULL), 1);
     for (int s = 0; s < NS; ++s) {
-      mbar_init(bar(K_FULL + s), 1);
-      mbar_init(bar(V_FULL + s), 1);
-      mbar_init(bar(K_EMPTY + s), 1);
-      mbar_init(bar(V_EMPTY + s), 1);
-      mbar_init(bar(CLEAN + s), 2);
+      mbar_init(bar(FULL + s), 1);
+      mbar_init(bar(EMPTY + s), 1);
     }
+    for (int s = 0; s < kCleanSlots; ++s) mbar_init(bar(CLEAN + s), 2);
     for (int w = 0; w < 2; ++w) {
       mbar_init(bar(CARE_V + w), 1);
       mbar_init(bar(CARE + w), 2);
@@ -380,151 +412,145 @@ __global__ void __launch_bounds__(kPkThreads, 1)
 #pragma unroll
         for (int b = 0; b < NB; ++b)
           tma_load_3d(smem_u32(sQ + w * TILE + b * 16384), &tm_q, 64 * b, seq0 + q0[w], head[w], bar(Q_FULL));
-      // the barrier and its parity that tile j of V arrives on
-      auto v_full = [&](int j) { return bar(j >= care ? CARE_V + j - care : V_FULL + j % NS); };
-      auto v_parity = [&](int j) { return j >= care ? 0 : (j / NS) & 1; };
-      int ks = 0, vs = 0;  // tiles asked for
-      while (vs < nk) {
-        const int s = ks % NS;
-        if (ks >= NS && (!mbar_wait(bar(K_EMPTY + s), ((ks / NS) - 1) & 1, kSitePkLoad) || *s_abort)) break;
-        mbar_expect_tx(bar(K_FULL + s), (uint32_t)TILE);
+      // the barrier and its parity that element i arrives on (V tiles that the cleaning warps wait for on their own)
+      auto full = [&](int i) { return bar((i & 1) && (i >> 1) >= care ? CARE_V + (i >> 1) - care : FULL + i % NS); };
+      auto parity = [&](int i) { return (i & 1) && (i >> 1) >= care ? 0 : (i / NS) & 1; };
+      int i = 0;
+      for (; i < 2 * nk; ++i) {
+        if (i >= NS && (!mbar_wait(bar(EMPTY + i % NS), ((i / NS) - 1) & 1, kSitePkLoad) || *s_abort)) break;
+        mbar_expect_tx(full(i), (uint32_t)TILE);
 #pragma unroll
         for (int b = 0; b < NB; ++b)
-          tma_load_3d(smem_u32(sK(s) + b * 16384), &tm_k, 64 * b, seq0 + 128 * ks, hk, bar(K_FULL + s));
-        ++ks;
-        if (vs >= NS && (!mbar_wait(bar(V_EMPTY + s), ((vs / NS) - 1) & 1, kSitePkLoad) || *s_abort)) break;
-        mbar_expect_tx(v_full(vs), (uint32_t)TILE);
-#pragma unroll
-        for (int b = 0; b < NB; ++b)
-          tma_load_3d(smem_u32(sV(s) + b * 16384), &tm_v, 64 * b, seq0 + 128 * vs, hk, v_full(vs));
-        ++vs;
+          tma_load_3d(smem_u32(slot_at(i) + b * 16384), i & 1 ? &tm_v : &tm_k, 64 * b, seq0 + 128 * (i >> 1), hk, full(i));
       }
-      if (vs < nk) *s_abort = 1;
+      if (i < 2 * nk) *s_abort = 1;
       // no copy may still be in flight when the CTA exits
       mbar_wait(bar(Q_FULL), 0, kSitePkLoad);
-      for (int jj = max(ks - NS, 0); jj < ks; ++jj) mbar_wait(bar(K_FULL + jj % NS), (jj / NS) & 1, kSitePkLoad);
-      for (int jj = max(vs - NS, 0); jj < vs; ++jj) mbar_wait(v_full(jj), v_parity(jj), kSitePkLoad);
+      for (int d = max(i - NS, 0); d < i; ++d) mbar_wait(full(d), parity(d), kSitePkLoad);
     }
     __syncwarp();
   } else if (warp == 1) {
     // ------------------------------------------------------------ products
+    // One warp for both tiles, which keeps them half a period apart. The whole warp runs the role and
+    // one elected lane issues: addresses, descriptors and the loop stay in uniform registers, which
+    // the instruction takes its operands from.
     regs_dec<56>();
-    if (lane == 0) {
-      constexpr uint32_t ID_S = idesc_f16(128, 128, BF16, false, false);
-      constexpr uint32_t ID_O = idesc_f16(128, D, BF16, false, true);
-      const uint32_t qa = smem_u32(sQ);
-      bool issued = false;
-      auto ready = [&](int jj, int full) {  // tile jj of K or V, clean where it has to be
-        if (jj >= care && full == V_FULL) return mbar_wait(bar(CARE + jj - care), 0, kSitePkMma);
-        if (GATED && jj < care) return mbar_wait(bar(CLEAN + jj % NS), (jj / NS) & 1, kSitePkMma);
-        return mbar_wait(bar(full + jj % NS), (jj / NS) & 1, kSitePkMma);
-      };
-      auto issue_s = [&](int w, int jj) {
-        const uint32_t qb = qa + (uint32_t)(w * TILE), kb = smem_u32(sK(jj % NS));
+    constexpr uint32_t ID_S = idesc_f16(128, 128, BF16, false, false);
+    constexpr uint32_t ID_O = idesc_f16(128, D, BF16, false, true);
+    const int n0 = __shfl_sync(0xffffffffu, nkw[0], 0), n1 = __shfl_sync(0xffffffffu, nkw[1], 0);
+    const int first_care = __shfl_sync(0xffffffffu, care, 0), nkt = max(n0, n1);
+    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+    const uint32_t qd = desc_lo(__shfl_sync(0xffffffffu, smem_u32(sQ), 0), 16);
+    const uint32_t kd = desc_lo(__shfl_sync(0xffffffffu, smem_u32(slot_at(0)), 0), 16);
+    const uint32_t vd = desc_lo(__shfl_sync(0xffffffffu, smem_u32(slot_at(0)), 0), 16384);
+    const bool lead = elect_one();
+    auto wait = [&](uint32_t b, uint32_t parity) { return (bool)__all_sync(0xffffffffu, mbar_wait(b, parity, kSitePkMma)); };
+    auto ready_k = [&](int j) {  // tile j of K, clean where it has to be
+      if (GATED && j < first_care) return wait(bar(CLEAN + j % kCleanSlots), (j / kCleanSlots) & 1);
+      return wait(bar(FULL + 2 * j % NS), (2 * j / NS) & 1);
+    };
+    auto ready_v = [&](int j) {
+      if (j >= first_care) return wait(bar(CARE + j - first_care), 0);
+      if (GATED) return wait(bar(CLEAN + j % kCleanSlots), (j / kCleanSlots) & 1);
+      return wait(bar(FULL + (2 * j + 1) % NS), ((2 * j + 1) / NS) & 1);
+    };
+    auto issue_s = [&](int w, int j, bool last) {
+      const uint32_t q1 = qd + (uint32_t)(w * (TILE >> 4)), k1 = kd + (uint32_t)((2 * j % NS) * (TILE >> 4));
+      if (lead) {
 #pragma unroll
         for (int ks = 0; ks < D / 16; ++ks) {
-          const uint32_t off = (uint32_t)((ks >> 2) * 16384 + (ks & 3) * 32);
-          umma_f16(tmem + T_S + 128 * w, sdesc_sw128(qb + off, 16, 1024), sdesc_sw128(kb + off, 16, 1024), ID_S,
-                   ks > 0 ? 1u : 0u);
+          const uint32_t off = (uint32_t)(((ks >> 2) * 16384 + (ks & 3) * 32) >> 4);
+          mma_ss(tm + T_S + 128 * w, q1 + off, k1 + off, ID_S, ks > 0);
         }
         umma_commit(bar(S_FULL + w));
-        issued = true;
-      };
-      bool fail = !mbar_wait(bar(Q_FULL), 0, kSitePkMma) || !ready(0, K_FULL);
-      if (!fail) {
-        tc_fence_after();
-        issue_s(0, 0);
-        if (nkw[1] > 0) issue_s(1, 0);
-        umma_commit(bar(K_EMPTY));
+        if (last) umma_commit(bar(EMPTY + 2 * j % NS));
       }
-      for (int j = 0; j < nk && !fail && !*s_abort; ++j) {
-        const int s = j % NS;
-        const uint32_t vb = smem_u32(sV(s));
-        bool have_v = false, have_k = false;
-        for (int w = 0; w < 2 && !fail; ++w) {
-          if (j >= nkw[w]) continue;
-          if ((!have_v && !ready(j, V_FULL)) || !mbar_wait(bar(P_FULL + w), j & 1, kSitePkMma)) {
-            fail = true;
-            break;
-          }
-          have_v = true;
-          tc_fence_after();
+    };
+    bool fail = !wait(bar(Q_FULL), 0) || !ready_k(0);
+    if (!fail) {
+      tc_fence_after();
+      issue_s(0, 0, n1 == 0);
+      if (n1 > 0) issue_s(1, 0, true);
+    }
+    for (int j = 0; j < nkt && !fail && !__any_sync(0xffffffffu, *s_abort); ++j) {
+      const uint32_t v1 = vd + (uint32_t)(((2 * j + 1) % NS) * (TILE >> 4));
+      if (!ready_v(j) || (j + 1 < nkt && !ready_k(j + 1))) {
+        fail = true;
+        break;
+      }
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        const int nw = w ? n1 : n0;
+        if (fail || j >= nw) continue;
+        if (!wait(bar(P_FULL + w), j & 1)) {
+          fail = true;
+          continue;
+        }
+        tc_fence_after();
+        if (lead) {
 #pragma unroll
           for (int ks = 0; ks < 8; ++ks)
-            umma_f16_ts(tmem + T_O + 128 * w, tmem + T_S + 128 * w + 8 * ks, sdesc_sw128(vb + 2048 * ks, 16384, 1024),
-                        ID_O, (j > 0 || ks > 0) ? 1u : 0u);
-          if (j + 1 < nkw[w]) {
-            if (!have_k && !ready(j + 1, K_FULL)) {
-              fail = true;
-              break;
-            }
-            have_k = true;
-            tc_fence_after();
-            issue_s(w, j + 1);  // over P_w(j): the products run in the order of their issue
-          } else {
-            umma_commit(bar(O_DONE + w));
-          }
+            mma_ts(tm + T_O + 128 * w, tm + T_S + 128 * w + 8 * ks, v1 + (uint32_t)(128 * ks), ID_O, j > 0 || ks > 0);
+          if (w == (j < n1 ? 1 : 0)) umma_commit(bar(EMPTY + (2 * j + 1) % NS));  // V_j has been used
         }
-        if (fail) break;
-        umma_commit(bar(V_EMPTY + s));
-        if (have_k) umma_commit(bar(K_EMPTY + (j + 1) % NS));
-      }
-      if (fail) *s_abort = 1;
-      // every product has completed before TMEM is released
-      if (issued) {
-        umma_commit(bar(DRAIN));
-        mbar_wait(bar(DRAIN), 0, kSitePkMma);
+        if (j + 1 < nw) {
+          issue_s(w, j + 1, w == (j + 1 < n1 ? 1 : 0));  // over P_w(j): products run in the order of their issue
+        } else if (lead) {
+          umma_commit(bar(O_DONE + w));
+        }
       }
     }
-    __syncwarp();
+    if (fail && lane == 0) *s_abort = 1;
+    // every product has completed before TMEM is released
+    if (lead) umma_commit(bar(DRAIN));
+    wait(bar(DRAIN), 0);
   } else if (warp < 4) {
     // ------------------------------------------------------------ clean tiles
     regs_dec<56>();
-    const int t = tid - 64;  // 0 .. 63: keys t and t + 64 of a tile
     auto gate_at = [&](int key) {
       if constexpr (!GATED) return 0.f;
       return key < tile.n ? a.lg[(long long)(seq0 + key) * a.Hk + hk] * kPkLog2e : 0.f;
     };
     bool ok = true;
     int j = GATED ? 0 : care;
-    float g0 = gate_at(128 * j + t), g1 = gate_at(128 * j + t + 64);
+    const int t = tid - 64;
+    float g[2];  // of keys 64 i + t
+#pragma unroll
+    for (int i = 0; i < 2; ++i) g[i] = gate_at(128 * j + 64 * i + t);
     for (; j < nk; ++j) {
-      const int s = j % NS;
+      uint8_t *kt = slot_at(2 * j), *vt = slot_at(2 * j + 1);
       ok = ok && !*s_abort;
       if (j < care)
-        ok = ok && mbar_wait_sleep(bar(K_FULL + s), (j / NS) & 1, kSitePkClean) &&
-             mbar_wait_sleep(bar(V_FULL + s), (j / NS) & 1, kSitePkClean);
+        ok = ok && mbar_wait_sleep(bar(FULL + 2 * j % NS), (2 * j / NS) & 1, kSitePkClean) &&
+             mbar_wait_sleep(bar(FULL + (2 * j + 1) % NS), ((2 * j + 1) / NS) & 1, kSitePkClean);
       else
         ok = ok && mbar_wait_sleep(bar(CARE_V + j - care), 0, kSitePkClean);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       if constexpr (GATED) {
-        gates[(j % kGateSlots) * 128 + t] = g0;
-        gates[(j % kGateSlots) * 128 + t + 64] = g1;
-        if (j < care) {
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            if ((half ? g1 : g0) != -INFINITY) continue;
-            const int key = t + 64 * half;
+        for (int i = 0; i < 2; ++i) {
+          gates[(j % GS) * 128 + 64 * i + t] = g[i];
+          if (j < care && g[i] == -INFINITY) {
 #pragma unroll
             for (int b = 0; b < NB; ++b)
 #pragma unroll
               for (int c = 0; c < 8; ++c) {
-                *reinterpret_cast<uint4*>(sK(s) + b * 16384 + key * 128 + c * 16) = make_uint4(0u, 0u, 0u, 0u);
-                *reinterpret_cast<uint4*>(sV(s) + b * 16384 + key * 128 + c * 16) = make_uint4(0u, 0u, 0u, 0u);
+                const int at = b * 16384 + (64 * i + t) * 128 + c * 16;
+                *reinterpret_cast<uint4*>(kt + at) = make_uint4(0u, 0u, 0u, 0u);
+                *reinterpret_cast<uint4*>(vt + at) = make_uint4(0u, 0u, 0u, 0u);
               }
           }
+          g[i] = gate_at(128 * (j + 1) + 64 * i + t);
         }
-        g0 = gate_at(128 * (j + 1) + t);
-        g1 = gate_at(128 * (j + 1) + t + 64);
       }
       if (j >= care) {
         constexpr uint32_t EXP = BF16 ? 0x7f80u : 0x7c00u;
-        uint4* vt = reinterpret_cast<uint4*>(sV(s));
+        uint4* ve = reinterpret_cast<uint4*>(vt);
         bool odd = false;
-#pragma unroll 4
+#pragma unroll 8
         for (int i = t; i < TILE / 16; i += 64) {
-          uint4 x = vt[i];
+          const uint4 x = ve[i];
           auto bad = [&](uint32_t w) {
             return (w & EXP) == EXP || (w & (EXP << 16)) == (EXP << 16);
           };
@@ -535,14 +561,14 @@ __global__ void __launch_bounds__(kPkThreads, 1)
               if ((w & (EXP << 16)) == (EXP << 16)) w &= 0xffffu;
               return w;
             };
-            vt[i] = make_uint4(fix(x.x), fix(x.y), fix(x.z), fix(x.w));
+            ve[i] = make_uint4(fix(x.x), fix(x.y), fix(x.z), fix(x.w));
           }
         }
         if (odd) *s_odd = 1;
       }
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(bar(j >= care ? CARE + j - care : CLEAN + s));
+      if (lane == 0) mbar_arrive(bar(j >= care ? CARE + j - care : CLEAN + j % kCleanSlots));
     }
     if (!ok) *s_abort = 1;
   } else {
@@ -564,13 +590,13 @@ __global__ void __launch_bounds__(kPkThreads, 1)
     };
     for (int j = 0; j < my_nk; ++j) {
       if (!warp_wait(bar(S_FULL + w), j & 1)) break;
-      if (GATED && !warp_wait(j >= care ? bar(CARE + j - care) : bar(CLEAN + j % NS), j >= care ? 0 : (j / NS) & 1)) break;
+      if (GATED && !warp_wait(j >= care ? bar(CARE + j - care) : bar(CLEAN + j % kCleanSlots), j >= care ? 0 : (j / kCleanSlots) & 1)) break;
       tc_fence_after();
       uint32_t sv[4][32];
 #pragma unroll
       for (int c = 0; c < 4; ++c) tmem_ld32(ts + 32 * c, sv[c]);
       tmem_wait_ld();
-      const float* g = gates + (j % kGateSlots) * 128;
+      const float* g = gates + (j % GS) * 128;
       float mp[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
       float mul = scale2;  // what the scores are still to be multiplied by
       if (j < care && (GATED || scale2 > 0.f)) {
@@ -737,10 +763,10 @@ cudaError_t packed_tc_t(const PackedArgs& a, cudaStream_t s) {
   const long long tiles = packed_tile_bound(a.T, a.R, k.pair ? 128 : 256);
   if (tiles > 65535) return cudaErrorInvalidValue;
   cudaError_t e = cudaFuncSetAttribute(sattn_packed_tc_kernel<T, D, GATED>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       (int)pk_smem<D>());
+                                       (int)pk_smem<D, GATED>());
   if (e != cudaSuccess) return e;
   sattn_packed_tc_kernel<T, D, GATED>
-      <<<dim3((unsigned)(k.pair ? a.Hq / 2 : a.Hq), (unsigned)tiles), kPkThreads, pk_smem<D>(), s>>>(mq, mk, mv, k);
+      <<<dim3((unsigned)(k.pair ? a.Hq / 2 : a.Hq), (unsigned)tiles), kPkThreads, pk_smem<D, GATED>(), s>>>(mq, mk, mv, k);
   return cudaGetLastError();
 }
 
