@@ -218,8 +218,10 @@ cudaError_t packed_simt_t(const PackedArgs& a, cudaStream_t s) {
 // (one exponential a score: 16 a clock and SM, just as long as the products of head_dim 128), so
 // every kPolyEvery-th pair of exponentials is a cubic on the FMA pipes.
 // TMEM columns: S_0 [0, 128) S_1 [128, 256) (P_w in the first 64 of S_w) O_0 [256, 256 + D) O_1 [384, 384 + D).
-// Every wait is bounded; a role that gives up records a site code, raises the CTA's abort flag and
-// leaves its loop.
+// Every wait is bounded; a role that gives up records a site code and leaves its loop, and the others'
+// waits for it run out in turn. A CTA goes from one pair of tiles to the next (cluster launch control:
+// it cancels the launch of a CTA that has not begun and takes over its number): the next pair's
+// loads and first scores run while the last rows are written.
 // ===========================================================================
 using namespace sm100;
 
@@ -240,11 +242,11 @@ template <int D> constexpr int pk_slots() { return D == 128 ? 5 : 8; }
 // Gates of tile j + G may take the place of tile j's: V_{j + G} is loaded when element
 // 2 (j + G) + 1 - slots has been used, K_{j + 1} or V_j, that is after the softmaxes of tile j.
 template <int D> constexpr int pk_gate_slots() { return D == 128 ? 3 : 4; }
-template <int D> constexpr int pk_bar_bytes() { return D == 128 ? 256 : 320; }
+template <int D> constexpr int pk_bar_bytes() { return D == 128 ? 304 : 352; }
 template <int D, bool GATED> constexpr size_t pk_smem() {
   return 1024 + (size_t)(2 + pk_slots<D>()) * pk_tile_bytes<D>() + (GATED ? pk_gate_slots<D>() * 128 * 4 : 0) + pk_bar_bytes<D>();
 }
-static_assert(pk_smem<128, true>() + sizeof(PackedTile) + 16 <= 227 * 1024, "shared memory of a CTA");
+static_assert(pk_smem<128, true>() + 96 <= 227 * 1024, "shared memory of a CTA");
 
 __device__ __forceinline__ float pk_ex2(float x) {
   float y;
@@ -327,6 +329,37 @@ struct PackedTcArgs {
   float scale;
 };
 
+// A CTA's pair of tiles, as the loading warp hands it to the others.
+struct PackedWork {
+  int seq0, q0, n;  // the sequence's first token, the (first) tile's position, the sequence's length
+  int head;         // the first tile's query head; < 0: no more work
+  int odd;          // elements of V were set to zero
+  __device__ __forceinline__ int tiles0() const { return q0 / 128 + 1; }                                    // key tiles
+  __device__ __forceinline__ int tiles1(int pair) const { return pair ? q0 / 128 + 1 : (q0 + 128 < n ? q0 / 128 + 2 : 0); }
+};
+
+// Asks for the launch of one more CTA of this grid to be cancelled; 16 bytes of answer go to `to`
+// and complete on `bar` (PTX ISA, clusterlaunchcontrol).
+__device__ __forceinline__ void ask_work(uint32_t to, uint32_t bar) {
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(to),
+               "r"(bar)
+               : "memory");
+}
+// The answer: the index of the cancelled CTA, x = -1 when there was none left.
+__device__ __forceinline__ int2 work_answer(uint32_t from) {
+  int2 c;
+  asm volatile(
+      "{\n\t.reg .b128 r;\n\t.reg .pred p;\n\t.reg .b32 z, w;\n\t"
+      "ld.shared.b128 r, [%2];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\t"
+      "mov.b32 %0, -1;\n\tmov.b32 %1, 0;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%0, %1, z, w}, r;\n\t}"
+      : "=r"(c.x), "=r"(c.y)
+      : "r"(from)
+      : "memory");
+  return c;
+}
+
 template <typename T, int D, bool GATED>
 __global__ void __launch_bounds__(kPkThreads, 1)
     sattn_packed_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
@@ -335,98 +368,134 @@ __global__ void __launch_bounds__(kPkThreads, 1)
   constexpr int NS = pk_slots<D>(), TILE = pk_tile_bytes<D>(), NB = D / 64;  // 64-column blocks of 16 KB
   constexpr int GS = pk_gate_slots<D>();
   extern __shared__ uint8_t smraw[];
-  __shared__ PackedTile s_tile;
   uint8_t* base = align1024_shared(smraw);
   uint8_t* sQ = base;
   auto slot_at = [&](int i) { return base + (2 + i % NS) * TILE; };  // of element i: K_j is 2 j, V_j 2 j + 1
   float* gates = reinterpret_cast<float*>(base + (2 + NS) * TILE);
   uint64_t* bars = reinterpret_cast<uint64_t*>(gates + (GATED ? pk_gate_slots<D>() * 128 : 0));
   enum {
-    Q_FULL = 0, FULL = 1, EMPTY = FULL + NS, CLEAN = EMPTY + NS, CARE_V = CLEAN + kCleanSlots, CARE = CARE_V + 2, S_FULL = CARE + 2, P_FULL = S_FULL + 2, O_DONE = P_FULL + 2,
-    DRAIN = O_DONE + 2, NBARS = DRAIN + 1
+    Q_FULL = 0, Q_EMPTY = 1, FULL = 2, EMPTY = FULL + NS, CLEAN = EMPTY + NS, CARE_V = CLEAN + kCleanSlots,
+    CARE = CARE_V + 2, S_FULL = CARE + 2, P_FULL = S_FULL + 2, O_DONE = P_FULL + 2, O_FREE = O_DONE + 2,
+    W_FULL = O_FREE + 2, W_EMPTY = W_FULL + 2, ANSWERED = W_EMPTY + 2, DRAIN = ANSWERED + 1, NBARS = DRAIN + 1
   };
-  static_assert(NBARS * 8 + 16 <= pk_bar_bytes<D>(), "barrier area");
   uint32_t* tslot = reinterpret_cast<uint32_t*>(bars + NBARS);
-  volatile int* s_abort = reinterpret_cast<volatile int*>(tslot + 1);
-  volatile int* s_odd = reinterpret_cast<volatile int*>(tslot + 2);
+  __shared__ __align__(16) uint8_t s_answer[16];
+  __shared__ volatile PackedWork s_work[2];
+  __shared__ PackedTile s_tile;
+  static_assert(NBARS * 8 + 8 <= pk_bar_bytes<D>(), "barrier area");
   auto bar = [&](int i) { return smem_u32(&bars[i]); };
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  if (warp == 0) {
-    find_packed_tile(a.cu, a.R, a.T, (int)blockIdx.y, a.pair ? 128 : 256, &s_tile);
-  } else if (warp == 1) {
-    tmem_alloc(smem_u32(tslot), 512);
-  } else if (tid == 64) {
+  if (warp == 1) tmem_alloc(smem_u32(tslot), 512);
+  if (tid == 64) {
     prefetch_tmap(&tm_q);
     prefetch_tmap(&tm_k);
     prefetch_tmap(&tm_v);
-    mbar_init(bar(Q_FULL), 1);
-    for (int s = 0; s < NS; ++s) {
-      mbar_init(bar(FULL + s), 1);
-      mbar_init(bar(EMPTY + s), 1);
+    for (int i = 0; i < NBARS; ++i) {
+      int n = 1;
+      if (i >= CLEAN && i < CLEAN + kCleanSlots) n = 2;  // two cleaning warps
+      if (i >= CARE && i < CARE + 2) n = 2;
+      if (i >= P_FULL && i < P_FULL + 2) n = 4;          // the four warps of a softmax
+      if (i >= O_FREE && i < O_FREE + 2) n = 4;
+      if (i >= W_EMPTY && i < W_EMPTY + 2) n = 11;       // every warp but the loading one
+      mbar_init(bar(i), n);
     }
-    for (int s = 0; s < kCleanSlots; ++s) mbar_init(bar(CLEAN + s), 2);
-    for (int w = 0; w < 2; ++w) {
-      mbar_init(bar(CARE_V + w), 1);
-      mbar_init(bar(CARE + w), 2);
-      mbar_init(bar(S_FULL + w), 1);
-      mbar_init(bar(P_FULL + w), 4);
-      mbar_init(bar(O_DONE + w), 1);
-    }
-    mbar_init(bar(DRAIN), 1);
-    *s_abort = 0;
-    *s_odd = 0;
     fence_mbar_init();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tslot;
-  const PackedTile tile = s_tile;
   T* out = reinterpret_cast<T*>(a.out);
-  if (tile.seq < 0) {  // nothing, or rows of no sequence
-    const int nh = a.pair ? 2 : 1, row = nh * D;
-    for (int i = tid; i < tile.rows * row; i += kPkThreads)
-      out[((long long)(tile.tok0 + i / row) * a.Hq + blockIdx.x * nh) * D + i % row] = from_f32<T>(0.f);
-    if (warp == 1) tmem_dealloc(tmem, 512);
-    return;
-  }
-  const int seq0 = tile.tok0 - tile.q0;  // the sequence's first token
-  const int q0[2] = {tile.q0, a.pair ? tile.q0 : tile.q0 + 128};
-  const int head[2] = {(int)blockIdx.x * (a.pair ? 2 : 1), (int)blockIdx.x * (a.pair ? 2 : 1) + (a.pair ? 1 : 0)};
-  const int hk = head[0] / (a.Hq / a.Hk);
-  const int nkw[2] = {q0[0] / 128 + 1, q0[1] < tile.n ? q0[1] / 128 + 1 : 0};
-  const int nk = max(nkw[0], nkw[1]);
-  const int care = nkw[0] - 1;  // key tiles from here on hold positions that some row does not see
   constexpr uint32_t T_S = 0, T_O = 256;
   // Registers: launched with 168 a thread (384 x 168 = 64512); warpgroup 0 keeps 56 and the two softmax
   // warpgroups take 208 each: 128 x 56 + 256 x 208 = 60416 <= 64512.
   static_assert(kPkThreads == 384, "register split assumes three warpgroups");
+  const int group = a.Hq / a.Hk;
+
+  // Work `it` of this CTA for the roles that use it (whole warps): false when a wait ran out.
+  auto next_work = [&](int it, PackedWork& w) {
+    if (!__all_sync(0xffffffffu, mbar_wait(bar(W_FULL + (it & 1)), (it >> 1) & 1, kSitePkLoad))) return false;
+    volatile PackedWork& s = s_work[it & 1];
+    w.seq0 = s.seq0, w.q0 = s.q0, w.n = s.n, w.head = s.head;
+    return true;
+  };
+  auto work_done = [&](int it) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar(W_EMPTY + (it & 1)));
+  };
 
   if (warp == 0) {
-    // ------------------------------------------------------------ loads
+    // ------------------------------------------------------------ work and loads
     regs_dec<56>();
-    if (lane == 0) {
-      const int nq = nkw[1] > 0 ? 2 : 1;
-      mbar_expect_tx(bar(Q_FULL), (uint32_t)(nq * TILE));
-      for (int w = 0; w < nq; ++w)
-#pragma unroll
-        for (int b = 0; b < NB; ++b)
-          tma_load_3d(smem_u32(sQ + w * TILE + b * 16384), &tm_q, 64 * b, seq0 + q0[w], head[w], bar(Q_FULL));
-      // the barrier and its parity that element i arrives on (V tiles that the cleaning warps wait for on their own)
-      auto full = [&](int i) { return bar((i & 1) && (i >> 1) >= care ? CARE_V + (i >> 1) - care : FULL + i % NS); };
-      auto parity = [&](int i) { return (i & 1) && (i >> 1) >= care ? 0 : (i / NS) & 1; };
-      int i = 0;
-      for (; i < 2 * nk; ++i) {
-        if (i >= NS && (!mbar_wait(bar(EMPTY + i % NS), ((i / NS) - 1) & 1, kSitePkLoad) || *s_abort)) break;
-        mbar_expect_tx(full(i), (uint32_t)TILE);
-#pragma unroll
-        for (int b = 0; b < NB; ++b)
-          tma_load_3d(smem_u32(slot_at(i) + b * 16384), i & 1 ? &tm_v : &tm_k, 64 * b, seq0 + 128 * (i >> 1), hk, full(i));
+    int2 c = make_int2((int)blockIdx.x, (int)blockIdx.y);
+    bool ok = true;
+    int it = 0, asked = 0, i0 = 0;  // works, answers, elements before this work
+    for (; c.x >= 0 && ok; ++asked) {
+      if (lane == 0) {
+        mbar_expect_tx(bar(ANSWERED), 16);
+        ask_work(smem_u32(s_answer), bar(ANSWERED));
       }
-      if (i < 2 * nk) *s_abort = 1;
-      // no copy may still be in flight when the CTA exits
-      mbar_wait(bar(Q_FULL), 0, kSitePkLoad);
-      for (int d = max(i - NS, 0); d < i; ++d) mbar_wait(full(d), parity(d), kSitePkLoad);
+      find_packed_tile(a.cu, a.R, a.T, c.y, a.pair ? 128 : 256, &s_tile);
+      __syncwarp();
+      const PackedTile tile = s_tile;
+      const int heads = a.pair ? 2 : 1, head = c.x * heads;
+      if (tile.seq < 0) {  // nothing, or rows of no sequence
+        const int row = heads * D / 8;  // 16-byte words of a token
+        for (int i = lane; i < tile.rows * row; i += 32)
+          *reinterpret_cast<uint4*>(out + ((long long)(tile.tok0 + i / row) * a.Hq + head) * D + i % row * 8) =
+              make_uint4(0u, 0u, 0u, 0u);
+      } else {
+        PackedWork w{tile.tok0 - tile.q0, tile.q0, tile.n, head, 0};
+        const int n0 = w.tiles0(), n1 = w.tiles1(a.pair), nk = max(n0, n1), care = n0 - 1, hk = head / group;
+        if (it >= 2) ok = __all_sync(0xffffffffu, mbar_wait(bar(W_EMPTY + (it & 1)), ((it >> 1) - 1) & 1, kSitePkLoad));
+        if (lane == 0 && ok) {
+          volatile PackedWork& s = s_work[it & 1];
+          s.seq0 = w.seq0, s.q0 = w.q0, s.n = w.n, s.head = w.head, s.odd = 0;
+          mbar_arrive(bar(W_FULL + (it & 1)));
+        }
+        if (ok && it > 0) ok = __all_sync(0xffffffffu, mbar_wait(bar(Q_EMPTY), (it - 1) & 1, kSitePkLoad));
+        if (ok) {
+          const int nq = n1 > 0 ? 2 : 1;
+          if (lane == 0) {
+            mbar_expect_tx(bar(Q_FULL), (uint32_t)(nq * TILE));
+            for (int t = 0; t < nq; ++t)
+#pragma unroll
+              for (int b = 0; b < NB; ++b)
+                tma_load_3d(smem_u32(sQ + t * TILE + b * 16384), &tm_q, 64 * b, w.seq0 + w.q0 + (a.pair ? 0 : 128 * t),
+                            head + (a.pair ? t : 0), bar(Q_FULL));
+          }
+          for (int e = 0; e < 2 * nk && ok; ++e) {
+            const int i = i0 + e, j = e >> 1, sl = i % NS;
+            if (i >= NS)
+              ok = __all_sync(0xffffffffu, mbar_wait(bar(EMPTY + sl), ((i / NS) - 1) & 1, kSitePkLoad));
+            if (!ok) break;
+            // V tiles that are to be cleaned arrive on a barrier of their own (the ring's goes on)
+            const bool special = (e & 1) && j >= care;
+            const uint32_t b_in = bar(special ? CARE_V + j - care : FULL + sl);
+            if (lane == 0) {
+              if (special) mbar_arrive(bar(FULL + sl));
+              mbar_expect_tx(b_in, (uint32_t)TILE);
+#pragma unroll
+              for (int b = 0; b < NB; ++b)
+                tma_load_3d(smem_u32(slot_at(i) + b * 16384), e & 1 ? &tm_v : &tm_k, 64 * b, w.seq0 + 128 * j, hk, b_in);
+            }
+          }
+          i0 += 2 * nk;
+        }
+        ++it;
+      }
+      if (!__all_sync(0xffffffffu, mbar_wait(bar(ANSWERED), asked & 1, kSitePkLoad))) ok = false;
+      c = work_answer(smem_u32(s_answer));
+      fence_proxy_async_smem();  // the answer has been read before the next one is written
+      __syncwarp();
+    }
+    if (ok && it >= 2) ok = __all_sync(0xffffffffu, mbar_wait(bar(W_EMPTY + (it & 1)), ((it >> 1) - 1) & 1, kSitePkLoad));
+    if (ok && lane == 0) {
+      s_work[it & 1].head = -1;
+      mbar_arrive(bar(W_FULL + (it & 1)));
+      // No copy may be in flight when the CTA exits: the last work has been used up. (After a wait that
+      // ran out, every copy has long arrived.)
+      if (it > 0) mbar_wait(bar(W_EMPTY + ((it - 1) & 1)), ((it - 1) >> 1) & 1, kSitePkLoad);
     }
     __syncwarp();
   } else if (warp == 1) {
@@ -437,296 +506,348 @@ __global__ void __launch_bounds__(kPkThreads, 1)
     regs_dec<56>();
     constexpr uint32_t ID_S = idesc_f16(128, 128, BF16, false, false);
     constexpr uint32_t ID_O = idesc_f16(128, D, BF16, false, true);
-    const int n0 = __shfl_sync(0xffffffffu, nkw[0], 0), n1 = __shfl_sync(0xffffffffu, nkw[1], 0);
-    const int first_care = __shfl_sync(0xffffffffu, care, 0), nkt = max(n0, n1);
     const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
     const uint32_t qd = desc_lo(__shfl_sync(0xffffffffu, smem_u32(sQ), 0), 16);
     const uint32_t kd = desc_lo(__shfl_sync(0xffffffffu, smem_u32(slot_at(0)), 0), 16);
     const uint32_t vd = desc_lo(__shfl_sync(0xffffffffu, smem_u32(slot_at(0)), 0), 16384);
     const bool lead = elect_one();
     auto wait = [&](uint32_t b, uint32_t parity) { return (bool)__all_sync(0xffffffffu, mbar_wait(b, parity, kSitePkMma)); };
-    auto ready_k = [&](int j) {  // tile j of K, clean where it has to be
-      if (GATED && j < first_care) return wait(bar(CLEAN + j % kCleanSlots), (j / kCleanSlots) & 1);
-      return wait(bar(FULL + 2 * j % NS), (2 * j / NS) & 1);
-    };
-    auto ready_v = [&](int j) {
-      if (j >= first_care) return wait(bar(CARE + j - first_care), 0);
-      if (GATED) return wait(bar(CLEAN + j % kCleanSlots), (j / kCleanSlots) & 1);
-      return wait(bar(FULL + (2 * j + 1) % NS), ((2 * j + 1) / NS) & 1);
-    };
-    auto issue_s = [&](int w, int j, bool last) {
-      const uint32_t q1 = qd + (uint32_t)(w * (TILE >> 4)), k1 = kd + (uint32_t)((2 * j % NS) * (TILE >> 4));
-      if (lead) {
-#pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks) {
-          const uint32_t off = (uint32_t)(((ks >> 2) * 16384 + (ks & 3) * 32) >> 4);
-          mma_ss(tm + T_S + 128 * w, q1 + off, k1 + off, ID_S, ks > 0);
-        }
-        umma_commit(bar(S_FULL + w));
-        if (last) umma_commit(bar(EMPTY + 2 * j % NS));
-      }
-    };
-    bool fail = !wait(bar(Q_FULL), 0) || !ready_k(0);
-    if (!fail) {
-      tc_fence_after();
-      issue_s(0, 0, n1 == 0);
-      if (n1 > 0) issue_s(1, 0, true);
-    }
-    for (int j = 0; j < nkt && !fail && !__any_sync(0xffffffffu, *s_abort); ++j) {
-      const uint32_t v1 = vd + (uint32_t)(((2 * j + 1) % NS) * (TILE >> 4));
-      if (!ready_v(j) || (j + 1 < nkt && !ready_k(j + 1))) {
+    int i0 = 0, cleaned = 0, care_used[2] = {0, 0}, steps[2] = {0, 0}, outs[2] = {0, 0};
+    bool fail = false;
+    for (int it = 0; !fail; ++it) {
+      PackedWork work;
+      if (!next_work(it, work)) {
         fail = true;
         break;
       }
-#pragma unroll
-      for (int w = 0; w < 2; ++w) {
-        const int nw = w ? n1 : n0;
-        if (fail || j >= nw) continue;
-        if (!wait(bar(P_FULL + w), j & 1)) {
-          fail = true;
-          continue;
-        }
-        tc_fence_after();
+      work_done(it);
+      if (work.head < 0) break;
+      const int n0 = __shfl_sync(0xffffffffu, work.tiles0(), 0), n1 = __shfl_sync(0xffffffffu, work.tiles1(a.pair), 0);
+      const int first_care = n0 - 1, nkt = max(n0, n1);
+      auto ready_k = [&](int j) {  // tile j of K, clean where it has to be
+        if (GATED && j < first_care) return wait(bar(CLEAN + (cleaned + j) % kCleanSlots), ((cleaned + j) / kCleanSlots) & 1);
+        return wait(bar(FULL + (i0 + 2 * j) % NS), ((i0 + 2 * j) / NS) & 1);
+      };
+      auto ready_v = [&](int j) {
+        if (j >= first_care) return wait(bar(CARE + j - first_care), care_used[j - first_care]++ & 1);
+        if (GATED) return wait(bar(CLEAN + (cleaned + j) % kCleanSlots), ((cleaned + j) / kCleanSlots) & 1);
+        return wait(bar(FULL + (i0 + 2 * j + 1) % NS), ((i0 + 2 * j + 1) / NS) & 1);
+      };
+      auto issue_s = [&](int w, int j, bool last) {
+        const int sl = (i0 + 2 * j) % NS;
+        const uint32_t q1 = qd + (uint32_t)(w * (TILE >> 4)), k1 = kd + (uint32_t)(sl * (TILE >> 4));
         if (lead) {
 #pragma unroll
-          for (int ks = 0; ks < 8; ++ks)
-            mma_ts(tm + T_O + 128 * w, tm + T_S + 128 * w + 8 * ks, v1 + (uint32_t)(128 * ks), ID_O, j > 0 || ks > 0);
-          if (w == (j < n1 ? 1 : 0)) umma_commit(bar(EMPTY + (2 * j + 1) % NS));  // V_j has been used
+          for (int ks = 0; ks < D / 16; ++ks) {
+            const uint32_t off = (uint32_t)(((ks >> 2) * 16384 + (ks & 3) * 32) >> 4);
+            mma_ss(tm + T_S + 128 * w, q1 + off, k1 + off, ID_S, ks > 0);
+          }
+          umma_commit(bar(S_FULL + w));
+          if (last) {
+            umma_commit(bar(EMPTY + sl));
+            if (j == nkt - 1) umma_commit(bar(Q_EMPTY));
+          }
         }
-        if (j + 1 < nw) {
-          issue_s(w, j + 1, w == (j + 1 < n1 ? 1 : 0));  // over P_w(j): products run in the order of their issue
-        } else if (lead) {
-          umma_commit(bar(O_DONE + w));
+      };
+      fail = !wait(bar(Q_FULL), it & 1) || !ready_k(0);
+      if (!fail) {
+        tc_fence_after();
+        issue_s(0, 0, n1 == 0);
+        if (n1 > 0) issue_s(1, 0, true);
+      }
+      for (int j = 0; j < nkt && !fail; ++j) {
+        const int sl = (i0 + 2 * j + 1) % NS;
+        const uint32_t v1 = vd + (uint32_t)(sl * (TILE >> 4));
+        if (!ready_v(j) || (j + 1 < nkt && !ready_k(j + 1))) {
+          fail = true;
+          break;
+        }
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          const int nw = w ? n1 : n0;
+          if (fail || j >= nw) continue;
+          // (the first product into O_w: the last work's rows have been read)
+          if (!wait(bar(P_FULL + w), steps[w]++ & 1) ||
+              (j == 0 && outs[w] > 0 && !wait(bar(O_FREE + w), (outs[w] - 1) & 1))) {
+            fail = true;
+            continue;
+          }
+          tc_fence_after();
+          if (lead) {
+#pragma unroll
+            for (int ks = 0; ks < 8; ++ks)
+              mma_ts(tm + T_O + 128 * w, tm + T_S + 128 * w + 8 * ks, v1 + (uint32_t)(128 * ks), ID_O, j > 0 || ks > 0);
+            if (w == (j < n1 ? 1 : 0)) umma_commit(bar(EMPTY + sl));  // V_j has been used
+          }
+          if (j + 1 < nw) {
+            issue_s(w, j + 1, w == (j + 1 < n1 ? 1 : 0));  // over P_w(j): products run in the order of their issue
+          } else {
+            if (lead) umma_commit(bar(O_DONE + w));
+            ++outs[w];
+          }
         }
       }
+      i0 += 2 * nkt;
+      cleaned += first_care;
     }
-    if (fail && lane == 0) *s_abort = 1;
     // every product has completed before TMEM is released
     if (lead) umma_commit(bar(DRAIN));
     wait(bar(DRAIN), 0);
   } else if (warp < 4) {
     // ------------------------------------------------------------ clean tiles
     regs_dec<56>();
-    auto gate_at = [&](int key) {
-      if constexpr (!GATED) return 0.f;
-      return key < tile.n ? a.lg[(long long)(seq0 + key) * a.Hk + hk] * kPkLog2e : 0.f;
-    };
+    const int t = tid - 64;  // 0 .. 63: keys t and t + 64 of a tile
+    int i0 = 0, cleaned = 0, tiles = 0, care_used[2] = {0, 0};
     bool ok = true;
-    int j = GATED ? 0 : care;
-    const int t = tid - 64;
-    float g[2];  // of keys 64 i + t
+    for (int it = 0; ok; ++it) {
+      PackedWork work;
+      ok = next_work(it, work);
+      if (!ok || work.head < 0) break;
+      const int care = work.tiles0() - 1, nk = max(work.tiles0(), work.tiles1(a.pair)), hk = work.head / group;
+      auto gate_at = [&](int key) {
+        if constexpr (!GATED) return 0.f;
+        return key < work.n ? a.lg[(long long)(work.seq0 + key) * a.Hk + hk] * kPkLog2e : 0.f;
+      };
+      int j = GATED ? 0 : care;
+      float g0 = gate_at(128 * j + t), g1 = gate_at(128 * j + t + 64);
+      for (; j < nk; ++j) {
+        const int ik = i0 + 2 * j;
+        uint8_t *kt = slot_at(ik), *vt = slot_at(ik + 1);
+        // (with gates also K of the tiles that are not changed here: the ring's phases are followed one by one)
+        if (GATED) ok = mbar_wait_sleep(bar(FULL + ik % NS), (ik / NS) & 1, kSitePkClean);
+        if (j < care)
+          ok = ok && mbar_wait_sleep(bar(FULL + (ik + 1) % NS), ((ik + 1) / NS) & 1, kSitePkClean);
+        else
+          ok = ok && mbar_wait_sleep(bar(CARE_V + j - care), care_used[j - care]++ & 1, kSitePkClean);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        if constexpr (GATED) {
+          gates[((tiles + j) % GS) * 128 + t] = g0;
+          gates[((tiles + j) % GS) * 128 + t + 64] = g1;
+          if (j < care) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) g[i] = gate_at(128 * j + 64 * i + t);
-    for (; j < nk; ++j) {
-      uint8_t *kt = slot_at(2 * j), *vt = slot_at(2 * j + 1);
-      ok = ok && !*s_abort;
-      if (j < care)
-        ok = ok && mbar_wait_sleep(bar(FULL + 2 * j % NS), (2 * j / NS) & 1, kSitePkClean) &&
-             mbar_wait_sleep(bar(FULL + (2 * j + 1) % NS), ((2 * j + 1) / NS) & 1, kSitePkClean);
-      else
-        ok = ok && mbar_wait_sleep(bar(CARE_V + j - care), 0, kSitePkClean);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-      if constexpr (GATED) {
+            for (int half = 0; half < 2; ++half) {
+              if ((half ? g1 : g0) != -INFINITY) continue;
+              const int key = t + 64 * half;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          gates[(j % GS) * 128 + 64 * i + t] = g[i];
-          if (j < care && g[i] == -INFINITY) {
+              for (int b = 0; b < NB; ++b)
 #pragma unroll
-            for (int b = 0; b < NB; ++b)
-#pragma unroll
-              for (int c = 0; c < 8; ++c) {
-                const int at = b * 16384 + (64 * i + t) * 128 + c * 16;
-                *reinterpret_cast<uint4*>(kt + at) = make_uint4(0u, 0u, 0u, 0u);
-                *reinterpret_cast<uint4*>(vt + at) = make_uint4(0u, 0u, 0u, 0u);
-              }
+                for (int c = 0; c < 8; ++c) {
+                  *reinterpret_cast<uint4*>(kt + b * 16384 + key * 128 + c * 16) = make_uint4(0u, 0u, 0u, 0u);
+                  *reinterpret_cast<uint4*>(vt + b * 16384 + key * 128 + c * 16) = make_uint4(0u, 0u, 0u, 0u);
+                }
+            }
           }
-          g[i] = gate_at(128 * (j + 1) + 64 * i + t);
+          g0 = gate_at(128 * (j + 1) + t);
+          g1 = gate_at(128 * (j + 1) + t + 64);
         }
-      }
-      if (j >= care) {
-        constexpr uint32_t EXP = BF16 ? 0x7f80u : 0x7c00u;
-        uint4* ve = reinterpret_cast<uint4*>(vt);
-        bool odd = false;
+        if (j >= care) {
+          constexpr uint32_t EXP = BF16 ? 0x7f80u : 0x7c00u;
+          uint4* ve = reinterpret_cast<uint4*>(vt);
+          bool odd = false;
 #pragma unroll 8
-        for (int i = t; i < TILE / 16; i += 64) {
-          const uint4 x = ve[i];
-          auto bad = [&](uint32_t w) {
-            return (w & EXP) == EXP || (w & (EXP << 16)) == (EXP << 16);
-          };
-          if (bad(x.x) || bad(x.y) || bad(x.z) || bad(x.w)) {
-            odd = true;
-            auto fix = [&](uint32_t w) {
-              if ((w & EXP) == EXP) w &= 0xffff0000u;
-              if ((w & (EXP << 16)) == (EXP << 16)) w &= 0xffffu;
-              return w;
+          for (int i = t; i < TILE / 16; i += 64) {
+            const uint4 x = ve[i];
+            auto bad = [&](uint32_t w) {
+              return (w & EXP) == EXP || (w & (EXP << 16)) == (EXP << 16);
             };
-            ve[i] = make_uint4(fix(x.x), fix(x.y), fix(x.z), fix(x.w));
+            if (bad(x.x) || bad(x.y) || bad(x.z) || bad(x.w)) {
+              odd = true;
+              auto fix = [&](uint32_t w) {
+                if ((w & EXP) == EXP) w &= 0xffff0000u;
+                if ((w & (EXP << 16)) == (EXP << 16)) w &= 0xffffu;
+                return w;
+              };
+              ve[i] = make_uint4(fix(x.x), fix(x.y), fix(x.z), fix(x.w));
+            }
           }
+          if (odd) s_work[it & 1].odd = 1;
         }
-        if (odd) *s_odd = 1;
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(j >= care ? CARE + j - care : CLEAN + (cleaned + j) % kCleanSlots));
       }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar(j >= care ? CARE + j - care : CLEAN + j % kCleanSlots));
+      i0 += 2 * nk;
+      cleaned += care;
+      tiles += nk;
+      work_done(it);
     }
-    if (!ok) *s_abort = 1;
   } else {
     // ------------------------------------------------------------ softmax of tile w
     regs_inc<208>();
     const int w = (warp - 4) >> 2;
     const int r = (warp & 3) * 32 + lane;
     const uint32_t tl = (uint32_t)((warp & 3) * 32) << 16;
-    const int my_nk = w ? nkw[1] : nkw[0];
-    const int qi = (w ? q0[1] : q0[0]) + r;
     const uint32_t ts = tmem + tl + T_S + 128 * w, to = tmem + tl + T_O + 128 * w;
     const float scale2 = a.scale * kPkLog2e;
-    float m_used = -INFINITY, lsum = 0.f;
-    bool not_a_number = false;  // the row has a score of NaN or +inf
+    int tiles = 0, cleaned = 0, care_used[2] = {0, 0}, steps = 0, outs = 0;
     bool wfail = false;
     auto warp_wait = [&](uint32_t b, uint32_t parity) {
       if (!wfail) wfail = !__all_sync(0xffffffffu, mbar_wait(b, parity, kSitePkSoft));
       return !wfail;
     };
-    for (int j = 0; j < my_nk; ++j) {
-      if (!warp_wait(bar(S_FULL + w), j & 1)) break;
-      if (GATED && !warp_wait(j >= care ? bar(CARE + j - care) : bar(CLEAN + j % kCleanSlots), j >= care ? 0 : (j / kCleanSlots) & 1)) break;
-      tc_fence_after();
-      uint32_t sv[4][32];
+    for (int it = 0; !wfail; ++it) {
+      PackedWork work;
+      wfail = !next_work(it, work);
+      if (wfail || work.head < 0) break;
+      const int care = work.tiles0() - 1, nk0 = work.tiles0(), nk1 = work.tiles1(a.pair), my_nk = w ? nk1 : nk0;
+      const int qi = work.q0 + (a.pair ? 0 : 128 * w) + r;
+      float m_used = -INFINITY, lsum = 0.f;
+      bool not_a_number = false;  // the row has a score of NaN or +inf
+      for (int j = 0; j < my_nk; ++j) {
+        if (!warp_wait(bar(S_FULL + w), steps & 1)) break;
+        ++steps;
+        if (GATED && !warp_wait(j >= care ? bar(CARE + j - care) : bar(CLEAN + (cleaned + j) % kCleanSlots),
+                                j >= care ? (care_used[j - care] & 1) : ((cleaned + j) / kCleanSlots) & 1))
+          break;
+        tc_fence_after();
+        uint32_t sv[4][32];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld32(ts + 32 * c, sv[c]);
-      tmem_wait_ld();
-      const float* g = gates + (j % GS) * 128;
-      float mp[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-      float mul = scale2;  // what the scores are still to be multiplied by
-      if (j < care && (GATED || scale2 > 0.f)) {
-        if constexpr (GATED) {
-          const uint64_t sc2 = pk2(scale2, scale2);
+        for (int c = 0; c < 4; ++c) tmem_ld32(ts + 32 * c, sv[c]);
+        tmem_wait_ld();
+        const float* g = gates + ((tiles + j) % GS) * 128;
+        float mp[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        float mul = scale2;  // what the scores are still to be multiplied by
+        if (j < care && (GATED || scale2 > 0.f)) {
+          if constexpr (GATED) {
+            const uint64_t sc2 = pk2(scale2, scale2);
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+              for (int e = 0; e < 32; e += 4) {
+                const float4 gg = *reinterpret_cast<const float4*>(g + 32 * c + e);
+                const uint64_t x0 = fma2(pk2(__uint_as_float(sv[c][e]), __uint_as_float(sv[c][e + 1])), sc2, pk2(gg.x, gg.y));
+                const uint64_t x1 = fma2(pk2(__uint_as_float(sv[c][e + 2]), __uint_as_float(sv[c][e + 3])), sc2, pk2(gg.z, gg.w));
+                sv[c][e] = (uint32_t)x0, sv[c][e + 1] = (uint32_t)(x0 >> 32);
+                sv[c][e + 2] = (uint32_t)x1, sv[c][e + 3] = (uint32_t)(x1 >> 32);
+              }
+            mul = 1.f;
+          }
+        } else {
+          // own position, later ones and dropped keys
 #pragma unroll
           for (int c = 0; c < 4; ++c)
 #pragma unroll
-            for (int e = 0; e < 32; e += 4) {
-              const float4 gg = *reinterpret_cast<const float4*>(g + 32 * c + e);
-              const uint64_t x0 = fma2(pk2(__uint_as_float(sv[c][e]), __uint_as_float(sv[c][e + 1])), sc2, pk2(gg.x, gg.y));
-              const uint64_t x1 = fma2(pk2(__uint_as_float(sv[c][e + 2]), __uint_as_float(sv[c][e + 3])), sc2, pk2(gg.z, gg.w));
-              sv[c][e] = (uint32_t)x0, sv[c][e + 1] = (uint32_t)(x0 >> 32);
-              sv[c][e + 2] = (uint32_t)x1, sv[c][e + 3] = (uint32_t)(x1 >> 32);
+            for (int e = 0; e < 32; ++e) {
+              const int key = 128 * j + 32 * c + e;
+              const float gg = GATED ? g[32 * c + e] : 0.f;
+              const float x = fmaf(__uint_as_float(sv[c][e]), scale2, key < qi ? gg : 0.f);
+              sv[c][e] = __float_as_uint(key == qi || (key < qi && gg != -INFINITY) ? x : -INFINITY);
             }
           mul = 1.f;
         }
-      } else {
-        // own position, later ones and dropped keys
 #pragma unroll
         for (int c = 0; c < 4; ++c)
 #pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            const int key = 128 * j + 32 * c + e;
-            const float gg = GATED ? g[32 * c + e] : 0.f;
-            const float x = fmaf(__uint_as_float(sv[c][e]), scale2, key < qi ? gg : 0.f);
-            sv[c][e] = __float_as_uint(key == qi || (key < qi && gg != -INFINITY) ? x : -INFINITY);
+          for (int e = 0; e < 32; e += 4)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) mp[q] = max_nan(mp[q], __uint_as_float(sv[c][e + q]));
+        const float mt = max_nan(max_nan(mp[0], mp[1]), max_nan(mp[2], mp[3])) * mul;
+        if (!(mt < INFINITY)) not_a_number = true;
+        float f = 1.f;
+        bool resc = false;
+        if (mt < INFINITY && mt > m_used + kPkRescale) {
+          if (m_used != -INFINITY) {  // O and the sum hold earlier tiles: rescale them
+            f = pk_ex2(m_used - mt);
+            lsum *= f;
+            resc = true;
           }
-        mul = 1.f;
-      }
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-#pragma unroll
-        for (int e = 0; e < 32; e += 4)
-#pragma unroll
-          for (int q = 0; q < 4; ++q) mp[q] = max_nan(mp[q], __uint_as_float(sv[c][e + q]));
-      const float mt = max_nan(max_nan(mp[0], mp[1]), max_nan(mp[2], mp[3])) * mul;
-      if (!(mt < INFINITY)) not_a_number = true;
-      float f = 1.f;
-      bool resc = false;
-      if (mt < INFINITY && mt > m_used + kPkRescale) {
-        if (m_used != -INFINITY) {  // O and the sum hold earlier tiles: rescale them
-          f = pk_ex2(m_used - mt);
-          lsum *= f;
-          resc = true;
+          m_used = mt;
         }
-        m_used = mt;
-      }
-      // S_w(j) is complete, and with it the products before it: O_w holds the tiles up to j - 1
-      if (__any_sync(0xffffffffu, resc)) {
+        // S_w(j) is complete, and with it the products before it: O_w holds the tiles up to j - 1
+        if (__any_sync(0xffffffffu, resc)) {
 #pragma unroll
-        for (int c = 0; c < D / 16; ++c) {
-          uint32_t o[16];
-          tmem_ld16(to + 16 * c, o);
-          tmem_wait_ld();
+          for (int c = 0; c < D / 16; ++c) {
+            uint32_t o[16];
+            tmem_ld16(to + 16 * c, o);
+            tmem_wait_ld();
 #pragma unroll
-          for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-          tmem_st16(to + 16 * c, o);
+            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+            tmem_st16(to + 16 * c, o);
+          }
         }
-      }
-      const float mb = m_used == -INFINITY ? 0.f : -m_used;
-      const uint64_t mul2 = pk2(mul, mul), mb2 = pk2(mb, mb);
-      uint64_t ls[2] = {0ull, 0ull};
-      auto weights = [&](auto cubic) {
+        const float mb = m_used == -INFINITY ? 0.f : -m_used;
+        const uint64_t mul2 = pk2(mul, mul), mb2 = pk2(mb, mb);
+        uint64_t ls[2] = {0ull, 0ull};
+        auto weights = [&](auto cubic) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t pk[16];
+          for (int c = 0; c < 4; ++c) {
+            uint32_t pk[16];
 #pragma unroll
-          for (int q = 0; q < 16; ++q) {
-            const uint64_t d = fma2(pk2(__uint_as_float(sv[c][2 * q]), __uint_as_float(sv[c][2 * q + 1])), mul2, mb2);
-            uint64_t p;
-            if (decltype(cubic)::value && kPolyEvery > 0 && q % (kPolyEvery > 0 ? kPolyEvery : 1) == 0) {
-              p = ex2_fma(d);
-            } else {
-              p = pk2(pk_ex2(lo2(d)), pk_ex2(hi2(d)));
+            for (int q = 0; q < 16; ++q) {
+              const uint64_t d = fma2(pk2(__uint_as_float(sv[c][2 * q]), __uint_as_float(sv[c][2 * q + 1])), mul2, mb2);
+              uint64_t p;
+              if (decltype(cubic)::value && kPolyEvery > 0 && q % (kPolyEvery > 0 ? kPolyEvery : 1) == 0) {
+                p = ex2_fma(d);
+              } else {
+                p = pk2(pk_ex2(lo2(d)), pk_ex2(hi2(d)));
+              }
+              ls[q & 1] = add2(ls[q & 1], p);
+              pk[q] = pack2<T>(lo2(p), hi2(p));
             }
-            ls[q & 1] = add2(ls[q & 1], p);
-            pk[q] = pack2<T>(lo2(p), hi2(p));
+            tmem_st16(ts + 16 * c, pk);  // (the scores of these columns are in registers)
           }
-          tmem_st16(ts + 16 * c, pk);  // (the scores of these columns are in registers)
-        }
-      };
-      // 2^-125 is no 0 to a large V: where positions are masked every exponential is the hardware's
-      if (j < care)
-        weights(std::true_type{});
-      else
-        weights(std::false_type{});
-      const uint64_t l2 = add2(ls[0], ls[1]);
-      lsum += lo2(l2) + hi2(l2);
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar(P_FULL + w));
-    }
-    if (!wfail && my_nk > 0 && warp_wait(bar(O_DONE + w), 0)) {
-      tc_fence_after();
-      const float inv = not_a_number ? __uint_as_float(0x7fffffffu) : 1.0f / lsum;
-      const bool odd = *s_odd != 0;
-      T* op = out + ((long long)(seq0 + qi) * a.Hq + (w ? head[1] : head[0])) * D;
+        };
+        // 2^-125 is no 0 to a large V: where positions are masked every exponential is the hardware's
+        if (j < care)
+          weights(std::true_type{});
+        else
+          weights(std::false_type{});
+        const uint64_t l2 = add2(ls[0], ls[1]);
+        lsum += lo2(l2) + hi2(l2);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(P_FULL + w));
+      }
+      if (my_nk > 0 && warp_wait(bar(O_DONE + w), outs & 1)) {
+        ++outs;
+        tc_fence_after();
+        const float inv = not_a_number ? __uint_as_float(0x7fffffffu) : 1.0f / lsum;
+        const bool odd = s_work[it & 1].odd != 0;
+        const int hk = work.head / group, head = work.head + (a.pair ? w : 0);
+        T* op = out + ((long long)(work.seq0 + qi) * a.Hq + head) * D;
 #pragma unroll
-      for (int c = 0; c < D / 32; ++c) {
-        uint32_t o[32];
-        tmem_ld32(to + 32 * c, o);
-        tmem_wait_ld();
-        if (qi < tile.n) {
-          if (odd) {
-            // the elements of V that were set to zero, for the rows that see them
-            for (int key = 128 * care; key <= qi; ++key) {
-              if (GATED && key < qi && a.lg[(long long)(seq0 + key) * a.Hk + hk] == -INFINITY) continue;
-              const T* vp = reinterpret_cast<const T*>(a.v) + (seq0 + key) * a.v_ts + hk * a.v_hs + 32 * c;
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t o[32];
+          tmem_ld32(to + 32 * c, o);
+          tmem_wait_ld();
+          if (c == D / 32 - 1) {  // O_w has been read
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(O_FREE + w));
+          }
+          if (qi < work.n) {
+            if (odd) {
+              // the elements of V that were set to zero, for the rows that see them
+              for (int key = 128 * care; key <= qi; ++key) {
+                if (GATED && key < qi && a.lg[(long long)(work.seq0 + key) * a.Hk + hk] == -INFINITY) continue;
+                const T* vp = reinterpret_cast<const T*>(a.v) + (work.seq0 + key) * a.v_ts + hk * a.v_hs + 32 * c;
 #pragma unroll
-              for (int e = 0; e < 32; ++e) {
-                const float x = to_f32<T>(vp[e]);
-                if (!(fabsf(x) < INFINITY)) o[e] = __float_as_uint(__uint_as_float(o[e]) + x);
+                for (int e = 0; e < 32; ++e) {
+                  const float x = to_f32<T>(vp[e]);
+                  if (!(fabsf(x) < INFINITY)) o[e] = __float_as_uint(__uint_as_float(o[e]) + x);
+                }
               }
             }
-          }
 #pragma unroll
-          for (int e = 0; e < 32; e += 8) {
-            uint4 y;
-            y.x = pack2<T>(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv);
-            y.y = pack2<T>(__uint_as_float(o[e + 2]) * inv, __uint_as_float(o[e + 3]) * inv);
-            y.z = pack2<T>(__uint_as_float(o[e + 4]) * inv, __uint_as_float(o[e + 5]) * inv);
-            y.w = pack2<T>(__uint_as_float(o[e + 6]) * inv, __uint_as_float(o[e + 7]) * inv);
-            *reinterpret_cast<uint4*>(op + 32 * c + e) = y;
+            for (int e = 0; e < 32; e += 8) {
+              uint4 y;
+              y.x = pack2<T>(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv);
+              y.y = pack2<T>(__uint_as_float(o[e + 2]) * inv, __uint_as_float(o[e + 3]) * inv);
+              y.z = pack2<T>(__uint_as_float(o[e + 4]) * inv, __uint_as_float(o[e + 5]) * inv);
+              y.w = pack2<T>(__uint_as_float(o[e + 6]) * inv, __uint_as_float(o[e + 7]) * inv);
+              *reinterpret_cast<uint4*>(op + 32 * c + e) = y;
+            }
           }
         }
       }
+      tiles += max(nk0, nk1);
+      cleaned += care;
+      ++care_used[0];
+      if (max(nk0, nk1) > nk0) ++care_used[1];
+      work_done(it);
     }
-    if (wfail) *s_abort = 1;
   }
   tc_fence_before();
   __syncthreads();
