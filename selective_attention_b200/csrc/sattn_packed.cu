@@ -57,7 +57,12 @@ __global__ void __launch_bounds__(256) sattn_packed_kernel(const T* __restrict__
   float* Ps = Vs + kPT * LD;
   float* gs = Ps + kPT * LDP;
   const int tid = threadIdx.x, tr = tid >> 4, tc = tid & 15;
-  if (tid < 32) find_packed_tile(cu, R, Tn, (int)blockIdx.y, kPT, &s_tile);
+  if (tid < 32) {
+    PackedFinder<6> finder;
+    finder.init(cu, R, Tn);
+    const PackedTile t = finder.find((int)blockIdx.y);
+    if (tid == 0) s_tile = t;
+  }
   __syncthreads();
   const PackedTile tile = s_tile;
   if (tile.rows <= 0) return;
@@ -319,12 +324,28 @@ __device__ __forceinline__ bool elect_one() {
   return x != 0;
 }
 
+// 64 bytes of one thread, as two whole 32-byte sectors where the address allows it.
+__device__ __forceinline__ void store64(void* p, const uint32_t (&y)[16], bool wide) {
+  if (wide) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(reinterpret_cast<char*>(p) + 32 * i),
+                   "r"(y[8 * i]), "r"(y[8 * i + 1]), "r"(y[8 * i + 2]), "r"(y[8 * i + 3]), "r"(y[8 * i + 4]),
+                   "r"(y[8 * i + 5]), "r"(y[8 * i + 6]), "r"(y[8 * i + 7])
+                   : "memory");
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      reinterpret_cast<uint4*>(p)[i] = make_uint4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
+  }
+}
+
 struct PackedTcArgs {
   const float* lg;
   const int* cu;
   const void* v;
   void* out;
-  int R, T, Hq, Hk, pair;  // pair: a CTA's tiles are two heads
+  int R, T, Hq, Hk;
   long long v_ts, v_hs;
   float scale;
 };
@@ -335,7 +356,7 @@ struct PackedWork {
   int head;         // the first tile's query head; < 0: no more work
   int odd;          // elements of V were set to zero
   __device__ __forceinline__ int tiles0() const { return q0 / 128 + 1; }                                    // key tiles
-  __device__ __forceinline__ int tiles1(int pair) const { return pair ? q0 / 128 + 1 : (q0 + 128 < n ? q0 / 128 + 2 : 0); }
+  __device__ __forceinline__ int tiles1(bool pair) const { return pair ? q0 / 128 + 1 : (q0 + 128 < n ? q0 / 128 + 2 : 0); }
 };
 
 // Asks for the launch of one more CTA of this grid to be cancelled; 16 bytes of answer go to `to`
@@ -360,7 +381,8 @@ __device__ __forceinline__ int2 work_answer(uint32_t from) {
   return c;
 }
 
-template <typename T, int D, bool GATED>
+// PAIR: the two tiles are two heads.
+template <typename T, int D, bool GATED, bool PAIR>
 __global__ void __launch_bounds__(kPkThreads, 1)
     sattn_packed_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                            const __grid_constant__ CUtensorMap tm_v, const PackedTcArgs a) {
@@ -381,7 +403,6 @@ __global__ void __launch_bounds__(kPkThreads, 1)
   uint32_t* tslot = reinterpret_cast<uint32_t*>(bars + NBARS);
   __shared__ __align__(16) uint8_t s_answer[16];
   __shared__ volatile PackedWork s_work[2];
-  __shared__ PackedTile s_tile;
   static_assert(NBARS * 8 + 8 <= pk_bar_bytes<D>(), "barrier area");
   auto bar = [&](int i) { return smem_u32(&bars[i]); };
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -430,15 +451,15 @@ __global__ void __launch_bounds__(kPkThreads, 1)
     int2 c = make_int2((int)blockIdx.x, (int)blockIdx.y);
     bool ok = true;
     int it = 0, asked = 0, i0 = 0;  // works, answers, elements before this work
+    PackedFinder<PAIR ? 7 : 8> finder;
+    finder.init(a.cu, a.R, a.T);
     for (; c.x >= 0 && ok; ++asked) {
       if (lane == 0) {
         mbar_expect_tx(bar(ANSWERED), 16);
         ask_work(smem_u32(s_answer), bar(ANSWERED));
       }
-      find_packed_tile(a.cu, a.R, a.T, c.y, a.pair ? 128 : 256, &s_tile);
-      __syncwarp();
-      const PackedTile tile = s_tile;
-      const int heads = a.pair ? 2 : 1, head = c.x * heads;
+      const PackedTile tile = finder.find(c.y);
+      const int heads = PAIR ? 2 : 1, head = c.x * heads;
       if (tile.seq < 0) {  // nothing, or rows of no sequence
         const int row = heads * D / 8;  // 16-byte words of a token
         for (int i = lane; i < tile.rows * row; i += 32)
@@ -446,7 +467,7 @@ __global__ void __launch_bounds__(kPkThreads, 1)
               make_uint4(0u, 0u, 0u, 0u);
       } else {
         PackedWork w{tile.tok0 - tile.q0, tile.q0, tile.n, head, 0};
-        const int n0 = w.tiles0(), n1 = w.tiles1(a.pair), nk = max(n0, n1), care = n0 - 1, hk = head / group;
+        const int n0 = w.tiles0(), n1 = w.tiles1(PAIR), nk = max(n0, n1), care = n0 - 1, hk = head / group;
         if (it >= 2) ok = __all_sync(0xffffffffu, mbar_wait(bar(W_EMPTY + (it & 1)), ((it >> 1) - 1) & 1, kSitePkLoad));
         if (lane == 0 && ok) {
           volatile PackedWork& s = s_work[it & 1];
@@ -461,8 +482,8 @@ __global__ void __launch_bounds__(kPkThreads, 1)
             for (int t = 0; t < nq; ++t)
 #pragma unroll
               for (int b = 0; b < NB; ++b)
-                tma_load_3d(smem_u32(sQ + t * TILE + b * 16384), &tm_q, 64 * b, w.seq0 + w.q0 + (a.pair ? 0 : 128 * t),
-                            head + (a.pair ? t : 0), bar(Q_FULL));
+                tma_load_3d(smem_u32(sQ + t * TILE + b * 16384), &tm_q, 64 * b, w.seq0 + w.q0 + (PAIR ? 0 : 128 * t),
+                            head + (PAIR ? t : 0), bar(Q_FULL));
           }
           for (int e = 0; e < 2 * nk && ok; ++e) {
             const int i = i0 + e, j = e >> 1, sl = i % NS;
@@ -522,7 +543,7 @@ __global__ void __launch_bounds__(kPkThreads, 1)
       }
       work_done(it);
       if (work.head < 0) break;
-      const int n0 = __shfl_sync(0xffffffffu, work.tiles0(), 0), n1 = __shfl_sync(0xffffffffu, work.tiles1(a.pair), 0);
+      const int n0 = __shfl_sync(0xffffffffu, work.tiles0(), 0), n1 = __shfl_sync(0xffffffffu, work.tiles1(PAIR), 0);
       const int first_care = n0 - 1, nkt = max(n0, n1);
       auto ready_k = [&](int j) {  // tile j of K, clean where it has to be
         if (GATED && j < first_care) return wait(bar(CLEAN + (cleaned + j) % kCleanSlots), ((cleaned + j) / kCleanSlots) & 1);
@@ -603,7 +624,7 @@ __global__ void __launch_bounds__(kPkThreads, 1)
       PackedWork work;
       ok = next_work(it, work);
       if (!ok || work.head < 0) break;
-      const int care = work.tiles0() - 1, nk = max(work.tiles0(), work.tiles1(a.pair)), hk = work.head / group;
+      const int care = work.tiles0() - 1, nk = max(work.tiles0(), work.tiles1(PAIR)), hk = work.head / group;
       auto gate_at = [&](int key) {
         if constexpr (!GATED) return 0.f;
         return key < work.n ? a.lg[(long long)(work.seq0 + key) * a.Hk + hk] * kPkLog2e : 0.f;
@@ -642,22 +663,35 @@ __global__ void __launch_bounds__(kPkThreads, 1)
           g1 = gate_at(128 * (j + 1) + t + 64);
         }
         if (j >= care) {
-          constexpr uint32_t EXP = BF16 ? 0x7f80u : 0x7c00u;
+          // x * 0 is 0 but for infinities and NaN: four packed products for 16 bytes see whether there are
+          // any; only then are they looked for.
           uint4* ve = reinterpret_cast<uint4*>(vt);
-          bool odd = false;
+          using T2 = typename std::conditional<BF16, __nv_bfloat162, __half2>::type;
+          uint32_t zeros[4] = {0u, 0u, 0u, 0u};
 #pragma unroll 8
           for (int i = t; i < TILE / 16; i += 64) {
             const uint4 x = ve[i];
-            auto bad = [&](uint32_t w) {
-              return (w & EXP) == EXP || (w & (EXP << 16)) == (EXP << 16);
+            const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const uint32_t zero = 0u;
+              const T2 y = __hfma2(*reinterpret_cast<const T2*>(&xs[q]), *reinterpret_cast<const T2*>(&zero),
+                                   *reinterpret_cast<const T2*>(&zeros[q]));
+              zeros[q] = *reinterpret_cast<const uint32_t*>(&y);
+            }
+          }
+          bool odd = false;
+          // (a sum is +0, -0 or NaN)
+          if (((zeros[0] | zeros[1] | zeros[2] | zeros[3]) & 0x7fff7fffu) != 0u) {
+            constexpr uint32_t EXP = BF16 ? 0x7f80u : 0x7c00u;
+            odd = true;
+            auto fix = [&](uint32_t w) {
+              if ((w & EXP) == EXP) w &= 0xffff0000u;
+              if ((w & (EXP << 16)) == (EXP << 16)) w &= 0xffffu;
+              return w;
             };
-            if (bad(x.x) || bad(x.y) || bad(x.z) || bad(x.w)) {
-              odd = true;
-              auto fix = [&](uint32_t w) {
-                if ((w & EXP) == EXP) w &= 0xffff0000u;
-                if ((w & (EXP << 16)) == (EXP << 16)) w &= 0xffffu;
-                return w;
-              };
+            for (int i = t; i < TILE / 16; i += 64) {
+              const uint4 x = ve[i];
               ve[i] = make_uint4(fix(x.x), fix(x.y), fix(x.z), fix(x.w));
             }
           }
@@ -690,8 +724,8 @@ __global__ void __launch_bounds__(kPkThreads, 1)
       PackedWork work;
       wfail = !next_work(it, work);
       if (wfail || work.head < 0) break;
-      const int care = work.tiles0() - 1, nk0 = work.tiles0(), nk1 = work.tiles1(a.pair), my_nk = w ? nk1 : nk0;
-      const int qi = work.q0 + (a.pair ? 0 : 128 * w) + r;
+      const int care = work.tiles0() - 1, nk0 = work.tiles0(), nk1 = work.tiles1(PAIR), my_nk = w ? nk1 : nk0;
+      const int qi = work.q0 + (PAIR ? 0 : 128 * w) + r;
       float m_used = -INFINITY, lsum = 0.f;
       bool not_a_number = false;  // the row has a score of NaN or +inf
       for (int j = 0; j < my_nk; ++j) {
@@ -708,8 +742,9 @@ __global__ void __launch_bounds__(kPkThreads, 1)
         const float* g = gates + ((tiles + j) % GS) * 128;
         float mp[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
         float mul = scale2;  // what the scores are still to be multiplied by
-        if (j < care && (GATED || scale2 > 0.f)) {
-          if constexpr (GATED) {
+        if constexpr (GATED) {
+          mul = 1.f;
+          if (j < care) {
             const uint64_t sc2 = pk2(scale2, scale2);
 #pragma unroll
             for (int c = 0; c < 4; ++c)
@@ -721,20 +756,35 @@ __global__ void __launch_bounds__(kPkThreads, 1)
                 sv[c][e] = (uint32_t)x0, sv[c][e + 1] = (uint32_t)(x0 >> 32);
                 sv[c][e + 2] = (uint32_t)x1, sv[c][e + 3] = (uint32_t)(x1 >> 32);
               }
-            mul = 1.f;
+          } else {
+            // (the keys of these tiles are as they came: a dropped one's score may be a NaN)
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+              for (int e = 0; e < 32; ++e) {
+                const bool own = 128 * j + 32 * c + e == qi;
+                const float gg = g[32 * c + e], x = __uint_as_float(sv[c][e]) * scale2;
+                sv[c][e] = __float_as_uint(own ? x : (gg == -INFINITY ? -INFINITY : x + gg));
+              }
           }
-        } else {
-          // own position, later ones and dropped keys
+        } else if (!(scale2 > 0.f)) {  // (the largest score is not the largest product's then)
+          mul = 1.f;
 #pragma unroll
           for (int c = 0; c < 4; ++c)
 #pragma unroll
-            for (int e = 0; e < 32; ++e) {
-              const int key = 128 * j + 32 * c + e;
-              const float gg = GATED ? g[32 * c + e] : 0.f;
-              const float x = fmaf(__uint_as_float(sv[c][e]), scale2, key < qi ? gg : 0.f);
-              sv[c][e] = __float_as_uint(key == qi || (key < qi && gg != -INFINITY) ? x : -INFINITY);
-            }
-          mul = 1.f;
+            for (int e = 0; e < 32; ++e) sv[c][e] = __float_as_uint(__uint_as_float(sv[c][e]) * scale2);
+        }
+        if (j >= care) {
+          // Later positions. The warp's rows see all keys up to column `edge` of the tile and each lane
+          // one more than the lane before it: blocks of 32 columns up to there stay as they are.
+          const int edge = qi - lane - 128 * j;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            if (32 * c + 31 <= edge) continue;
+            const int last = edge + lane - 32 * c;  // the block's last column that the row sees
+#pragma unroll
+            for (int e = 0; e < 32; ++e) sv[c][e] = e > last ? __float_as_uint(-INFINITY) : sv[c][e];
+          }
         }
 #pragma unroll
         for (int c = 0; c < 4; ++c)
@@ -805,8 +855,9 @@ __global__ void __launch_bounds__(kPkThreads, 1)
         tc_fence_after();
         const float inv = not_a_number ? __uint_as_float(0x7fffffffu) : 1.0f / lsum;
         const bool odd = s_work[it & 1].odd != 0;
-        const int hk = work.head / group, head = work.head + (a.pair ? w : 0);
+        const int hk = work.head / group, head = work.head + (PAIR ? w : 0);
         T* op = out + ((long long)(work.seq0 + qi) * a.Hq + head) * D;
+        const bool wide = (reinterpret_cast<uintptr_t>(out) & 31u) == 0;
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) {
           uint32_t o[32];
@@ -830,15 +881,11 @@ __global__ void __launch_bounds__(kPkThreads, 1)
                 }
               }
             }
+            uint32_t y[16];
 #pragma unroll
-            for (int e = 0; e < 32; e += 8) {
-              uint4 y;
-              y.x = pack2<T>(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv);
-              y.y = pack2<T>(__uint_as_float(o[e + 2]) * inv, __uint_as_float(o[e + 3]) * inv);
-              y.z = pack2<T>(__uint_as_float(o[e + 4]) * inv, __uint_as_float(o[e + 5]) * inv);
-              y.w = pack2<T>(__uint_as_float(o[e + 6]) * inv, __uint_as_float(o[e + 7]) * inv);
-              *reinterpret_cast<uint4*>(op + 32 * c + e) = y;
-            }
+            for (int e = 0; e < 16; ++e)
+              y[e] = pack2<T>(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv);
+            store64(op + 32 * c, y, wide);
           }
         }
       }
@@ -867,7 +914,7 @@ bool make_map_packed(CUtensorMap* map, const void* base, bool bf16, int D, int T
              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename T, int D, bool GATED>
+template <typename T, int D, bool GATED, bool PAIR>
 cudaError_t packed_tc_t(const PackedArgs& a, cudaStream_t s) {
   const bool bf16 = std::is_same<T, __nv_bfloat16>::value;
   CUtensorMap mq, mk, mv;
@@ -878,23 +925,26 @@ cudaError_t packed_tc_t(const PackedArgs& a, cudaStream_t s) {
   PackedTcArgs k{};
   k.lg = a.log_gate, k.cu = a.cu, k.v = a.v, k.out = a.out;
   k.R = a.R, k.T = a.T, k.Hq = a.Hq, k.Hk = a.Hk;
-  k.pair = (a.Hq / a.Hk) % 2 == 0;
   k.v_ts = a.st.v_ts, k.v_hs = a.st.v_hs;
   k.scale = a.scale;
-  const long long tiles = packed_tile_bound(a.T, a.R, k.pair ? 128 : 256);
+  const long long tiles = packed_tile_bound(a.T, a.R, PAIR ? 128 : 256);
   if (tiles > 65535) return cudaErrorInvalidValue;
-  cudaError_t e = cudaFuncSetAttribute(sattn_packed_tc_kernel<T, D, GATED>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       (int)pk_smem<D, GATED>());
+  auto fn = sattn_packed_tc_kernel<T, D, GATED, PAIR>;
+  cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pk_smem<D, GATED>());
   if (e != cudaSuccess) return e;
-  sattn_packed_tc_kernel<T, D, GATED>
-      <<<dim3((unsigned)(k.pair ? a.Hq / 2 : a.Hq), (unsigned)tiles), kPkThreads, pk_smem<D, GATED>(), s>>>(mq, mk, mv, k);
+  fn<<<dim3((unsigned)(PAIR ? a.Hq / 2 : a.Hq), (unsigned)tiles), kPkThreads, pk_smem<D, GATED>(), s>>>(mq, mk, mv, k);
   return cudaGetLastError();
 }
 
 template <typename T>
 cudaError_t packed_tc(const PackedArgs& a, cudaStream_t s) {
-  if (a.D == 64) return a.log_gate ? packed_tc_t<T, 64, true>(a, s) : packed_tc_t<T, 64, false>(a, s);
-  return a.log_gate ? packed_tc_t<T, 128, true>(a, s) : packed_tc_t<T, 128, false>(a, s);
+  const bool pair = (a.Hq / a.Hk) % 2 == 0;
+  if (a.D == 64) {
+    if (a.log_gate) return pair ? packed_tc_t<T, 64, true, true>(a, s) : packed_tc_t<T, 64, true, false>(a, s);
+    return pair ? packed_tc_t<T, 64, false, true>(a, s) : packed_tc_t<T, 64, false, false>(a, s);
+  }
+  if (a.log_gate) return pair ? packed_tc_t<T, 128, true, true>(a, s) : packed_tc_t<T, 128, true, false>(a, s);
+  return pair ? packed_tc_t<T, 128, false, true>(a, s) : packed_tc_t<T, 128, false, false>(a, s);
 }
 
 }  // namespace
