@@ -156,7 +156,9 @@ def dtype_code(dt: torch.dtype, what: str) -> int:
 
 
 def stream_handle(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    # the raw handle, without a Stream object around it (0.2 us instead of 2)
+    index = device.index
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
 
 
 def check(status: int, what: str) -> None:

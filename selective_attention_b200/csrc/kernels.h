@@ -97,6 +97,20 @@ unsigned int fetch_error_sattn(cudaStream_t s);
 cudaError_t launch_sattn_attn_fa(const void* q, const void* k, const void* v, const float* lg, void* out, float* lse,
                                  int b, int H, int L, float scale, int dtype, int causal, cudaStream_t s);
 
+// A kernel's dynamic shared memory limit, set on its first launch on each device (the call costs as
+// much as a launch).
+template <typename F>
+inline cudaError_t allow_smem(F fn, size_t bytes, unsigned long long& done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const unsigned long long bit = 1ull << (dev & 63);
+  if (dev < 64 && (__atomic_load_n(&done, __ATOMIC_RELAXED) & bit)) return cudaSuccess;
+  e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (e == cudaSuccess) __atomic_fetch_or(&done, bit, __ATOMIC_RELAXED);
+  return e;
+}
+
 // paged.cu (the paged 8-bit key/value cache), paged_decode.cu (attention over it)
 struct PagedCache {
   unsigned char *k, *v;  // codes (pages, nkv, page, D)

@@ -722,8 +722,8 @@ cudaError_t decode_launch(DecodeArgs a, const PagedCache& c, cudaStream_t s) {
   if (!make_map_codes(&mk, c.k, D, c.page, (uint64_t)c.pages * c.nkv) ||
       !make_map_codes(&mv, c.v, D, c.page, (uint64_t)c.pages * c.nkv))
     return cudaErrorInvalidValue;
-  cudaError_t e = cudaFuncSetAttribute(paged_decode_kernel<T, C, D, NG>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       (int)smem);
+  static unsigned long long allowed = 0;
+  cudaError_t e = allow_smem(paged_decode_kernel<T, C, D, NG>, smem, allowed);
   if (e != cudaSuccess) return e;
   a.ngrp = (a.g + 8 * NG - 1) / (8 * NG);
   // no more CTAs than the table has tiles for

@@ -930,7 +930,8 @@ cudaError_t packed_tc_t(const PackedArgs& a, cudaStream_t s) {
   const long long tiles = packed_tile_bound(a.T, a.R, PAIR ? 128 : 256);
   if (tiles > 65535) return cudaErrorInvalidValue;
   auto fn = sattn_packed_tc_kernel<T, D, GATED, PAIR>;
-  cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pk_smem<D, GATED>());
+  static unsigned long long allowed = 0;
+  cudaError_t e = allow_smem(fn, pk_smem<D, GATED>(), allowed);
   if (e != cudaSuccess) return e;
   fn<<<dim3((unsigned)(PAIR ? a.Hq / 2 : a.Hq), (unsigned)tiles), kPkThreads, pk_smem<D, GATED>(), s>>>(mq, mk, mv, k);
   return cudaGetLastError();

@@ -14,17 +14,28 @@ Every launch goes on the current torch stream of the inputs' device; nothing syn
 """
 from __future__ import annotations
 
-from ctypes import byref, c_void_p
+import functools
+import struct
 from typing import Optional
 
 import torch
 
 from . import _lib
-from .kernels import _aligned16, _stream
+from .kernels import _aligned16
 from .utils import check_cuda, check_ndim, check_shape, to_contiguous
 
 PAGE_SIZES = (16, 32, 64, 128)
 CACHE_HEAD_DIMS = (32, 64, 128, 256)
+_I32, _I64, _F32 = torch.int32, torch.int64, torch.float32
+
+
+# Each call looks its arguments over in one expression, and where that fails goes through them one by
+# one for the message: on small inputs the checks would otherwise take longer than the kernel.
+
+# The C structs as bytes: building them field by field through ctypes takes longer than these calls'
+# kernels do on such inputs. (A test holds them against the ctypes mirrors.)
+_CACHE = struct.Struct("@qqqqi4xPPPPP")
+_PACKED = struct.Struct("@qqqqqqqqqqqiif4xPPPPPP")
 
 
 def _int32(t: torch.Tensor, name: str, shape=None) -> None:
@@ -32,6 +43,41 @@ def _int32(t: torch.Tensor, name: str, shape=None) -> None:
         raise ValueError(f"[{name}] expected a contiguous int32 tensor")
     if shape is not None:
         check_shape(t, shape, name)
+
+
+class _on:
+    """The device of a call's tensors as the current one (it mostly is)."""
+
+    def __init__(self, dev):
+        here = torch._C._cuda_getDevice()
+        self.guard = None if here == dev.index else torch.cuda.device(dev)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *e):
+        if self.guard is not None:
+            self.guard.__exit__(*e)
+
+
+def _plan_faults(lengths, new_lengths, block_table, free_pages, free_state, num_tokens, page_size) -> None:
+    check_ndim(lengths, 1, "lengths")
+    check_ndim(block_table, 2, "block_table")
+    check_ndim(free_pages, 1, "free_pages")
+    check_cuda((lengths, new_lengths, block_table, free_pages, free_state),
+               ("lengths", "new_lengths", "block_table", "free_pages", "free_state"))
+    R = block_table.shape[0]
+    _int32(lengths, "lengths", (R,))
+    _int32(new_lengths, "new_lengths", (R,))
+    _int32(block_table, "block_table")
+    _int32(free_pages, "free_pages")
+    if free_state.dtype != _I64 or not free_state.is_contiguous():
+        raise ValueError("[free_state] expected a contiguous int64 tensor")
+    check_shape(free_state, (2,), "free_state")
+    if page_size not in PAGE_SIZES:
+        raise ValueError(f"[page_size] {page_size} is not one of {PAGE_SIZES}")
+    raise ValueError(f"[num_tokens] {num_tokens} is negative")
 
 
 def sattn_paged_plan(lengths, new_lengths, block_table, free_pages, free_state, num_tokens: int, page_size: int):
@@ -49,39 +95,34 @@ def sattn_paged_plan(lengths, new_lengths, block_table, free_pages, free_state, 
     slots (page * page_size + place) and int32 positions, and the ring's new state. A request whose
     pages are not to be had keeps its length and gets slots of -1.
     """
-    check_ndim(lengths, 1, "lengths")
-    check_ndim(block_table, 2, "block_table")
-    check_ndim(free_pages, 1, "free_pages")
-    R, W = block_table.shape
-    dev = check_cuda([lengths, new_lengths, block_table, free_pages, free_state],
-                     ["lengths", "new_lengths", "block_table", "free_pages", "free_state"])
-    _int32(lengths, "lengths", (R,))
-    _int32(new_lengths, "new_lengths", (R,))
-    _int32(block_table, "block_table")
-    _int32(free_pages, "free_pages")
-    if free_state.dtype != torch.int64 or not free_state.is_contiguous():
-        raise ValueError("[free_state] expected a contiguous int64 tensor")
-    check_shape(free_state, (2,), "free_state")
-    if page_size not in PAGE_SIZES:
-        raise ValueError(f"[page_size] {page_size} is not one of {PAGE_SIZES}")
-    if num_tokens < 0:
-        raise ValueError(f"[num_tokens] {num_tokens} is negative")
+    d = lengths.get_device()
+    shape = block_table.shape
+    if not (d >= 0 and len(shape) == 2 and lengths.shape == new_lengths.shape == shape[:1]
+            and lengths.dtype == new_lengths.dtype == block_table.dtype == free_pages.dtype == _I32
+            and free_state.dtype == _I64 and free_state.shape == (2,) and len(free_pages.shape) == 1
+            and new_lengths.get_device() == block_table.get_device() == free_pages.get_device()
+            == free_state.get_device() == d and lengths.is_contiguous() and new_lengths.is_contiguous()
+            and block_table.is_contiguous() and free_pages.is_contiguous() and free_state.is_contiguous()
+            and page_size in PAGE_SIZES and num_tokens >= 0):
+        _plan_faults(lengths, new_lengths, block_table, free_pages, free_state, num_tokens, page_size)
+    R, W = shape
+    dev = lengths.device
     # the int32 outputs are parts of one allocation, as are the int64 ones
-    small = torch.empty(2 * R + 1 + num_tokens, device=dev, dtype=torch.int32)
-    large = torch.empty(num_tokens + 2, device=dev, dtype=torch.int64)
-    lengths_out, cu_new, positions = small[:R], small[R:2 * R + 1], small[2 * R + 1:]
-    slots, state_out = large[:num_tokens], large[num_tokens:]
-    with torch.cuda.device(dev):
+    lengths_out, cu_new, positions = torch.empty(2 * R + 1 + num_tokens, device=dev, dtype=torch.int32).split_with_sizes(
+        (R, R + 1, num_tokens))
+    slots, state_out = torch.empty(num_tokens + 2, device=dev, dtype=torch.int64).split_with_sizes((num_tokens, 2))
+    with _on(dev):
         st = _lib.lib().sattn_paged_plan(
-            _lib.ptr(lengths), _lib.ptr(new_lengths), _lib.ptr(block_table), _lib.ptr(free_pages),
-            _lib.ptr(free_state), _lib.ptr(lengths_out), _lib.ptr(cu_new), _lib.ptr(slots), _lib.ptr(positions),
-            _lib.ptr(state_out), R, W, free_pages.numel(), num_tokens, page_size, _stream(dev))
+            lengths.data_ptr(), new_lengths.data_ptr(), block_table.data_ptr(), free_pages.data_ptr(),
+            free_state.data_ptr(), lengths_out.data_ptr(), cu_new.data_ptr(), slots.data_ptr(), positions.data_ptr(),
+            state_out.data_ptr(), R, W, free_pages.shape[0], num_tokens, page_size, _lib.stream_handle(dev))
     _lib.check(st, "sattn_paged_plan")
     return lengths_out, cu_new, slots, positions, state_out
 
 
-def _cache(k_cache, v_cache, k_scale, v_scale, log_gate_cache) -> _lib.SattnCache:
-    """Checks a cache's tensors and describes them."""
+def _cache_faults(k_cache, v_cache, k_scale, v_scale, log_gate_cache) -> None:
+    """Says what is wrong with a cache's tensors."""
+    check_cuda((k_cache, v_cache, k_scale, v_scale, log_gate_cache), _CACHE_NAMES + ("log_gate_cache",))
     check_ndim(k_cache, 4, "k_cache")
     P, H, page, D = k_cache.shape
     if k_cache.dtype not in _lib.CACHE_CODES:
@@ -105,29 +146,61 @@ def _cache(k_cache, v_cache, k_scale, v_scale, log_gate_cache) -> _lib.SattnCach
     for t, n in ((k_cache, "k_cache"), (v_cache, "v_cache"), (log_gate_cache, "log_gate_cache")):
         if t is not None and t.data_ptr() % 16:
             raise ValueError(f"[{n}] must start on a 16-byte boundary")
-    return _lib.SattnCache(num_pages=P, nkv=H, page_size=page, head_dim=D, code=_lib.CACHE_CODES[k_cache.dtype],
-                           k_codes=_lib.ptr(k_cache), v_codes=_lib.ptr(v_cache), k_scale=_lib.ptr(k_scale),
-                           v_scale=_lib.ptr(v_scale), log_gate=_lib.ptr(log_gate_cache))
 
 
-_CACHE_NAMES = ["k_cache", "v_cache", "k_scale", "v_scale", "log_gate_cache"]
+def _cache(k_cache, v_cache, k_scale, v_scale, log_gate_cache):
+    """``(sattn_cache as bytes, heads, page size, head dim, device index)`` of checked tensors."""
+    shape, kind, dev = k_cache.shape, k_cache.dtype, k_cache.get_device()
+    kp, vp = k_cache.data_ptr(), v_cache.data_ptr()
+    gp = 0 if log_gate_cache is None else log_gate_cache.data_ptr()
+    good = (dev >= 0 and v_cache.get_device() == k_scale.get_device() == v_scale.get_device() == dev
+            and len(shape) == 4 and shape[2] in PAGE_SIZES and shape[3] in CACHE_HEAD_DIMS and v_cache.shape == shape
+            and kind in _lib.CACHE_CODES and v_cache.dtype == kind and k_scale.shape == shape[:2]
+            and v_scale.shape == shape[:2] and k_scale.dtype == _F32 and v_scale.dtype == _F32
+            and k_cache.is_contiguous() and v_cache.is_contiguous() and k_scale.is_contiguous()
+            and v_scale.is_contiguous() and not (kp | vp | gp) & 15)
+    if good and log_gate_cache is not None:
+        good = (log_gate_cache.shape == shape[:3] and log_gate_cache.dtype == _F32
+                and log_gate_cache.is_contiguous() and log_gate_cache.get_device() == dev)
+    if not good:
+        _cache_faults(k_cache, v_cache, k_scale, v_scale, log_gate_cache)
+    P, H, page, D = shape
+    return _CACHE.pack(P, H, page, D, _lib.CACHE_CODES[kind], kp, vp, k_scale.data_ptr(), v_scale.data_ptr(), gp), \
+        H, page, D, dev
 
 
-def _slots(slots) -> torch.Tensor:
-    check_ndim(slots, 1, "slots")
-    if slots.dtype != torch.int64:
-        raise ValueError(f"[slots] expected int64, got {slots.dtype}")
-    return to_contiguous(slots)
+_CACHE_NAMES = ("k_cache", "v_cache", "k_scale", "v_scale")
 
 
 def _rows(t: torch.Tensor):
     """``(tensor, token stride, head stride)`` of a (tokens, heads, D) tensor whose rows of D lie
     together; strides of dimensions of size one do not count and a broadcast one is written out."""
-    if (t.stride(2) != 1 and t.shape[2] > 1) or any(t.stride(i) == 0 and t.shape[i] > 1 for i in (0, 1)):
+    (n, h, d), (ts, hs, ds) = t.shape, t.stride()
+    if (ds != 1 and d > 1) or (ts == 0 and n > 1) or (hs == 0 and h > 1):
         t = t.contiguous()
-    hs = t.stride(1) if t.shape[1] > 1 else t.shape[2]
-    ts = t.stride(0) if t.shape[0] > 1 else t.shape[1] * hs
+        ts, hs, _ = t.stride()
+    if h == 1:
+        hs = d
+    if n == 1:
+        ts = h * hs
     return t, ts, hs
+
+
+def _append_faults(k, v, slots, k_cache, log_gate, log_gate_cache, H, D) -> None:
+    check_cuda((k_cache, k, v, slots, log_gate), ("k_cache", "k", "v", "slots", "log_gate"))
+    check_ndim(k, 3, "k")
+    T = k.shape[0]
+    check_shape(k, (T, H, D), "k")
+    check_shape(v, (T, H, D), "v")
+    if v.dtype != k.dtype:
+        raise ValueError(f"[v] dtype {v.dtype} differs from k's {k.dtype}")
+    _lib.dtype_code(k.dtype, "k")
+    if slots.dtype != _I64:
+        raise ValueError(f"[slots] expected int64, got {slots.dtype}")
+    check_shape(slots, (T,), "slots")
+    if (log_gate is None) != (log_gate_cache is None):
+        raise ValueError("[log_gate] a cache with log-gates takes them, and one without does not")
+    check_shape(log_gate, (T, H), "log_gate")
 
 
 def sattn_paged_append(k, v, slots, k_cache, v_cache, k_scale, v_scale, log_gate=None, log_gate_cache=None) -> None:
@@ -138,48 +211,68 @@ def sattn_paged_append(k, v, slots, k_cache, v_cache, k_scale, v_scale, log_gate
     ``v_cache`` ``(pages, Hkv, page_size, D)`` int8 or float8_e4m3fn; ``k_scale``, ``v_scale``
     ``(pages, Hkv)`` float32; ``log_gate`` ``(T, Hkv)`` and ``log_gate_cache`` ``(pages, Hkv, page_size)``
     float32, both or neither. A page's scale is the largest magnitude that it has held (finite ones
-    count) times the reciprocal of the largest code, 127 or 448: where new tokens raise it, the page's earlier codes are
-    rounded anew.
+    count) times the reciprocal of the largest code, 127 or 448: where new tokens raise it, the page's
+    earlier codes are rounded anew.
     """
-    dev = check_cuda([k, v, slots, k_cache, v_cache, k_scale, v_scale, log_gate, log_gate_cache],
-                     ["k", "v", "slots"] + _CACHE_NAMES[:4] + ["log_gate", "log_gate_cache"])
-    c = _cache(k_cache, v_cache, k_scale, v_scale, log_gate_cache)
-    check_ndim(k, 3, "k")
+    c, H, _, D, d = _cache(k_cache, v_cache, k_scale, v_scale, log_gate_cache)
     T = k.shape[0]
-    check_shape(k, (T, c.nkv, c.head_dim), "k")
-    check_shape(v, (T, c.nkv, c.head_dim), "v")
-    if v.dtype != k.dtype:
-        raise ValueError(f"[v] dtype {v.dtype} differs from k's {k.dtype}")
-    code = _lib.dtype_code(k.dtype, "k")
-    slots = _slots(slots)
-    check_shape(slots, (T,), "slots")
-    if (log_gate is None) != (log_gate_cache is None):
-        raise ValueError("[log_gate] a cache with log-gates takes them, and one without does not")
+    if not (k.shape == v.shape == (T, H, D) and k.dtype == v.dtype and k.dtype in _lib.DTYPE_CODES
+            and slots.dtype == _I64 and slots.shape == (T,)
+            and k.get_device() == v.get_device() == slots.get_device() == d
+            and (log_gate is None) == (log_gate_cache is None)
+            and (log_gate is None or (log_gate.shape == (T, H) and log_gate.get_device() == d))):
+        _append_faults(k, v, slots, k_cache, log_gate, log_gate_cache, H, D)
+    dev = k.device
+    code = _lib.DTYPE_CODES[k.dtype]
+    slots = to_contiguous(slots)
     if log_gate is not None:
-        check_shape(log_gate, (T, c.nkv), "log_gate")
         log_gate = to_contiguous(log_gate.float())
     k, k_ts, k_hs = _rows(k)
     v, v_ts, v_hs = _rows(v)
-    with torch.cuda.device(dev):
-        st = _lib.lib().sattn_paged_append(byref(c), _lib.ptr(k), _lib.ptr(v), _lib.ptr(log_gate), _lib.ptr(slots), T,
-                                           k_ts, k_hs, v_ts, v_hs, code, _stream(dev))
+    with _on(dev):
+        st = _lib.lib().sattn_paged_append(c, k.data_ptr(), v.data_ptr(), _lib.ptr(log_gate), slots.data_ptr(), T, k_ts,
+                                           k_hs, v_ts, v_hs, code, _lib.stream_handle(dev))
     _lib.check(st, "sattn_paged_append")
 
 
 def sattn_paged_read(slots, k_cache, v_cache, k_scale, v_scale, dtype: torch.dtype = torch.float32):
     """Values of slots of a paged cache (C-ABI ``sattn_paged_read``): ``(k, v)``, each
     ``(len(slots), Hkv, D)`` in ``dtype``; zeros where a slot is not the cache's (-1)."""
-    dev = check_cuda([slots, k_cache, v_cache, k_scale, v_scale], ["slots"] + _CACHE_NAMES[:4])
-    c = _cache(k_cache, v_cache, k_scale, v_scale, None)
+    c, H, _, D, d = _cache(k_cache, v_cache, k_scale, v_scale, None)
     code = _lib.dtype_code(dtype, "dtype")
-    slots = _slots(slots)
-    k = torch.empty(slots.numel(), c.nkv, c.head_dim, device=dev, dtype=dtype)
-    v = torch.empty_like(k)
-    with torch.cuda.device(dev):
-        st = _lib.lib().sattn_paged_read(byref(c), _lib.ptr(slots), slots.numel(), _lib.ptr(k), _lib.ptr(v), code,
-                                         _stream(dev))
+    if not (slots.dtype == _I64 and len(slots.shape) == 1 and slots.get_device() == d):
+        check_cuda((k_cache, slots), ("k_cache", "slots"))
+        check_ndim(slots, 1, "slots")
+        raise ValueError(f"[slots] expected int64, got {slots.dtype}")
+    slots = to_contiguous(slots)
+    dev = slots.device
+    n = slots.shape[0]
+    k = torch.empty((n, H, D), device=dev, dtype=dtype)
+    v = torch.empty((n, H, D), device=dev, dtype=dtype)
+    with _on(dev):
+        st = _lib.lib().sattn_paged_read(c, slots.data_ptr(), n, k.data_ptr(), v.data_ptr(), code,
+                                         _lib.stream_handle(dev))
     _lib.check(st, "sattn_paged_read")
     return k, v
+
+
+@functools.lru_cache(maxsize=None)
+def _decode_workspace(heads: int, page: int, head_dim: int, nheads: int) -> int:
+    """Bytes of workspace of a decode step; they go by the head geometry alone."""
+    c = _CACHE.pack(1, heads, page, head_dim, 0, 16, 16, 16, 16, 0)
+    return int(_lib.lib().sattn_paged_decode_workspace_size(c, 1, 1, nheads))
+
+
+def _decode_faults(q, k_cache, block_table, lengths, H, D) -> None:
+    check_cuda((k_cache, q, block_table, lengths), ("k_cache", "q", "block_table", "lengths"))
+    check_ndim(q, 3, "q")
+    check_ndim(block_table, 2, "block_table")
+    R, Hq, d = q.shape
+    if d != D or Hq == 0 or Hq % H:
+        raise ValueError(f"[q] expected (requests, a multiple of {H} heads, {D}), got {tuple(q.shape)}")
+    _lib.dtype_code(q.dtype, "q")
+    _int32(block_table, "block_table", (R, block_table.shape[1]))
+    _int32(lengths, "lengths", (R,))
 
 
 def sattn_paged_decode(q, k_cache, v_cache, k_scale, v_scale, block_table, lengths, log_gate_cache=None, scale=None,
@@ -194,23 +287,23 @@ def sattn_paged_decode(q, k_cache, v_cache, k_scale, v_scale, block_table, lengt
     ``D ** -0.5``. Returns ``(R, Hq, D)`` in ``q``'s dtype. ``workspace`` (uint8) is allocated when it
     is ``None`` or too small; calls that overlap on the GPU need one each.
     """
-    dev = check_cuda([q, k_cache, v_cache, k_scale, v_scale, block_table, lengths, log_gate_cache],
-                     ["q"] + _CACHE_NAMES[:4] + ["block_table", "lengths", "log_gate_cache"])
-    c = _cache(k_cache, v_cache, k_scale, v_scale, log_gate_cache)
-    check_ndim(q, 3, "q")
-    check_ndim(block_table, 2, "block_table")
-    R, Hq, D = q.shape
-    if D != c.head_dim or Hq == 0 or Hq % c.nkv:
-        raise ValueError(f"[q] expected (requests, a multiple of {c.nkv} heads, {c.head_dim}), got {tuple(q.shape)}")
-    code = _lib.dtype_code(q.dtype, "q")
-    W = block_table.shape[1]
-    _int32(block_table, "block_table", (R, W))
-    _int32(lengths, "lengths", (R,))
+    c, H, page, D, d = _cache(k_cache, v_cache, k_scale, v_scale, log_gate_cache)
+    shape = q.shape
+    R, Hq = shape[0], shape[1]
+    W = block_table.shape[-1]
+    if not (len(shape) == 3 and shape[2] == D and Hq and Hq % H == 0 and q.dtype in _lib.DTYPE_CODES
+            and block_table.shape == (R, W) and lengths.shape == (R,) and block_table.dtype == lengths.dtype == _I32
+            and block_table.is_contiguous() and lengths.is_contiguous()
+            and q.get_device() == block_table.get_device() == lengths.get_device() == d):
+        _decode_faults(q, k_cache, block_table, lengths, H, D)
+    if out is not None or workspace is not None:
+        check_cuda((q, out, workspace), ("q", "out", "workspace"))
+    code = _lib.DTYPE_CODES[q.dtype]
+    dev = q.device
     q = _aligned16(to_contiguous(q))
     if out is None:
-        out = torch.empty(R, Hq, D, device=dev, dtype=q.dtype)
+        out = torch.empty_like(q)
     else:
-        check_cuda([q, out], ["q", "out"])
         check_shape(out, (R, Hq, D), "out")
         if out.dtype != q.dtype or not out.is_contiguous() or out.data_ptr() % 16:
             raise ValueError("[out] expected a contiguous, 16-byte aligned tensor of q's dtype")
@@ -218,17 +311,35 @@ def sattn_paged_decode(q, k_cache, v_cache, k_scale, v_scale, block_table, lengt
         return out
     if W == 0:
         return out.zero_()
-    need = int(_lib.lib().sattn_paged_decode_workspace_size(byref(c), R, W, Hq))
-    if need and (workspace is None or workspace.numel() * workspace.element_size() < need):
+    need = _decode_workspace(H, page, D, Hq)
+    if workspace is None or workspace.numel() * workspace.element_size() < need or workspace.data_ptr() % 16:
         workspace = torch.empty(need, device=dev, dtype=torch.uint8)
-    elif need:
-        check_cuda([q, workspace], ["q", "workspace"])
-    with torch.cuda.device(dev):
-        st = _lib.lib().sattn_paged_decode(byref(c), _lib.ptr(q), _lib.ptr(block_table), _lib.ptr(lengths),
-                                           _lib.ptr(out), R, W, Hq, float(D ** -0.5 if scale is None else scale), code,
-                                           c_void_p(_lib.ptr(workspace) if need else None), need, _stream(dev))
+    with _on(dev):
+        st = _lib.lib().sattn_paged_decode(c, q.data_ptr(), block_table.data_ptr(), lengths.data_ptr(), out.data_ptr(),
+                                           R, W, Hq, D ** -0.5 if scale is None else float(scale), code,
+                                           workspace.data_ptr(), need, _lib.stream_handle(dev))
     _lib.check(st, "sattn_paged_decode")
     return out
+
+
+def _packed_faults(q, k, v, cu_seqlens, log_gate) -> None:
+    check_ndim(q, 3, "q")
+    check_ndim(k, 3, "k")
+    check_ndim(cu_seqlens, 1, "cu_seqlens")
+    check_cuda((q, k, v, cu_seqlens, log_gate), ("q", "k", "v", "cu_seqlens", "log_gate"))
+    T, Hq, D = q.shape
+    Hk = k.shape[1]
+    if Hk == 0 or Hq == 0 or Hq % Hk:
+        raise ValueError(f"[k] {Hq} query heads are not a multiple of {Hk} key heads")
+    for t, n in ((k, "k"), (v, "v")):
+        check_shape(t, (T, Hk, D), n)
+        if t.dtype != q.dtype:
+            raise ValueError(f"[{n}] dtype {t.dtype} differs from q's {q.dtype}")
+    check_shape(log_gate, (T, Hk), "log_gate", optional=True)
+    if cu_seqlens.shape[0] == 0:
+        raise ValueError("[cu_seqlens] expected the offsets of the sequences, from 0")
+    _int32(cu_seqlens, "cu_seqlens")
+    _lib.dtype_code(q.dtype, "q")
 
 
 def sattn_prefill_packed(q, k, v, cu_seqlens, log_gate=None, scale=None, out=None, impl: str = "auto"):
@@ -242,23 +353,21 @@ def sattn_prefill_packed(q, k, v, cu_seqlens, log_gate=None, scale=None, out=Non
     past the last sequence. ``scale`` defaults to ``D ** -0.5``. ``impl``: ``"auto"`` (tensor cores for
     16-bit types with ``D`` 64 or 128), ``"tc"`` or ``"simt"``.
     """
-    check_ndim(q, 3, "q")
-    check_ndim(k, 3, "k")
-    check_ndim(cu_seqlens, 1, "cu_seqlens")
-    T, Hq, D = q.shape
+    d = q.get_device()
+    shape = q.shape
+    if not (d >= 0 and len(shape) == 3 and len(k.shape) == 3 and k.shape == v.shape and k.shape[0] == shape[0]
+            and k.shape[2] == shape[2] and k.shape[1] and shape[1] and shape[1] % k.shape[1] == 0
+            and q.dtype == k.dtype == v.dtype and q.dtype in _lib.DTYPE_CODES and cu_seqlens.dtype == _I32
+            and len(cu_seqlens.shape) == 1 and cu_seqlens.shape[0] and cu_seqlens.is_contiguous()
+            and k.get_device() == v.get_device() == cu_seqlens.get_device() == d
+            and (log_gate is None or (log_gate.shape == k.shape[:2] and log_gate.get_device() == d))):
+        _packed_faults(q, k, v, cu_seqlens, log_gate)
+    if out is not None:
+        check_cuda((q, out), ("q", "out"))
+    T, Hq, D = shape
     Hk = k.shape[1]
-    dev = check_cuda([q, k, v, cu_seqlens, log_gate, out], ["q", "k", "v", "cu_seqlens", "log_gate", "out"])
-    if Hk == 0 or Hq == 0 or Hq % Hk:
-        raise ValueError(f"[k] {Hq} query heads are not a multiple of {Hk} key heads")
-    for t, n in ((k, "k"), (v, "v")):
-        check_shape(t, (T, Hk, D), n)
-        if t.dtype != q.dtype:
-            raise ValueError(f"[{n}] dtype {t.dtype} differs from q's {q.dtype}")
-    check_shape(log_gate, (T, Hk), "log_gate", optional=True)
-    if cu_seqlens.numel() == 0:
-        raise ValueError("[cu_seqlens] expected the offsets of the sequences, from 0")
-    _int32(cu_seqlens, "cu_seqlens")
-    code = _lib.dtype_code(q.dtype, "q")
+    dev = q.device
+    code = _lib.DTYPE_CODES[q.dtype]
     per = 16 // q.element_size()
 
     def rows(t):
@@ -270,18 +379,15 @@ def sattn_prefill_packed(q, k, v, cu_seqlens, log_gate=None, scale=None, out=Non
     (q, q_ts, q_hs), (k, k_ts, k_hs), (v, v_ts, v_hs) = rows(q), rows(k), rows(v)
     log_gate = None if log_gate is None else to_contiguous(log_gate.float())
     if out is None:
-        out = torch.empty(T, Hq, D, device=dev, dtype=q.dtype)
+        out = torch.empty((T, Hq, D), device=dev, dtype=q.dtype)
     else:
         check_shape(out, (T, Hq, D), "out")
         if out.dtype != q.dtype or not out.is_contiguous() or out.data_ptr() % 16:
             raise ValueError("[out] expected a contiguous, 16-byte aligned tensor of q's dtype")
-    p = _lib.SattnPackedParams(
-        num_tokens=T, num_seqs=cu_seqlens.numel() - 1, nheads=Hq, nkv=Hk, head_dim=D, q_token_stride=q_ts,
-        q_head_stride=q_hs, k_token_stride=k_ts, k_head_stride=k_hs, v_token_stride=v_ts, v_head_stride=v_hs,
-        dtype=code, impl=_lib.IMPLS[impl], scale=float(D ** -0.5 if scale is None else scale), q=_lib.ptr(q),
-        k=_lib.ptr(k), v=_lib.ptr(v), log_gate=_lib.ptr(log_gate), cu_seqlens=_lib.ptr(cu_seqlens),
-        out=_lib.ptr(out))
-    with torch.cuda.device(dev):
-        st = _lib.lib().sattn_prefill_packed(byref(p), _stream(dev))
+    p = _PACKED.pack(T, cu_seqlens.shape[0] - 1, Hq, Hk, D, q_ts, q_hs, k_ts, k_hs, v_ts, v_hs, code, _lib.IMPLS[impl],
+                     D ** -0.5 if scale is None else float(scale), q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                     0 if log_gate is None else log_gate.data_ptr(), cu_seqlens.data_ptr(), out.data_ptr())
+    with _on(dev):
+        st = _lib.lib().sattn_prefill_packed(p, _lib.stream_handle(dev))
     _lib.check(st, "sattn_prefill_packed")
     return out

@@ -73,7 +73,14 @@ def test_structs_match_the_header():
 
     if shutil.which("gcc") is None:
         pytest.skip("gcc not available")
-    for cname, cls in (("sattn_cache", _lib.SattnCache), ("sattn_packed_params", _lib.SattnPackedParams)):
+    from selective_attention_b200 import paged
+
+    for cname, cls, packed in (("sattn_cache", _lib.SattnCache, paged._CACHE),
+                               ("sattn_packed_params", _lib.SattnPackedParams, paged._PACKED)):
+        # the bytes that the wrappers pass have every field in its place
+        values = [(i + 1) / 2 if "f" == t._type_ else i + 1 for i, (_, t) in enumerate(cls._fields_)]
+        got = cls.from_buffer_copy(packed.pack(*values))
+        assert [getattr(got, f) for f, _ in cls._fields_] == values
         fields = [f[0] for f in cls._fields_]
         prog = ["#include <stdio.h>", "#include <stddef.h>",
                 f'#include "{os.path.join(ROOT, "include", "ssd_b200.h")}"', "int main(void){",
