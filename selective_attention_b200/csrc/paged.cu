@@ -163,20 +163,41 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(
 // ---------------------------------------------------------------------------
 // CTA = (block of `per` tokens, key head, K or V). A segment is a run of tokens with consecutive
 // slots in one page; the CTA in whose block it begins writes all of it (up to page - 1 tokens
-// past its block), so each page and head has one writer. Three steps: the largest finite
-// magnitude of each row; the segment's scale from its rows and the page's old scale; the codes
-// of the rows, and, where the scale grew, of the page's older rows. x is read twice, the
-// second time from L1/L2.
+// past its block), so each page and head has one writer. The rows are loaded once, all loads in
+// flight together, and stay in registers as they came (the rows past the first kAppHeld passes
+// are read again); then the largest finite magnitude of each row, the segment's scale from its
+// rows and the page's old scale, and the codes of the rows and, where the scale grew, of the
+// page's older rows. Bound by reading x and writing the codes.
 constexpr int kAppThreads = 256;
 constexpr int kAppRows = 256;  // rows of one CTA: per + page - 1 <= 255
+constexpr int kAppHeld = 8;
 
+// Eight elements as they lie in memory.
+template <typename T> struct Raw8 {
+  uint4 w[sizeof(T) / 2];
+};
 template <typename T, bool VEC>
-__device__ __forceinline__ void load_row8(const T* p, float (&x)[8]) {
+__device__ __forceinline__ void load_raw(const T* p, Raw8<T>& x) {
   if constexpr (VEC) {
-    load8<T>(p, x);
-  } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = Ld<T>::f(p + e);
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) x.w[i] = reinterpret_cast<const uint4*>(p)[i];
+  } else {
+    T* d = reinterpret_cast<T*>(x.w);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) d[e] = p[e];
+  }
+}
+template <typename T>
+__device__ __forceinline__ void floats(const Raw8<T>& x, float (&v)[8]) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      v[4 * i] = __uint_as_float(x.w[i].x), v[4 * i + 1] = __uint_as_float(x.w[i].y);
+      v[4 * i + 2] = __uint_as_float(x.w[i].z), v[4 * i + 3] = __uint_as_float(x.w[i].w);
+    }
+  } else {
+    const float2 a = unpack2<T>(x.w[0].x), b = unpack2<T>(x.w[0].y), c = unpack2<T>(x.w[0].z), d = unpack2<T>(x.w[0].w);
+    v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y, v[4] = c.x, v[5] = c.y, v[6] = d.x, v[7] = d.y;
   }
 }
 
@@ -186,11 +207,15 @@ __global__ void __launch_bounds__(kAppThreads) paged_append_kernel(
     const long long* __restrict__ slots, unsigned char* kc, unsigned char* vc, float* ks, float* vs, float* gc,
     long long num_pages, int H, int page_shift, int D, long long Tn, long long k_ts, long long k_hs, long long v_ts,
     long long v_hs, int per) {
-  __shared__ float rmax[kAppRows];    // per row; the segment's new scale after step 2
-  __shared__ float ratio[kAppRows];   // at a segment's first row: old / new scale where it grew, else 0
-  __shared__ short head_of[kAppRows]; // row -> its segment's first row, -1 if the row is not this CTA's
-  __shared__ int s_rows;
-  const int tid = threadIdx.x, page = 1 << page_shift;
+  __shared__ int smax[kAppRows];           // at a segment's first row: its largest magnitude (as bits), then its scale
+  __shared__ float inverse[kAppRows];      // 1 / the scale
+  __shared__ float ratio[kAppRows];        // of a page that grew: old / new scale
+  __shared__ short grown[kAppRows];        // first rows of the segments whose pages hold older rows and grew
+  __shared__ short head_of[kAppRows];      // row -> its segment's first row, -1 if the row is not this CTA's
+  __shared__ long long s_slot[kAppRows];
+  __shared__ int wlast[kAppThreads / 32];  // last segment start of each warp's rows
+  __shared__ int s_rows, s_grown;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, page = 1 << page_shift;
   const int h = blockIdx.y;
   const bool is_v = blockIdx.z != 0;
   const T* x = is_v ? vx + h * v_hs : kx + h * k_hs;
@@ -198,40 +223,51 @@ __global__ void __launch_bounds__(kAppThreads) paged_append_kernel(
   unsigned char* codes = is_v ? vc : kc;
   float* scale = is_v ? vs : ks;
   const long long t0 = (long long)blockIdx.x * per;
-  const long long nslots = num_pages << page_shift;
   const int most = (int)min((long long)per + page - 1, Tn - t0);  // rows that can be this CTA's
-  if (tid == 0) s_rows = 0;
-  auto slot_of = [&](long long t) -> long long {
-    const long long s = slots[t];
-    return s >= 0 && s < nslots ? s : -1;
-  };
-  // a row's segment begins at the row or at most page - 1 rows before it
-  for (int i = tid; i < most; i += kAppThreads) {
-    const long long s = slot_of(t0 + i);
-    int first = -1;
-    if (s >= 0) {
-      const int back = (int)(s & (page - 1));
-      int b = 0;
-      while (b < back && t0 + i - b > 0 && slots[t0 + i - b - 1] == s - b - 1) ++b;
-      first = i - b;
-      if (first < 0 || first >= per) first = -1;  // another CTA's
+  if (tid == 0) s_rows = 0, s_grown = 0;
+  // thread = row: where segments begin, then a running maximum of the beginnings
+  {
+    long long s = -1, before = -2;
+    if (tid < most) {
+      s = slots[t0 + tid];
+      if (t0 + tid > 0) before = slots[t0 + tid - 1];
     }
-    head_of[i] = (short)first;
-    rmax[i] = 0.f;
-    if (first >= 0) atomicMax(&s_rows, i + 1);
+    const bool in = s >= 0 && s < num_pages << page_shift;
+    const bool starts = in && ((s & (page - 1)) == 0 || before != s - 1);
+    int m = starts ? tid : -1;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, m, off);
+      if (lane >= off) m = max(m, o);
+    }
+    if (lane == 31) wlast[warp] = m;
+    __syncthreads();
+    for (int w = 0; w < warp; ++w) m = max(m, wlast[w]);
+    const int first = in && m < per ? m : -1;  // (m = -1: begun in an earlier block)
+    head_of[tid] = (short)first;
+    s_slot[tid] = s;
+    smax[tid] = 0;
+    const unsigned mine = __ballot_sync(0xffffffffu, first >= 0);
+    if (lane == 0 && mine) atomicMax(&s_rows, warp * 32 + 32 - __clz(mine));
   }
   __syncthreads();
   const int rows = s_rows;
   if (rows == 0) return;
-  const int lpr = D >> 3;                   // lanes per row, 8 elements each
-  const int sub = tid % lpr, grp = tid / lpr, ngrp = kAppThreads / lpr;
-  for (int i0 = 0; i0 < rows; i0 += ngrp) {
-    const int i = i0 + grp;
-    const bool live = i < rows && head_of[i] >= 0;
+  const int lpr = D >> 3, lshift = 31 - __clz(lpr);  // lanes per row, 8 elements each
+  const int sub = tid & (lpr - 1), grp = tid >> lshift, ngrp = kAppThreads >> lshift;
+  Raw8<T> held[kAppHeld];
+#pragma unroll
+  for (int u = 0; u < kAppHeld; ++u) {
+    const int i = u * ngrp + grp;
+    if (i < rows && head_of[i] >= 0) load_raw<T, VEC>(x + (t0 + i) * ts + sub * 8, held[u]);
+  }
+  // (all lanes of a warp are in the same number of steps: the bound is rounded up to whole passes)
+  const int passes = (rows + ngrp - 1) / ngrp;
+  auto row_max = [&](int i, const Raw8<T>& raw) {
     float m = 0.f;
-    if (live) {
+    if (i < rows && head_of[i] >= 0) {
       float v[8];
-      load_row8<T, VEC>(x + (t0 + i) * ts + sub * 8, v);
+      floats<T>(raw, v);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const float a = fabsf(v[e]);
@@ -239,41 +275,72 @@ __global__ void __launch_bounds__(kAppThreads) paged_append_kernel(
       }
     }
     for (int off = 1; off < lpr; off <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
-    if (live && sub == 0) rmax[i] = m;
+    // (magnitudes order as their bits do)
+    if (i < rows && head_of[i] >= 0 && sub == 0) atomicMax(&smax[head_of[i]], __float_as_int(m));
+  };
+#pragma unroll
+  for (int u = 0; u < kAppHeld; ++u)
+    if (u < passes) row_max(u * ngrp + grp, held[u]);
+  for (int u = kAppHeld; u < passes; ++u) {
+    const int i = u * ngrp + grp;
+    Raw8<T> raw;
+    if (i < rows && head_of[i] >= 0) load_raw<T, VEC>(x + (t0 + i) * ts + sub * 8, raw);
+    row_max(i, raw);
   }
   __syncthreads();
-  for (int i = tid; i < rows; i += kAppThreads) {
-    if (head_of[i] != i) continue;
-    float m = 0.f;
-    for (int j = i; j < rows && j < i + page && head_of[j] == i; ++j) m = fmaxf(m, rmax[j]);
-    const long long s = slots[t0 + i];
+  if (tid < rows && head_of[tid] == tid) {
+    const long long s = s_slot[tid];
+    const bool older = (s & (page - 1)) != 0;  // a page that begins here has no older rows
     float* sp = scale + (s >> page_shift) * H + h;
-    const float was = (s & (page - 1)) ? *sp : 0.f;  // a page that begins here has no older rows
-    const float now = fmaxf(was, m * Code<C>::kPerMost);
-    ratio[i] = now > was ? __fdiv_rn(was, now) : -1.f;
+    const float was = older ? *sp : 0.f;
+    const float now = fmaxf(was, __int_as_float(smax[tid]) * Code<C>::kPerMost);
     *sp = now;
-    // the rows' step reads it below; other segments' rows are apart
-    rmax[i] = now;
+    smax[tid] = __float_as_int(now);
+    inverse[tid] = 1.0f / now;
+    if (older && now > was) {
+      ratio[tid] = __fdiv_rn(was, now);
+      grown[atomicAdd(&s_grown, 1)] = (short)tid;
+    }
   }
   __syncthreads();
-  for (int i0 = 0; i0 < rows; i0 += ngrp) {
-    const int i = i0 + grp;
+  auto encode = [&](int i, const Raw8<T>& raw) {
     const int first = i < rows ? head_of[i] : -1;
-    if (first < 0) continue;
-    const long long s = slots[t0 + i];
+    if (first < 0) return;
+    const long long s = s_slot[i];
     const long long row = ((s >> page_shift) * H + h) * page + (s & (page - 1));
     float v[8];
-    load_row8<T, VEC>(x + (t0 + i) * ts + sub * 8, v);
-    const float sc = rmax[first];
+    floats<T>(raw, v);
+    // The codes are those of the quotient x / scale. A product with the reciprocal gives the same code but
+    // next to the middle between two; there, and where the reciprocal is no normal number, divide.
+    const float sc = __int_as_float(smax[first]), inv = inverse[first];
+    float y[8];
+    bool divide = !(inv < 1e37f);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = sc > 0.f ? __fdiv_rn(v[e], sc) : 0.f;
-    *reinterpret_cast<uint2*>(codes + row * D + sub * 8) = Code<C>::pack8(v);
+    for (int e = 0; e < 8; ++e) {
+      y[e] = v[e] * inv;
+      divide |= Code<C>::unsure(y[e]);
+    }
+    if (divide) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = sc > 0.f ? __fdiv_rn(v[e], sc) : 0.f;
+    }
+    *reinterpret_cast<uint2*>(codes + row * D + sub * 8) = Code<C>::pack8(y);
     if (!is_v && gate && sub == 0) gc[row] = gate[(t0 + i) * H + h];
+  };
+#pragma unroll
+  for (int u = 0; u < kAppHeld; ++u)
+    if (u < passes) encode(u * ngrp + grp, held[u]);
+  for (int u = kAppHeld; u < passes; ++u) {
+    const int i = u * ngrp + grp;
+    if (i >= rows || head_of[i] < 0) continue;
+    Raw8<T> raw;
+    load_raw<T, VEC>(x + (t0 + i) * ts + sub * 8, raw);
+    encode(i, raw);
   }
   // older rows of the pages whose scale grew
-  for (int i = 0; i < min(rows, per); ++i) {
-    if (head_of[i] != i || ratio[i] < 0.f) continue;
-    const long long s = slots[t0 + i];
+  for (int k = 0; k < s_grown; ++k) {
+    const int i = grown[k];
+    const long long s = s_slot[i];
     const int older = (int)(s & (page - 1));
     unsigned char* base = codes + ((s >> page_shift) * H + h) * (long long)page * D;
     for (int j = grp; j < older; j += ngrp) {
@@ -291,42 +358,59 @@ __global__ void __launch_bounds__(kAppThreads) paged_append_kernel(
 // read: values of the given slots, (N, H, D) for K and V; slots outside the cache give zeros.
 // One thread reads 8 codes and writes 8 values; bound by writing them.
 // ---------------------------------------------------------------------------
+constexpr int kReadThreads = 256;
+constexpr int kReadItems = 4;  // of a thread, their codes all in flight
+
 template <typename T, typename C>
-__global__ void __launch_bounds__(256) paged_read_kernel(const long long* __restrict__ slots,
-                                                         const unsigned char* __restrict__ kc,
-                                                         const unsigned char* __restrict__ vc,
-                                                         const float* __restrict__ ks, const float* __restrict__ vs,
-                                                         T* __restrict__ ko, T* __restrict__ vo, long long num_pages,
-                                                         int H, int page_shift, int D, long long n8) {
-  const int lpr = D >> 3, page = 1 << page_shift;
+__global__ void __launch_bounds__(kReadThreads) paged_read_kernel(
+    const long long* __restrict__ slots, const unsigned char* __restrict__ kc, const unsigned char* __restrict__ vc,
+    const float* __restrict__ ks, const float* __restrict__ vs, T* __restrict__ ko, T* __restrict__ vo,
+    long long num_pages, int H, int page_shift, int D, long long n, int per) {
+  const int lshift = 31 - __clz(D >> 3), page = 1 << page_shift;
   const bool is_v = blockIdx.y != 0;
   const unsigned char* codes = is_v ? vc : kc;
   const float* scale = is_v ? vs : ks;
   T* out = is_v ? vo : ko;
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n8; i += (long long)gridDim.x * 256) {
-    const long long rh = i / lpr;
-    const int sub = (int)(i - rh * lpr);
-    const long long t = rh / H;
-    const int h = (int)(rh - t * H);
-    const long long s = slots[t];
-    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (s >= 0 && s < (num_pages << page_shift)) {
-      const long long ph = (s >> page_shift) * H + h;
-      Code<C>::unpack8(*reinterpret_cast<const uint2*>(codes + (ph * page + (s & (page - 1))) * D + sub * 8), v);
-      const float sc = scale[ph];
+  const long long first = (long long)blockIdx.x * per;              // the CTA's slots, `per` of them
+  const unsigned row = (unsigned)H << lshift;                       // items of a slot
+  const unsigned items = (unsigned)min((long long)per, n - first) * row;
+  for (unsigned i0 = threadIdx.x; i0 < items; i0 += kReadItems * kReadThreads) {
+    uint2 w[kReadItems];
+    float sc[kReadItems];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] *= sc;
+    for (int u = 0; u < kReadItems; ++u) {
+      const unsigned i = i0 + u * kReadThreads;
+      w[u] = make_uint2(0u, 0u);
+      sc[u] = 0.f;
+      if (i < items) {
+        const unsigned t = i / row, in = i - t * row, h = in >> lshift, sub = in & ((1u << lshift) - 1u);
+        const long long s = slots[first + t];
+        if (s >= 0 && s < num_pages << page_shift) {
+          const long long ph = (s >> page_shift) * H + h;
+          w[u] = *reinterpret_cast<const uint2*>(codes + (ph * page + (s & (page - 1))) * D + sub * 8);
+          sc[u] = scale[ph];
+        }
+      }
     }
-    store8<T>(out + i * 8, v);
+#pragma unroll
+    for (int u = 0; u < kReadItems; ++u) {
+      const unsigned i = i0 + u * kReadThreads;
+      if (i >= items) break;
+      float v[8];
+      Code<C>::unpack8(w[u], v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] *= sc[u];
+      store8<T>(out + (first * row + i) * 8, v);
+    }
   }
 }
 
 template <typename T, typename C>
 cudaError_t append_t(const PagedCache& c, const void* k, const void* v, const float* gate, const long long* slots,
                      long long n, long long k_ts, long long k_hs, long long v_ts, long long v_hs, cudaStream_t s) {
-  // Few tokens: small blocks, so that many CTAs share them. Many: a block is a page (each CTA then
-  // has one segment or two, and few CTAs find none).
-  const int per = n * c.nkv <= 2048 ? 4 : (c.page < 16 ? 16 : c.page);
+  // Few tokens: small blocks, so that many CTAs share them. Many: 128 tokens, which a CTA's threads hold
+  // in registers for head_dim 128 (a page each: 64 us instead of 59 for 16k tokens of 8 heads).
+  const int per = n * c.nkv <= 2048 ? 4 : 128;
   const bool vec = (reinterpret_cast<uintptr_t>(k) % 16 == 0) && (reinterpret_cast<uintptr_t>(v) % 16 == 0) &&
                    (k_ts * sizeof(T)) % 16 == 0 && (k_hs * sizeof(T)) % 16 == 0 && (v_ts * sizeof(T)) % 16 == 0 &&
                    (v_hs * sizeof(T)) % 16 == 0;
@@ -341,11 +425,14 @@ cudaError_t append_t(const PagedCache& c, const void* k, const void* v, const fl
 
 template <typename T, typename C>
 cudaError_t read_t(const PagedCache& c, const long long* slots, long long n, void* ko, void* vo, cudaStream_t s) {
-  const long long n8 = n * c.nkv * (c.D >> 3);
-  const long long blocks = (n8 + 255) / 256;
-  dim3 grid((unsigned)(blocks < 148 * 64 ? blocks : 148 * 64), 2);
-  paged_read_kernel<T, C><<<grid, 256, 0, s>>>(slots, c.k, c.v, c.ks, c.vs, (T*)ko, (T*)vo, c.pages, c.nkv,
-                                               c.page_shift, c.D, n8);
+  // slots of a CTA: about kReadItems items a thread
+  const long long row = (long long)c.nkv * (c.D >> 3);
+  const long long per = row >= kReadItems * kReadThreads ? 1 : kReadItems * kReadThreads / row;
+  const long long blocks = (n + per - 1) / per;
+  if (blocks > 0x7fffffffll) return cudaErrorInvalidValue;
+  dim3 grid((unsigned)blocks, 2);
+  paged_read_kernel<T, C><<<grid, kReadThreads, 0, s>>>(slots, c.k, c.v, c.ks, c.vs, (T*)ko, (T*)vo, c.pages, c.nkv,
+                                                        c.page_shift, c.D, n, (int)per);
   return cudaGetLastError();
 }
 

@@ -16,6 +16,8 @@ struct E4M3 {};
 template <typename C> struct Code;
 template <> struct Code<Int8> {
   static constexpr float kPerMost = 1.0f / 127.0f;
+  // Whether a quotient that is off by up to 3 * 2^-24 of itself may round to another code.
+  static __device__ __forceinline__ bool unsure(float q) { return fabsf(q - rintf(q)) > 0.4999f; }
   static __device__ __forceinline__ unsigned pack1(float x) {
     // fmaxf / fminf would turn a NaN into a bound
     const float y = x == x ? fminf(fmaxf(rintf(x), -127.f), 127.f) : 0.f;
@@ -37,6 +39,10 @@ template <> struct Code<Int8> {
 };
 template <> struct Code<E4M3> {
   static constexpr float kPerMost = 1.0f / 448.0f;
+  // (codes have three mantissa bits: the middle between two is at bit 19; those below 2^-6 lie evenly)
+  static __device__ __forceinline__ bool unsure(float q) {
+    return (__float_as_uint(q) & 0xfffffu) - 0x7fff8u <= 16u || fabsf(q) < 0.01563f;
+  }
   static __device__ __forceinline__ unsigned pack2c(float a, float b) {
     return (unsigned)__nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
   }
