@@ -45,6 +45,7 @@ using namespace sm100;
 constexpr int kDecWarps = 4;                        // computing warps
 constexpr int kDecThreads = (kDecWarps + 1) * 32;   // and one that fetches
 constexpr int kMinTiles = 8;                        // 16-token tiles that a CTA's share has at least
+constexpr int kStart = 8;                           // a row group's start and join, in tiles' time (see below)
 constexpr unsigned int kSiteDecLoad = 0x401, kSiteDecUse = 0x402;
 constexpr float kDecLog2e = 1.4426950408889634f;
 constexpr float kGrow = 8.0f;      // log2: O is rescaled when a row's maximum grows by more
@@ -110,6 +111,11 @@ template <int D, int NG> constexpr size_t dec_smem() {
          2 * 32 * dec_xchg_words<D, NG>() * 4 + 128;
 }
 
+// Adds to the bytes that a barrier's phase waits for, without arriving on it.
+__device__ __forceinline__ void mbar_announce(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+
 struct DecodeArgs {
   const void* q;
   const float *ks, *vs, *gc;
@@ -129,21 +135,26 @@ __device__ __forceinline__ int dec_tiles(const DecodeArgs& a, int r) { return (d
 // All requests' tiles, request by request and, within one, row group by row group (a row group:
 // the up to 8 NG query heads that share one reading of a key head), are one line; CTA i works on
 // [i * per, (i + 1) * per) of it. So every CTA has the same share whatever the lengths are, and one
-// long request is spread over all of them. A row group that crosses from one CTA into the next
-// leaves a part in each, which paged_decode_join_kernel joins in their order.
+// long request is spread over all of them. Each row group begins with kStart places without a tile,
+// for the time that its start and its join take: counted by tiles alone, the CTAs of short requests
+// took up to 1.75 times the median (24 requests of 1 to 4097 tokens, 24 heads of 64: 79 us of 45). A row
+// group that crosses from one CTA into the next leaves a part in each, which
+// paged_decode_join_kernel joins in their order.
+__device__ __forceinline__ int dec_places(int tiles) { return tiles > 0 ? tiles + kStart : 0; }
+
 __device__ __forceinline__ long long dec_share(long long units, int ctas) {
   const long long per = (units + ctas - 1) / ctas;
   return per < kMinTiles ? kMinTiles : per;
 }
 
-// Called by a whole CTA of N threads: the tiles of all requests (returned), and those before
-// request `upto` (before). sums: 2 * N / 32 words of shared memory.
+// Called by a whole CTA of N threads: the places of one row group of every request (returned), and those
+// before request `upto` (before). sums: 2 * N / 32 words of shared memory.
 template <int N>
 __device__ __forceinline__ long long dec_count(const DecodeArgs& a, int upto, long long& before, long long* sums) {
   const int tid = threadIdx.x;
   long long all = 0, pre = 0;
   for (int r = tid; r < a.R; r += N) {
-    const int t = dec_tiles(a, r);
+    const int t = dec_places(dec_tiles(a, r));
     all += t;
     if (r < upto) pre += t;
   }
@@ -166,27 +177,34 @@ template <int D, int NG> constexpr int dec_ctas_per_sm() {
   return D == 256 || NG == 2 ? 2 : (D == 128 ? 3 : 4);
 }
 
-// A run of tiles of one row group.
+// A run of tiles of one row group (none, where the share ends within the places before the first tile).
 struct DecSegment {
-  int r, n, tiles, group, first, last;
+  int r, n, group, first, last;
+  int places;          // of the line that it takes
+  bool whole, begun;   // all of the row group; begun by an earlier CTA
 };
-// The segment at `at` of the line, r and r_at (the request and its first tile on the line) moved on to it.
+// The segment at `at` of the line, r and r_at (the request and its first place on the line) moved on to it.
 __device__ __forceinline__ DecSegment dec_segment(const DecodeArgs& a, int groups, long long at, long long end, int& r,
                                                   long long& r_at) {
   DecSegment s;
+  int places;
   for (;;) {
     s.n = dec_length(a, r);
-    s.tiles = (s.n + 15) >> 4;
-    const long long all = (long long)s.tiles * groups;
+    places = dec_places((s.n + 15) >> 4);
+    const long long all = (long long)places * groups;
     if (at < r_at + all) break;
     r_at += all;
     ++r;
   }
   s.r = r;
   const long long in = at - r_at;
-  s.group = (int)(in / s.tiles);
-  s.first = (int)(in - (long long)s.group * s.tiles);
-  s.last = (int)min((long long)s.tiles, s.first + (end - at));
+  s.group = (int)(in / places);
+  const int from = (int)(in - (long long)s.group * places), to = (int)min((long long)places, from + (end - at));
+  s.places = to - from;
+  s.first = max(from - kStart, 0);
+  s.last = max(to - kStart, 0);
+  s.begun = from > kStart;
+  s.whole = !s.begun && to == places;
   return s;
 }
 
@@ -236,7 +254,7 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas_per_sm<D, NG>())
   if (warp == 0) {
     long long base = 0;
     for (int r0 = 0; r0 < a.R; r0 += 32) {
-      const int t = r0 + lane < a.R ? dec_tiles(a, r0 + lane) : 0;
+      const int t = r0 + lane < a.R ? dec_places(dec_tiles(a, r0 + lane)) : 0;
       long long incl = (long long)t * groups;
 #pragma unroll
       for (int off = 1; off < 32; off <<= 1) {
@@ -263,6 +281,7 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas_per_sm<D, NG>())
     bool dead = false;
     for (long long at = begin; at < end;) {
       const DecSegment sg = dec_segment(a, groups, at, end, r, r_at);
+      at += sg.places;
       const int hk = sg.group / a.ngrp;
       const int* row = a.table + (long long)sg.r * a.W;
       auto page_of = [&](int t) { return t < sg.last ? row[t >> tiles_page] : -1; };
@@ -284,16 +303,14 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas_per_sm<D, NG>())
         if (step >= NST && !dead) dead = !mbar_wait_sleep(empty(st), ((step / NST) - 1) & 1, kSiteDecLoad);
         dead = __any_sync(0xffffffffu, dead);
         const int my = __shfl_sync(0xffffffffu, id, 4 * in + w);
-        const float mk = __shfl_sync(0xffffffffu, ksc, 4 * in + w), mv = __shfl_sync(0xffffffffu, vsc, 4 * in + w);
         const bool live = mt < sg.last && valid(my) && !dead;
         const long long ph = live ? (long long)my * a.Hk + hk : 0;
         const int row0 = (mt & ((1 << tiles_page) - 1)) << 4;
         float* info = infos + (st * kDecWarps + w) * kInfoFloats;
         const int role = lane >> 2;
-        if (role == 3) info[16] = mk, info[17] = mv, info[18] = live ? 1.f : 0.f;
         const int n_live = __popc(__ballot_sync(0xffffffffu, live) & 0xfu);
-        __syncwarp();
-        if (lane == 0) mbar_expect_tx(full(st), (uint32_t)(n_live * (2 * TILE + (a.gc ? 64 : 0))));
+        // the bytes are announced and asked for; the stage is handed over below, with the scales
+        if (lane == 0) mbar_announce(full(st), (uint32_t)(n_live * (2 * TILE + (a.gc ? 64 : 0))));
         __syncwarp();
         if (live) {
           const uint32_t kd = smem_u32(ring + st * STAGE + w * TILE), vd = kd + kDecWarps * TILE;
@@ -303,8 +320,11 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas_per_sm<D, NG>())
           if (D == 256 && role == 4) tma_load_3d(kd + 2048, &tm_k, 128, row0, (int)ph, full(st));
           if (D == 256 && role == 5) tma_load_3d(vd + 2048, &tm_v, 128, row0, (int)ph, full(st));
         }
+        const float mk = __shfl_sync(0xffffffffu, ksc, 4 * in + w), mv = __shfl_sync(0xffffffffu, vsc, 4 * in + w);
+        if (role == 3) info[16] = mk, info[17] = mv, info[18] = live ? 1.f : 0.f;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(full(st));
       }
-      at += sg.last - sg.first;
     }
     // no copy may be in flight when the CTA exits
     if (lane == 0)
@@ -319,6 +339,8 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas_per_sm<D, NG>())
   bool dead = false;
   for (long long at = begin; at < end;) {
     const DecSegment sg = dec_segment(a, groups, at, end, r, r_at);
+    at += sg.places;
+    if (sg.first >= sg.last) continue;
     const int hk = sg.group / a.ngrp, hg = sg.group - hk * a.ngrp;
     const int h0 = hk * a.g + hg * 8 * NG, nh = min(a.g - hg * 8 * NG, 8 * NG);
     const int n = sg.n;
@@ -589,9 +611,9 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas_per_sm<D, NG>())
       named_bar_sync(2, 64);
       if (warp == 0) {
         take(xchg + 32 * dec_xchg_words<D, NG>());
-        const bool whole = sg.first == 0 && sg.last == sg.tiles;
-        // parts of a row group: the first of a CTA's share in place 0, a later one (its last) in place 1
-        const long long part = (2ll * blockIdx.x + (at == begin ? 0 : 1)) * (8 * NG);
+        const bool whole = sg.whole;
+        // parts of a row group: one that an earlier CTA began in place 0, one begun here in place 1
+        const long long part = (2ll * blockIdx.x + (sg.begun ? 0 : 1)) * (8 * NG);
 #pragma unroll
         for (int x = 0; x < NG; ++x)
 #pragma unroll
@@ -626,27 +648,26 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas_per_sm<D, NG>())
           }
       }
     }
-    at += sg.last - sg.first;
   }
 }
 
 // Joins the parts of the row groups that several CTAs worked on. CTA = (request, query head); a warp
-// takes every kJoinWarps-th part, a lane four dimensions.
-constexpr int kJoinWarps = 8;
-
-template <typename T, int D, int NG>
-__global__ void __launch_bounds__(kJoinWarps * 32) paged_decode_join_kernel(const DecodeArgs a) {
+// takes every JW-th part, a lane four dimensions.
+// (few rows have many parts each: 16 warps; many rows few: 4, so that all CTAs fit at once)
+template <typename T, int D, int NG, int JW>
+__global__ void __launch_bounds__(JW * 32) paged_decode_join_kernel(const DecodeArgs a) {
   constexpr int VEC = D >= 128 ? 4 : D / 32, COLS = D / (32 * VEC);  // D = 32: 1 x 1, 64: 2 x 1, 128: 4 x 1, 256: 4 x 2
-  __shared__ long long s_sums[2 * kJoinWarps];
-  __shared__ float s_m[kJoinWarps], s_l[kJoinWarps];
-  __shared__ __align__(16) float s_o[kJoinWarps][D];
+  __shared__ long long s_sums[2 * JW];
+  __shared__ float s_m[JW], s_l[JW];
+  __shared__ __align__(16) float s_o[JW][D];
   const int h = blockIdx.x, r = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int tiles = dec_tiles(a, r);
   const int hk = h / a.g, hg = (h - hk * a.g) / (8 * NG), groups = a.Hk * a.ngrp;
   long long before;
-  const long long units = dec_count<kJoinWarps * 32>(a, r, before, s_sums) * groups;
+  const long long units = dec_count<JW * 32>(a, r, before, s_sums) * groups;
   const long long per = dec_share(units, a.ctas);
-  const long long lo = before * groups + (long long)(hk * a.ngrp + hg) * tiles, hi = lo + tiles;
+  // the places of the row group's first tile and of the one after its last
+  const long long lo = before * groups + (long long)(hk * a.ngrp + hg) * dec_places(tiles) + kStart, hi = lo + tiles;
   const int c0 = (int)(lo / per), c1 = (int)((hi - 1) / per);
   const int hl = h - hk * a.g - hg * 8 * NG;
   asm volatile("griddepcontrol.wait;" ::: "memory");  // every CTA waits: this grid must not end before the first one
@@ -657,8 +678,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_decode_join_kernel(cons
 #pragma unroll
     for (int e = 0; e < VEC; ++e) o[j][e] = 0.f;
 #pragma unroll 4
-  for (int c = c0 + warp; c <= c1; c += kJoinWarps) {
-    const long long p = (2ll * c + (c * per >= lo ? 0 : 1)) * (8 * NG) + hl;
+  for (int c = c0 + warp; c <= c1; c += JW) {
+    const long long p = (2ll * c + (c * per > lo ? 0 : 1)) * (8 * NG) + hl;
     const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * p);
     const float mn = fmaxf(m, ml.x);
     const float f = m == -INFINITY ? 0.f : dec_ex2(m - mn), g = ml.x == -INFINITY ? 0.f : dec_ex2(ml.x - mn);
@@ -677,12 +698,12 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_decode_join_kernel(cons
 #pragma unroll
     for (int e = 0; e < VEC; ++e) s_o[warp][j * 128 + lane * VEC + e] = o[j][e];
   __syncthreads();
-  for (int d = tid; d < D; d += kJoinWarps * 32) {
+  for (int d = tid; d < D; d += JW * 32) {
     float mm = -INFINITY, ll = 0.f, acc = 0.f;
 #pragma unroll
-    for (int w = 0; w < kJoinWarps; ++w) mm = fmaxf(mm, s_m[w]);
+    for (int w = 0; w < JW; ++w) mm = fmaxf(mm, s_m[w]);
 #pragma unroll
-    for (int w = 0; w < kJoinWarps; ++w) {
+    for (int w = 0; w < JW; ++w) {
       const float f = s_m[w] == -INFINITY ? 0.f : dec_ex2(s_m[w] - mm);
       ll = fmaf(s_l[w], f, ll);
       acc = fmaf(s_o[w][d], f, acc);
@@ -727,7 +748,7 @@ cudaError_t decode_launch(DecodeArgs a, const PagedCache& c, cudaStream_t s) {
   if (e != cudaSuccess) return e;
   a.ngrp = (a.g + 8 * NG - 1) / (8 * NG);
   // no more CTAs than the table has tiles for
-  const long long units = (((long long)a.W << a.page_shift) + 15) / 16 * a.R * a.Hk * a.ngrp;
+  const long long units = ((((long long)a.W << a.page_shift) + 15) / 16 + kStart) * a.R * a.Hk * a.ngrp;
   const long long want = (units + kMinTiles - 1) / kMinTiles;
   a.ctas = 148 * dec_ctas_per_sm<D, NG>();
   if (want < a.ctas) a.ctas = (int)want;
@@ -735,14 +756,15 @@ cudaError_t decode_launch(DecodeArgs a, const PagedCache& c, cudaStream_t s) {
   if ((e = cudaGetLastError()) != cudaSuccess || a.ctas == 1) return e;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)a.Hq, (unsigned)a.R);
-  cfg.blockDim = dim3(kJoinWarps * 32);
+  const bool few = (long long)a.R * a.Hq < 148 * 4;
+  cfg.blockDim = dim3(few ? 16 * 32 : 4 * 32);
   cfg.stream = s;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, paged_decode_join_kernel<T, D, NG>, a);
+  return cudaLaunchKernelEx(&cfg, few ? paged_decode_join_kernel<T, D, NG, 16> : paged_decode_join_kernel<T, D, NG, 4>, a);
 }
 
 template <typename T, typename C>
