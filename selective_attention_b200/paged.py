@@ -27,6 +27,8 @@ from .utils import check_cuda, check_ndim, check_shape, to_contiguous
 PAGE_SIZES = (16, 32, 64, 128)
 CACHE_HEAD_DIMS = (32, 64, 128, 256)
 _I32, _I64, _F32 = torch.int32, torch.int64, torch.float32
+_FUNCTIONS = {}  # the C entries by name
+_current_device, _current_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
 
 # Each call looks its arguments over in one expression, and where that fails goes through them one by
@@ -45,20 +47,18 @@ def _int32(t: torch.Tensor, name: str, shape=None) -> None:
         check_shape(t, shape, name)
 
 
-class _on:
-    """The device of a call's tensors as the current one (it mostly is)."""
-
-    def __init__(self, dev):
-        here = torch._C._cuda_getDevice()
-        self.guard = None if here == dev.index else torch.cuda.device(dev)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *e):
-        if self.guard is not None:
-            self.guard.__exit__(*e)
+def _call(name: str, d: int, *args) -> None:
+    """One C entry with the tensors' device as the current one (it mostly is), on its current stream."""
+    fn = _FUNCTIONS.get(name)
+    if fn is None:
+        fn = _FUNCTIONS[name] = getattr(_lib.lib(), name)
+    if _current_device() == d:
+        status = fn(*args, _current_stream(d))
+    else:
+        with torch.cuda.device(d):
+            status = fn(*args, _current_stream(d))
+    if status:
+        _lib.check(status, name)
 
 
 def _plan_faults(lengths, new_lengths, block_table, free_pages, free_state, num_tokens, page_size) -> None:
@@ -108,15 +108,14 @@ def sattn_paged_plan(lengths, new_lengths, block_table, free_pages, free_state, 
     R, W = shape
     dev = lengths.device
     # the int32 outputs are parts of one allocation, as are the int64 ones
-    lengths_out, cu_new, positions = torch.empty(2 * R + 1 + num_tokens, device=dev, dtype=torch.int32).split_with_sizes(
-        (R, R + 1, num_tokens))
-    slots, state_out = torch.empty(num_tokens + 2, device=dev, dtype=torch.int64).split_with_sizes((num_tokens, 2))
-    with _on(dev):
-        st = _lib.lib().sattn_paged_plan(
-            lengths.data_ptr(), new_lengths.data_ptr(), block_table.data_ptr(), free_pages.data_ptr(),
-            free_state.data_ptr(), lengths_out.data_ptr(), cu_new.data_ptr(), slots.data_ptr(), positions.data_ptr(),
-            state_out.data_ptr(), R, W, free_pages.shape[0], num_tokens, page_size, _lib.stream_handle(dev))
-    _lib.check(st, "sattn_paged_plan")
+    small = torch.empty(2 * R + 1 + num_tokens, device=dev, dtype=_I32)
+    wide = torch.empty(num_tokens + 2, device=dev, dtype=_I64)
+    lengths_out, cu_new, positions = small.split_with_sizes((R, R + 1, num_tokens))
+    slots, state_out = wide.split_with_sizes((num_tokens, 2))
+    at, large = small.data_ptr(), wide.data_ptr()
+    _call("sattn_paged_plan", d, lengths.data_ptr(), new_lengths.data_ptr(), block_table.data_ptr(),
+          free_pages.data_ptr(), free_state.data_ptr(), at, at + 4 * R, large, at + 8 * R + 4, large + 8 * num_tokens, R,
+          W, free_pages.shape[0], num_tokens, page_size)
     return lengths_out, cu_new, slots, positions, state_out
 
 
@@ -222,17 +221,14 @@ def sattn_paged_append(k, v, slots, k_cache, v_cache, k_scale, v_scale, log_gate
             and (log_gate is None) == (log_gate_cache is None)
             and (log_gate is None or (log_gate.shape == (T, H) and log_gate.get_device() == d))):
         _append_faults(k, v, slots, k_cache, log_gate, log_gate_cache, H, D)
-    dev = k.device
     code = _lib.DTYPE_CODES[k.dtype]
     slots = to_contiguous(slots)
     if log_gate is not None:
         log_gate = to_contiguous(log_gate.float())
     k, k_ts, k_hs = _rows(k)
     v, v_ts, v_hs = _rows(v)
-    with _on(dev):
-        st = _lib.lib().sattn_paged_append(c, k.data_ptr(), v.data_ptr(), _lib.ptr(log_gate), slots.data_ptr(), T, k_ts,
-                                           k_hs, v_ts, v_hs, code, _lib.stream_handle(dev))
-    _lib.check(st, "sattn_paged_append")
+    _call("sattn_paged_append", d, c, k.data_ptr(), v.data_ptr(), None if log_gate is None else log_gate.data_ptr(),
+          slots.data_ptr(), T, k_ts, k_hs, v_ts, v_hs, code)
 
 
 def sattn_paged_read(slots, k_cache, v_cache, k_scale, v_scale, dtype: torch.dtype = torch.float32):
@@ -249,10 +245,7 @@ def sattn_paged_read(slots, k_cache, v_cache, k_scale, v_scale, dtype: torch.dty
     n = slots.shape[0]
     k = torch.empty((n, H, D), device=dev, dtype=dtype)
     v = torch.empty((n, H, D), device=dev, dtype=dtype)
-    with _on(dev):
-        st = _lib.lib().sattn_paged_read(c, slots.data_ptr(), n, k.data_ptr(), v.data_ptr(), code,
-                                         _lib.stream_handle(dev))
-    _lib.check(st, "sattn_paged_read")
+    _call("sattn_paged_read", d, c, slots.data_ptr(), n, k.data_ptr(), v.data_ptr(), code)
     return k, v
 
 
@@ -314,11 +307,8 @@ def sattn_paged_decode(q, k_cache, v_cache, k_scale, v_scale, block_table, lengt
     need = _decode_workspace(H, page, D, Hq)
     if workspace is None or workspace.numel() * workspace.element_size() < need or workspace.data_ptr() % 16:
         workspace = torch.empty(need, device=dev, dtype=torch.uint8)
-    with _on(dev):
-        st = _lib.lib().sattn_paged_decode(c, q.data_ptr(), block_table.data_ptr(), lengths.data_ptr(), out.data_ptr(),
-                                           R, W, Hq, D ** -0.5 if scale is None else float(scale), code,
-                                           workspace.data_ptr(), need, _lib.stream_handle(dev))
-    _lib.check(st, "sattn_paged_decode")
+    _call("sattn_paged_decode", d, c, q.data_ptr(), block_table.data_ptr(), lengths.data_ptr(), out.data_ptr(), R, W, Hq,
+          D ** -0.5 if scale is None else float(scale), code, workspace.data_ptr(), need)
     return out
 
 
@@ -387,7 +377,5 @@ def sattn_prefill_packed(q, k, v, cu_seqlens, log_gate=None, scale=None, out=Non
     p = _PACKED.pack(T, cu_seqlens.shape[0] - 1, Hq, Hk, D, q_ts, q_hs, k_ts, k_hs, v_ts, v_hs, code, _lib.IMPLS[impl],
                      D ** -0.5 if scale is None else float(scale), q.data_ptr(), k.data_ptr(), v.data_ptr(),
                      0 if log_gate is None else log_gate.data_ptr(), cu_seqlens.data_ptr(), out.data_ptr())
-    with _on(dev):
-        st = _lib.lib().sattn_prefill_packed(p, _lib.stream_handle(dev))
-    _lib.check(st, "sattn_prefill_packed")
+    _call("sattn_prefill_packed", d, p)
     return out
