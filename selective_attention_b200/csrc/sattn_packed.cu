@@ -247,7 +247,7 @@ template <int D> constexpr int pk_slots() { return D == 128 ? 5 : 8; }
 // Gates of tile j + G may take the place of tile j's: V_{j + G} is loaded when element
 // 2 (j + G) + 1 - slots has been used, K_{j + 1} or V_j, that is after the softmaxes of tile j.
 template <int D> constexpr int pk_gate_slots() { return D == 128 ? 3 : 4; }
-template <int D> constexpr int pk_bar_bytes() { return D == 128 ? 304 : 352; }
+template <int D> constexpr int pk_bar_bytes() { return D == 128 ? 320 : 368; }
 template <int D, bool GATED> constexpr size_t pk_smem() {
   return 1024 + (size_t)(2 + pk_slots<D>()) * pk_tile_bytes<D>() + (GATED ? pk_gate_slots<D>() * 128 * 4 : 0) + pk_bar_bytes<D>();
 }
@@ -397,7 +397,7 @@ __global__ void __launch_bounds__(kPkThreads, 1)
   uint64_t* bars = reinterpret_cast<uint64_t*>(gates + (GATED ? pk_gate_slots<D>() * 128 : 0));
   enum {
     Q_FULL = 0, Q_EMPTY = 1, FULL = 2, EMPTY = FULL + NS, CLEAN = EMPTY + NS, CARE_V = CLEAN + kCleanSlots,
-    CARE = CARE_V + 2, S_FULL = CARE + 2, P_FULL = S_FULL + 2, O_DONE = P_FULL + 2, O_FREE = O_DONE + 2,
+    CARE = CARE_V + 4, S_FULL = CARE + 4, P_FULL = S_FULL + 2, O_DONE = P_FULL + 2, O_FREE = O_DONE + 2,
     W_FULL = O_FREE + 2, W_EMPTY = W_FULL + 2, ANSWERED = W_EMPTY + 2, DRAIN = ANSWERED + 1, NBARS = DRAIN + 1
   };
   uint32_t* tslot = reinterpret_cast<uint32_t*>(bars + NBARS);
@@ -414,7 +414,7 @@ __global__ void __launch_bounds__(kPkThreads, 1)
     for (int i = 0; i < NBARS; ++i) {
       int n = 1;
       if (i >= CLEAN && i < CLEAN + kCleanSlots) n = 2;  // two cleaning warps
-      if (i >= CARE && i < CARE + 2) n = 2;
+      if (i >= CARE && i < CARE + 4) n = 2;
       if (i >= P_FULL && i < P_FULL + 2) n = 4;          // the four warps of a softmax
       if (i >= O_FREE && i < O_FREE + 2) n = 4;
       if (i >= W_EMPTY && i < W_EMPTY + 2) n = 11;       // every warp but the loading one
@@ -440,6 +440,10 @@ __global__ void __launch_bounds__(kPkThreads, 1)
     w.seq0 = s.seq0, w.q0 = s.q0, w.n = s.n, w.head = s.head;
     return true;
   };
+  // The barriers of a work's one or two last key tiles (c) are those of every other work: the loading and
+  // cleaning warps may be a work ahead of the others, but not two (a work's place is free when every
+  // role is done with it). `second` counts the works of either kind so far that have two.
+  auto care_parity = [&](int it, int c, const int (&second)[2]) { return (c ? second[it & 1] : it >> 1) & 1; };
   auto work_done = [&](int it) {
     __syncwarp();
     if (lane == 0) mbar_arrive(bar(W_EMPTY + (it & 1)));
@@ -492,7 +496,7 @@ __global__ void __launch_bounds__(kPkThreads, 1)
             if (!ok) break;
             // V tiles that are to be cleaned arrive on a barrier of their own (the ring's goes on)
             const bool special = (e & 1) && j >= care;
-            const uint32_t b_in = bar(special ? CARE_V + j - care : FULL + sl);
+            const uint32_t b_in = bar(special ? CARE_V + 2 * (it & 1) + j - care : FULL + sl);
             if (lane == 0) {
               if (special) mbar_arrive(bar(FULL + sl));
               mbar_expect_tx(b_in, (uint32_t)TILE);
@@ -533,7 +537,7 @@ __global__ void __launch_bounds__(kPkThreads, 1)
     const uint32_t vd = desc_lo(__shfl_sync(0xffffffffu, smem_u32(slot_at(0)), 0), 16384);
     const bool lead = elect_one();
     auto wait = [&](uint32_t b, uint32_t parity) { return (bool)__all_sync(0xffffffffu, mbar_wait(b, parity, kSitePkMma)); };
-    int i0 = 0, cleaned = 0, care_used[2] = {0, 0}, steps[2] = {0, 0}, outs[2] = {0, 0};
+    int i0 = 0, cleaned = 0, second[2] = {0, 0}, steps[2] = {0, 0}, outs[2] = {0, 0};
     bool fail = false;
     for (int it = 0; !fail; ++it) {
       PackedWork work;
@@ -541,7 +545,6 @@ __global__ void __launch_bounds__(kPkThreads, 1)
         fail = true;
         break;
       }
-      work_done(it);
       if (work.head < 0) break;
       const int n0 = __shfl_sync(0xffffffffu, work.tiles0(), 0), n1 = __shfl_sync(0xffffffffu, work.tiles1(PAIR), 0);
       const int first_care = n0 - 1, nkt = max(n0, n1);
@@ -550,7 +553,8 @@ __global__ void __launch_bounds__(kPkThreads, 1)
         return wait(bar(FULL + (i0 + 2 * j) % NS), ((i0 + 2 * j) / NS) & 1);
       };
       auto ready_v = [&](int j) {
-        if (j >= first_care) return wait(bar(CARE + j - first_care), care_used[j - first_care]++ & 1);
+        if (j >= first_care)
+          return wait(bar(CARE + 2 * (it & 1) + j - first_care), care_parity(it, j - first_care, second));
         if (GATED) return wait(bar(CLEAN + (cleaned + j) % kCleanSlots), ((cleaned + j) / kCleanSlots) & 1);
         return wait(bar(FULL + (i0 + 2 * j + 1) % NS), ((i0 + 2 * j + 1) / NS) & 1);
       };
@@ -565,7 +569,7 @@ __global__ void __launch_bounds__(kPkThreads, 1)
           }
           umma_commit(bar(S_FULL + w));
           if (last) {
-            umma_commit(bar(EMPTY + sl));
+            if (!GATED || j < first_care) umma_commit(bar(EMPTY + sl));
             if (j == nkt - 1) umma_commit(bar(Q_EMPTY));
           }
         }
@@ -598,7 +602,12 @@ __global__ void __launch_bounds__(kPkThreads, 1)
 #pragma unroll
             for (int ks = 0; ks < 8; ++ks)
               mma_ts(tm + T_O + 128 * w, tm + T_S + 128 * w + 8 * ks, v1 + (uint32_t)(128 * ks), ID_O, j > 0 || ks > 0);
-            if (w == (j < n1 ? 1 : 0)) umma_commit(bar(EMPTY + sl));  // V_j has been used
+            if (w == (j < n1 ? 1 : 0)) {
+              umma_commit(bar(EMPTY + sl));  // V_j has been used
+              // The cleaning warps wait for the last K tiles, too, but hand over nothing before V: only now
+              // is it certain that they have seen this one, and its place may be filled again.
+              if (GATED && j >= first_care) umma_commit(bar(EMPTY + (i0 + 2 * j) % NS));
+            }
           }
           if (j + 1 < nw) {
             issue_s(w, j + 1, w == (j + 1 < n1 ? 1 : 0));  // over P_w(j): products run in the order of their issue
@@ -610,6 +619,8 @@ __global__ void __launch_bounds__(kPkThreads, 1)
       }
       i0 += 2 * nkt;
       cleaned += first_care;
+      second[it & 1] += nkt > n0;
+      work_done(it);
     }
     // every product has completed before TMEM is released
     if (lead) umma_commit(bar(DRAIN));
@@ -618,7 +629,7 @@ __global__ void __launch_bounds__(kPkThreads, 1)
     // ------------------------------------------------------------ clean tiles
     regs_dec<56>();
     const int t = tid - 64;  // 0 .. 63: keys t and t + 64 of a tile
-    int i0 = 0, cleaned = 0, tiles = 0, care_used[2] = {0, 0};
+    int i0 = 0, cleaned = 0, tiles = 0, second[2] = {0, 0};
     bool ok = true;
     for (int it = 0; ok; ++it) {
       PackedWork work;
@@ -639,7 +650,7 @@ __global__ void __launch_bounds__(kPkThreads, 1)
         if (j < care)
           ok = ok && mbar_wait_sleep(bar(FULL + (ik + 1) % NS), ((ik + 1) / NS) & 1, kSitePkClean);
         else
-          ok = ok && mbar_wait_sleep(bar(CARE_V + j - care), care_used[j - care]++ & 1, kSitePkClean);
+          ok = ok && mbar_wait_sleep(bar(CARE_V + 2 * (it & 1) + j - care), care_parity(it, j - care, second), kSitePkClean);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         if constexpr (GATED) {
@@ -699,11 +710,12 @@ __global__ void __launch_bounds__(kPkThreads, 1)
         }
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(bar(j >= care ? CARE + j - care : CLEAN + (cleaned + j) % kCleanSlots));
+        if (lane == 0) mbar_arrive(bar(j >= care ? CARE + 2 * (it & 1) + j - care : CLEAN + (cleaned + j) % kCleanSlots));
       }
       i0 += 2 * nk;
       cleaned += care;
       tiles += nk;
+      second[it & 1] += nk > care + 1;
       work_done(it);
     }
   } else {
@@ -714,7 +726,7 @@ __global__ void __launch_bounds__(kPkThreads, 1)
     const uint32_t tl = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t ts = tmem + tl + T_S + 128 * w, to = tmem + tl + T_O + 128 * w;
     const float scale2 = a.scale * kPkLog2e;
-    int tiles = 0, cleaned = 0, care_used[2] = {0, 0}, steps = 0, outs = 0;
+    int tiles = 0, cleaned = 0, second[2] = {0, 0}, steps = 0, outs = 0;
     bool wfail = false;
     auto warp_wait = [&](uint32_t b, uint32_t parity) {
       if (!wfail) wfail = !__all_sync(0xffffffffu, mbar_wait(b, parity, kSitePkSoft));
@@ -731,8 +743,8 @@ __global__ void __launch_bounds__(kPkThreads, 1)
       for (int j = 0; j < my_nk; ++j) {
         if (!warp_wait(bar(S_FULL + w), steps & 1)) break;
         ++steps;
-        if (GATED && !warp_wait(j >= care ? bar(CARE + j - care) : bar(CLEAN + (cleaned + j) % kCleanSlots),
-                                j >= care ? (care_used[j - care] & 1) : ((cleaned + j) / kCleanSlots) & 1))
+        if (GATED && !warp_wait(j >= care ? bar(CARE + 2 * (it & 1) + j - care) : bar(CLEAN + (cleaned + j) % kCleanSlots),
+                                j >= care ? care_parity(it, j - care, second) : ((cleaned + j) / kCleanSlots) & 1))
           break;
         tc_fence_after();
         uint32_t sv[4][32];
@@ -891,8 +903,7 @@ __global__ void __launch_bounds__(kPkThreads, 1)
       }
       tiles += max(nk0, nk1);
       cleaned += care;
-      ++care_used[0];
-      if (max(nk0, nk1) > nk0) ++care_used[1];
+      second[it & 1] += max(nk0, nk1) > nk0;
       work_done(it);
     }
   }

@@ -99,6 +99,27 @@ def test_lengths(dtype, lens, D):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("gated", [True, False])
+@pytest.mark.parametrize("D", [64, 128])
+def test_long_and_short_works_follow_one_another(D, gated):
+    """Heads that cannot be paired: works of two, one and no second tile, several for each CTA, checked
+    against the CUDA-core kernel (fp32 sums over the same 16-bit inputs), twice with the same result."""
+    import selective_attention_b200 as sab
+
+    lens = [2047, 1, 758, 1266, 300, 129, 1900, 17, 640, 1024, 385]
+    qkv, gate, cu = make(lens, 24, 24, D, torch.bfloat16, gated, seed=9)
+    d, g = qkv.cuda(), None if gate is None else gate.cuda()
+    args = (d[:, :24], d[:, 24:48], d[:, 48:], cu.cuda(), g)
+    ref = sab.sattn_prefill_packed(*args, impl="simt")
+    got = sab.sattn_prefill_packed(*args, impl="tc")
+    sab.check_device_error()
+    vmax = d[:, 48:].float().abs().max().item()
+    close(got, ref.float(), 2 * vmax, "against the CUDA cores")  # (both sides round)
+    for _ in range(3):
+        assert torch.equal(got, sab.sattn_prefill_packed(*args, impl="tc"))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("impl", ["auto", "simt"])
 def test_many_short_sequences_and_padding_rows(impl):
     lens = [(7 * i) % 41 for i in range(150)]
