@@ -13,7 +13,8 @@ Public surface (mirrors the reference's ``selective_attention.ops`` and
   ``libssd_b200.so`` (``include/ssd_b200.h``).
 - ``paged``: served selective attention, a paged 8-bit cache for many requests
   (``sattn_paged_plan``, ``sattn_paged_append``, ``sattn_paged_decode``, ``sattn_paged_read``) and
-  attention over packed prompts with grouped heads (``sattn_prefill_packed``).
+  attention over packed prompts with grouped heads (``sattn_prefill_packed``); ``PagedSelectiveCache``
+  keeps the pages of a stack of layers and the requests in them.
 - ``HostStreamScan``: the SSD forward on inputs in pinned host memory, with the copies
   of row slices overlapped with the scan (no reference counterpart).
 - ``shim.install()``: make an installed reference package use these kernels.
@@ -40,6 +41,7 @@ from .kernels import (
     state_passing_forward,
 )
 from .paged import (
+    PagedSelectiveCache,
     sattn_paged_append,
     sattn_paged_decode,
     sattn_paged_plan,
@@ -52,6 +54,6 @@ __all__ = [
     "chunk_state_forward", "state_passing_forward", "bmm_chunk_forward", "chunk_scan_forward",
     "ssd_scan_backward", "ssm_conv_prefill", "ssm_conv_decode", "sattn_decode_step", "selective_attn_step",
     "sattn_prefill", "sattn_train_forward", "sattn_train_backward", "SelectiveAttnTrainFn", "selective_attn_train",
-    "sattn_paged_plan", "sattn_paged_append", "sattn_paged_decode", "sattn_paged_read", "sattn_prefill_packed",
+    "sattn_paged_plan", "sattn_paged_append", "sattn_paged_decode", "sattn_paged_read", "sattn_prefill_packed", "PagedSelectiveCache",
     "check_device_error", "device_error",
 ]

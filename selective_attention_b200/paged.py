@@ -379,3 +379,71 @@ def sattn_prefill_packed(q, k, v, cu_seqlens, log_gate=None, scale=None, out=Non
                      0 if log_gate is None else log_gate.data_ptr(), cu_seqlens.data_ptr(), out.data_ptr())
     _call("sattn_prefill_packed", d, p)
     return out
+
+
+class PagedSelectiveCache:
+    """The paged caches of a stack of selective-attention layers and the requests that they hold.
+
+    ``requests`` rows, each up to ``max_tokens`` tokens, share ``num_pages`` pages of ``page_size``
+    tokens in every layer (a page has the same number in all of them). A step is: :meth:`plan` for the
+    numbers of new tokens, then for each layer :meth:`append` of their keys, values and log-gates and
+    either :func:`sattn_prefill_packed` (whole prompts, packed by the plan's ``cu_seqlens``) or
+    :meth:`decode` (one token for each request); :meth:`release` gives a finished request's pages
+    back. Nothing synchronizes: which requests a plan served is read from its ``lengths`` when the
+    host wants to know.
+    """
+
+    def __init__(self, layers: int, requests: int, max_tokens: int, num_pages: int, heads: int, head_dim: int,
+                 page_size: int = 16, dtype: torch.dtype = torch.int8, gated: bool = True, device="cuda"):
+        if page_size not in PAGE_SIZES or head_dim not in CACHE_HEAD_DIMS or dtype not in _lib.CACHE_CODES:
+            raise ValueError(f"expected a page size in {PAGE_SIZES}, a head dim in {CACHE_HEAD_DIMS} and a dtype in "
+                             f"{tuple(_lib.CACHE_CODES)}, got {page_size}, {head_dim}, {dtype}")
+        shape = (layers, num_pages, heads, page_size, head_dim)
+        self.page_size = page_size
+        self.k_cache = torch.zeros(shape, dtype=dtype, device=device)
+        self.v_cache = torch.zeros(shape, dtype=dtype, device=device)
+        self.k_scale = torch.zeros(shape[:3], device=device)
+        self.v_scale = torch.zeros(shape[:3], device=device)
+        self.log_gate_cache = torch.zeros(shape[:4], device=device) if gated else None
+        self.block_table = torch.full((requests, -(-max_tokens // page_size)), -1, dtype=_I32, device=device)
+        self.lengths = torch.zeros(requests, dtype=_I32, device=device)
+        # the ring of free pages, and a place past it for what release() does not return
+        self._ring = torch.arange(num_pages + 1, dtype=_I32, device=device)
+        self.free_state = torch.tensor([0, num_pages], dtype=_I64, device=device)
+
+    @property
+    def free_pages(self) -> torch.Tensor:
+        return self._ring[:-1]
+
+    def layer(self, i: int) -> dict:
+        """Layer ``i``'s cache, as the functions of this module take it."""
+        return dict(k_cache=self.k_cache[i], v_cache=self.v_cache[i], k_scale=self.k_scale[i],
+                    v_scale=self.v_scale[i],
+                    log_gate_cache=None if self.log_gate_cache is None else self.log_gate_cache[i])
+
+    def plan(self, new_lengths: torch.Tensor, num_tokens: int):
+        """Pages for ``new_lengths`` ``(requests,)`` int32 more tokens (0: the request takes no part);
+        ``num_tokens`` is their sum, or more. Returns ``(cu_seqlens, slots, positions)``."""
+        self.lengths, cu, slots, positions, self.free_state = sattn_paged_plan(
+            self.lengths, new_lengths, self.block_table, self.free_pages, self.free_state, num_tokens, self.page_size)
+        return cu, slots, positions
+
+    def append(self, layer: int, k, v, slots, log_gate=None) -> None:
+        sattn_paged_append(k, v, slots, log_gate=log_gate, **self.layer(layer))
+
+    def decode(self, layer: int, q, scale=None, out=None, workspace=None):
+        """Attention of one token for each request (``q`` ``(requests, Hq, D)``) over all that it holds."""
+        return sattn_paged_decode(q, block_table=self.block_table, lengths=self.lengths, scale=scale, out=out,
+                                  workspace=workspace, **self.layer(layer))
+
+    def release(self, rows: torch.Tensor) -> None:
+        """Gives back the pages of the requests ``rows`` (int64 indices, each once)."""
+        held = (self.lengths[rows].long() + self.page_size - 1) // self.page_size
+        at = torch.arange(self.block_table.shape[1], device=rows.device)
+        there = at[None, :] < held[:, None]
+        place = (self.free_state[1] + (held.cumsum(0) - held)[:, None] + at) % (self._ring.shape[0] - 1)
+        place = torch.where(there, place, self._ring.shape[0] - 1)
+        self._ring[place] = self.block_table[rows]
+        self.free_state = self.free_state + torch.stack([torch.zeros_like(held[:1]).sum(), held.sum()])
+        self.block_table[rows] = -1
+        self.lengths = self.lengths.index_fill(0, rows, 0)

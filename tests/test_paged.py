@@ -457,3 +457,73 @@ def test_gpu_refusals():
         sab.sattn_paged_plan(n, n, t, n, torch.zeros(2, dtype=torch.int64, device="cuda"), 1, 17)
     with pytest.raises(ValueError):
         sab.sattn_paged_read(s.int(), *(c[x] for x in ("k_cache", "v_cache", "k_scale", "v_scale")))
+
+
+# ----------------------------------------------------------------------------- GPU: all of it together
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", [torch.int8, torch.float8_e4m3fn])
+def test_cache_object_over_steps_with_requests_coming_and_going(kind):
+    """Plans, appends, decodes and releases in turn: pages go round the ring, and each decode is that of
+    the oracle on the cache as it stands."""
+    import selective_attention_b200 as sab
+
+    g = torch.Generator().manual_seed(5)
+    c = sab.PagedSelectiveCache(2, 3, 64, 7, 2, 64, 16, kind)
+    news = [[20, 0, 33], [1, 5, 1], [0, 1, 0], "release 0 2", [40, 1, 0], [1, 1, 16], "release 1", [0, 17, 1]]
+    for new in news:
+        if isinstance(new, str):
+            rows = torch.tensor([int(x) for x in new.split()[1:]])
+            c.release(rows.cuda())
+            continue
+        before = c.lengths.cpu()
+        T = sum(new)
+        cu, slots, pos = c.plan(torch.tensor(new, dtype=torch.int32, device="cuda"), T)
+        n = c.lengths.cpu()
+        assert n.tolist() == [b + a for b, a in zip(before.tolist(), new)], "every request is served"
+        assert cu.tolist() == [0] + torch.tensor(new).cumsum(0).tolist()
+        held = [p for r in range(3) for p in c.block_table[r, :-(-int(n[r]) // 16)].tolist()]
+        assert len(set(held)) == len(held) and all(0 <= p < 7 for p in held), "no page has two owners"
+        for layer in range(2):
+            k, v = (torch.randn(T, 2, 64, generator=g).to(torch.bfloat16) for _ in range(2))
+            gate = torch.nn.functional.logsigmoid(torch.randn(T, 2, generator=g))
+            c.append(layer, k.cuda(), v.cuda(), slots, gate.cuda())
+            q = torch.randn(3, 4, 64, generator=g).to(torch.bfloat16)
+            at = {m: None if t is None else t.cpu() for m, t in c.layer(layer).items()}
+            ref = paged_ref.decode(q, at["k_cache"], at["v_cache"], at["k_scale"], at["v_scale"], c.block_table.cpu(),
+                                   n, at["log_gate_cache"])
+            close(c.decode(layer, q.cuda()), ref, 5.0, f"{new} layer {layer}")
+    assert c.free_state[0].item() - 7 <= c.free_state[1].item() - 7 <= c.free_state[0].item()
+
+
+@pytest.mark.gpu
+def test_cache_that_is_full_leaves_requests_waiting():
+    import selective_attention_b200 as sab
+
+    c = sab.PagedSelectiveCache(1, 2, 64, 2, 1, 64, 16)
+    cu, slots, _ = c.plan(torch.tensor([30, 30], dtype=torch.int32, device="cuda"), 60)
+    assert c.lengths.tolist() == [30, 0] and (slots[30:] == -1).all() and (slots[:30] >= 0).all()
+    x = torch.randn(60, 1, 64, device="cuda")
+    c.append(0, x, x, slots, torch.zeros(60, 1, device="cuda"))
+    c.release(torch.tensor([0], device="cuda"))
+    c.plan(torch.tensor([0, 30], dtype=torch.int32, device="cuda"), 30)
+    assert c.lengths.tolist() == [0, 30]
+
+
+@pytest.mark.gpu
+def test_example_serves_every_request_and_returns_every_page():
+    import importlib.util
+    import os
+
+    from conftest import ROOT
+
+    spec = importlib.util.spec_from_file_location("serve_selective", os.path.join(ROOT, "examples", "serve_selective.py"))
+    ex = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(ex)
+    g = torch.Generator().manual_seed(2)
+    prompts = [torch.randint(512, (n,), generator=g).tolist() for n in (3, 40, 17, 1, 64)]
+    budgets = [4, 2, 6, 5, 3]
+    done, cache = ex.serve(prompts, budgets, rows=2)
+    assert [len(done[i]) for i in range(5)] == [len(p) + b for p, b in zip(prompts, budgets)]
+    assert all(done[i][:len(p)] == p for i, p in enumerate(prompts))
+    head, tail = cache.free_state.tolist()
+    assert tail - head == cache.free_pages.numel()  # every page is back
