@@ -220,8 +220,11 @@ cudaError_t packed_simt_t(const PackedArgs& a, cudaStream_t s) {
 //                     the rows that do see one add it at the end (`odd`); with gates, they write the
 //                     tile's gates and set the K and V rows of dropped keys to zero.
 // The bound is the tensor core (4 D operations a score) together with the special-function unit
-// (one exponential a score: 16 a clock and SM, just as long as the products of head_dim 128), so
-// every kPolyEvery-th pair of exponentials is a cubic on the FMA pipes.
+// (one exponential a score: 16 a clock and SM, just as long as the products of head_dim 128).
+// Every second to eighth pair of exponentials on the FMA pipes instead (a cubic) gained 4 % on a cool card
+// and lost 1 to 7 % at the power limit, where such kernels run when there is more than one of them.
+// A prompt of 8192 tokens, 32 heads on 8 of 128, bf16: 477 us (1150 TFLOP/s) cool, 550 us (1000) back to
+// back; a pair of 128 x 128 tiles takes 3400 cycles, of which its products alone 2040.
 // TMEM columns: S_0 [0, 128) S_1 [128, 256) (P_w in the first 64 of S_w) O_0 [256, 256 + D) O_1 [384, 384 + D).
 // Every wait is bounded; a role that gives up records a site code and leaves its loop, and the others'
 // waits for it run out in turn. A CTA goes from one pair of tiles to the next (cluster launch control:
@@ -235,11 +238,6 @@ constexpr int kCleanSlots = 4;
 constexpr float kPkLog2e = 1.4426950408889634f;
 constexpr float kPkRescale = 8.0f * kPkLog2e;
 constexpr unsigned int kSitePkLoad = 0x411, kSitePkMma = 0x412, kSitePkSoft = 0x413, kSitePkClean = 0x414;
-#ifndef SSD_PK_POLY_EVERY
-#define SSD_PK_POLY_EVERY 4
-#endif
-constexpr int kPolyEvery = SSD_PK_POLY_EVERY;
-
 template <int D> constexpr int pk_tile_bytes() { return 128 * D * 2; }
 // One ring for the tiles of K and V in the order of their use, K_0 V_0 K_1 V_1 ...: what shared memory
 // holds beside the two Q tiles.
@@ -258,12 +256,6 @@ __device__ __forceinline__ float pk_ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// (a NaN stays one)
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float y;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
-  return y;
-}
 // Packed fp32 pairs.
 __device__ __forceinline__ uint64_t pk2(float a, float b) {
   return (uint64_t)__float_as_uint(a) | ((uint64_t)__float_as_uint(b) << 32);
@@ -280,20 +272,13 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
 }
 __device__ __forceinline__ float lo2(uint64_t x) { return __uint_as_float((uint32_t)x); }
 __device__ __forceinline__ float hi2(uint64_t x) { return __uint_as_float((uint32_t)(x >> 32)); }
-// 2^d for a pair on the FMA pipes: d = n + f, n the nearest integer (left in the low mantissa bits by
-// adding 1.5 * 2^23), 2^f by a cubic least-squares fit on [-0.5, 0.5] (relative error below 8e-5,
-// against 4.9e-4 or more of the 16-bit rounding that follows), n added to the exponent. d is held
-// at -125 or above, so that the exponent stays normal: 2^-125 stands for 0.
-__device__ __forceinline__ uint64_t ex2_fma(uint64_t x) {
-  constexpr float kMagic = 12582912.0f;
-  const uint64_t d = pk2(fmaxf(lo2(x), -125.f), fmaxf(hi2(x), -125.f));
-  const uint64_t r = add2(d, pk2(kMagic, kMagic));
-  const uint64_t f = add2(d, add2(pk2(kMagic, kMagic), r ^ 0x8000000080000000ull));
-  uint64_t p = fma2(f, pk2(0.055171605f, 0.055171605f), pk2(0.24261111f, 0.24261111f));
-  p = fma2(p, f, pk2(0.69326097f, 0.69326097f));
-  p = fma2(p, f, pk2(0.99992806f, 0.99992806f));
-  return (uint64_t)((uint32_t)p + ((uint32_t)r << 23)) |
-         ((uint64_t)((uint32_t)(p >> 32) + ((uint32_t)(r >> 32) << 23)) << 32);
+// A wait for warps that mostly wait: suspended in the barrier, so that they take neither issue slots nor
+// power from the others. Bounded by the number of waits, each of at most about 10 us.
+__device__ __forceinline__ bool idle_wait(uint32_t bar, uint32_t parity, unsigned int site) {
+  for (uint32_t it = 0; it < 100000u; ++it)
+    if (mbar_try_wait(bar, parity, 10000u)) return true;
+  record_error(site);
+  return false;
 }
 
 // Low word of a 128-byte-swizzled operand's descriptor; the high word is the same for all of them (8-row
@@ -472,13 +457,13 @@ __global__ void __launch_bounds__(kPkThreads, 1)
       } else {
         PackedWork w{tile.tok0 - tile.q0, tile.q0, tile.n, head, 0};
         const int n0 = w.tiles0(), n1 = w.tiles1(PAIR), nk = max(n0, n1), care = n0 - 1, hk = head / group;
-        if (it >= 2) ok = __all_sync(0xffffffffu, mbar_wait(bar(W_EMPTY + (it & 1)), ((it >> 1) - 1) & 1, kSitePkLoad));
+        if (it >= 2) ok = __all_sync(0xffffffffu, idle_wait(bar(W_EMPTY + (it & 1)), ((it >> 1) - 1) & 1, kSitePkLoad));
         if (lane == 0 && ok) {
           volatile PackedWork& s = s_work[it & 1];
           s.seq0 = w.seq0, s.q0 = w.q0, s.n = w.n, s.head = w.head, s.odd = 0;
           mbar_arrive(bar(W_FULL + (it & 1)));
         }
-        if (ok && it > 0) ok = __all_sync(0xffffffffu, mbar_wait(bar(Q_EMPTY), (it - 1) & 1, kSitePkLoad));
+        if (ok && it > 0) ok = __all_sync(0xffffffffu, idle_wait(bar(Q_EMPTY), (it - 1) & 1, kSitePkLoad));
         if (ok) {
           const int nq = n1 > 0 ? 2 : 1;
           if (lane == 0) {
@@ -492,7 +477,7 @@ __global__ void __launch_bounds__(kPkThreads, 1)
           for (int e = 0; e < 2 * nk && ok; ++e) {
             const int i = i0 + e, j = e >> 1, sl = i % NS;
             if (i >= NS)
-              ok = __all_sync(0xffffffffu, mbar_wait(bar(EMPTY + sl), ((i / NS) - 1) & 1, kSitePkLoad));
+              ok = __all_sync(0xffffffffu, idle_wait(bar(EMPTY + sl), ((i / NS) - 1) & 1, kSitePkLoad));
             if (!ok) break;
             // V tiles that are to be cleaned arrive on a barrier of their own (the ring's goes on)
             const bool special = (e & 1) && j >= care;
@@ -514,13 +499,13 @@ __global__ void __launch_bounds__(kPkThreads, 1)
       fence_proxy_async_smem();  // the answer has been read before the next one is written
       __syncwarp();
     }
-    if (ok && it >= 2) ok = __all_sync(0xffffffffu, mbar_wait(bar(W_EMPTY + (it & 1)), ((it >> 1) - 1) & 1, kSitePkLoad));
+    if (ok && it >= 2) ok = __all_sync(0xffffffffu, idle_wait(bar(W_EMPTY + (it & 1)), ((it >> 1) - 1) & 1, kSitePkLoad));
     if (ok && lane == 0) {
       s_work[it & 1].head = -1;
       mbar_arrive(bar(W_FULL + (it & 1)));
       // No copy may be in flight when the CTA exits: the last work has been used up. (After a wait that
       // ran out, every copy has long arrived.)
-      if (it > 0) mbar_wait(bar(W_EMPTY + ((it - 1) & 1)), ((it - 1) >> 1) & 1, kSitePkLoad);
+      if (it > 0) idle_wait(bar(W_EMPTY + ((it - 1) & 1)), ((it - 1) >> 1) & 1, kSitePkLoad);
     }
     __syncwarp();
   } else if (warp == 1) {
@@ -646,11 +631,11 @@ __global__ void __launch_bounds__(kPkThreads, 1)
         const int ik = i0 + 2 * j;
         uint8_t *kt = slot_at(ik), *vt = slot_at(ik + 1);
         // (with gates also K of the tiles that are not changed here: the ring's phases are followed one by one)
-        if (GATED) ok = mbar_wait_sleep(bar(FULL + ik % NS), (ik / NS) & 1, kSitePkClean);
+        if (GATED) ok = idle_wait(bar(FULL + ik % NS), (ik / NS) & 1, kSitePkClean);
         if (j < care)
-          ok = ok && mbar_wait_sleep(bar(FULL + (ik + 1) % NS), ((ik + 1) / NS) & 1, kSitePkClean);
+          ok = ok && idle_wait(bar(FULL + (ik + 1) % NS), ((ik + 1) / NS) & 1, kSitePkClean);
         else
-          ok = ok && mbar_wait_sleep(bar(CARE_V + 2 * (it & 1) + j - care), care_parity(it, j - care, second), kSitePkClean);
+          ok = ok && idle_wait(bar(CARE_V + 2 * (it & 1) + j - care), care_parity(it, j - care, second), kSitePkClean);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         if constexpr (GATED) {
@@ -739,7 +724,6 @@ __global__ void __launch_bounds__(kPkThreads, 1)
       const int care = work.tiles0() - 1, nk0 = work.tiles0(), nk1 = work.tiles1(PAIR), my_nk = w ? nk1 : nk0;
       const int qi = work.q0 + (PAIR ? 0 : 128 * w) + r;
       float m_used = -INFINITY, lsum = 0.f;
-      bool not_a_number = false;  // the row has a score of NaN or +inf
       for (int j = 0; j < my_nk; ++j) {
         if (!warp_wait(bar(S_FULL + w), steps & 1)) break;
         ++steps;
@@ -801,11 +785,12 @@ __global__ void __launch_bounds__(kPkThreads, 1)
 #pragma unroll
         for (int c = 0; c < 4; ++c)
 #pragma unroll
-          for (int e = 0; e < 32; e += 4)
+          for (int e = 0; e < 32; e += 8)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) mp[q] = max_nan(mp[q], __uint_as_float(sv[c][e + q]));
-        const float mt = max_nan(max_nan(mp[0], mp[1]), max_nan(mp[2], mp[3])) * mul;
-        if (!(mt < INFINITY)) not_a_number = true;
+            for (int q = 0; q < 4; ++q)
+              mp[q] = fmaxf(fmaxf(mp[q], __uint_as_float(sv[c][e + 2 * q])), __uint_as_float(sv[c][e + 2 * q + 1]));
+        // (a score of NaN or +inf makes the row's sum NaN or +inf, and its results NaN)
+        const float mt = fmaxf(fmaxf(mp[0], mp[1]), fmaxf(mp[2], mp[3])) * mul;
         float f = 1.f;
         bool resc = false;
         if (mt < INFINITY && mt > m_used + kPkRescale) {
@@ -831,30 +816,18 @@ __global__ void __launch_bounds__(kPkThreads, 1)
         const float mb = m_used == -INFINITY ? 0.f : -m_used;
         const uint64_t mul2 = pk2(mul, mul), mb2 = pk2(mb, mb);
         uint64_t ls[2] = {0ull, 0ull};
-        auto weights = [&](auto cubic) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint32_t pk[16];
+        for (int c = 0; c < 4; ++c) {
+          uint32_t pk[16];
 #pragma unroll
-            for (int q = 0; q < 16; ++q) {
-              const uint64_t d = fma2(pk2(__uint_as_float(sv[c][2 * q]), __uint_as_float(sv[c][2 * q + 1])), mul2, mb2);
-              uint64_t p;
-              if (decltype(cubic)::value && kPolyEvery > 0 && q % (kPolyEvery > 0 ? kPolyEvery : 1) == 0) {
-                p = ex2_fma(d);
-              } else {
-                p = pk2(pk_ex2(lo2(d)), pk_ex2(hi2(d)));
-              }
-              ls[q & 1] = add2(ls[q & 1], p);
-              pk[q] = pack2<T>(lo2(p), hi2(p));
-            }
-            tmem_st16(ts + 16 * c, pk);  // (the scores of these columns are in registers)
+          for (int q = 0; q < 16; ++q) {
+            const uint64_t d = fma2(pk2(__uint_as_float(sv[c][2 * q]), __uint_as_float(sv[c][2 * q + 1])), mul2, mb2);
+            const float p0 = pk_ex2(lo2(d)), p1 = pk_ex2(hi2(d));
+            ls[q & 1] = add2(ls[q & 1], pk2(p0, p1));
+            pk[q] = pack2<T>(p0, p1);
           }
-        };
-        // 2^-125 is no 0 to a large V: where positions are masked every exponential is the hardware's
-        if (j < care)
-          weights(std::true_type{});
-        else
-          weights(std::false_type{});
+          tmem_st16(ts + 16 * c, pk);  // (the scores of these columns are in registers)
+        }
         const uint64_t l2 = add2(ls[0], ls[1]);
         lsum += lo2(l2) + hi2(l2);
         tmem_wait_st();
@@ -865,7 +838,7 @@ __global__ void __launch_bounds__(kPkThreads, 1)
       if (my_nk > 0 && warp_wait(bar(O_DONE + w), outs & 1)) {
         ++outs;
         tc_fence_after();
-        const float inv = not_a_number ? __uint_as_float(0x7fffffffu) : 1.0f / lsum;
+        const float inv = 1.0f / lsum;
         const bool odd = s_work[it & 1].odd != 0;
         const int hk = work.head / group, head = work.head + (PAIR ? w : 0);
         T* op = out + ((long long)(work.seq0 + qi) * a.Hq + head) * D;
