@@ -268,10 +268,13 @@ __global__ void __launch_bounds__(kAppThreads) paged_append_kernel(
     if (i < rows && head_of[i] >= 0) {
       float v[8];
       floats<T>(raw, v);
+      // infinities and NaN do not set the scale (a maximum passes over NaN)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float a = fabsf(v[e]);
-        m = fmaxf(m, a < INFINITY ? a : 0.f);  // infinities and NaN do not set the scale
+      for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(v[e]));
+      if (m == INFINITY) {
+        m = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(v[e]) < INFINITY ? fabsf(v[e]) : 0.f);
       }
     }
     for (int off = 1; off < lpr; off <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
@@ -374,6 +377,7 @@ __global__ void __launch_bounds__(kReadThreads) paged_read_kernel(
   const long long first = (long long)blockIdx.x * per;              // the CTA's slots, `per` of them
   const unsigned row = (unsigned)H << lshift;                       // items of a slot
   const unsigned items = (unsigned)min((long long)per, n - first) * row;
+  const bool wide = (reinterpret_cast<uintptr_t>(out) & 31u) == 0;
   for (unsigned i0 = threadIdx.x; i0 < items; i0 += kReadItems * kReadThreads) {
     uint2 w[kReadItems];
     float sc[kReadItems];
@@ -400,7 +404,7 @@ __global__ void __launch_bounds__(kReadThreads) paged_read_kernel(
       Code<C>::unpack8(w[u], v);
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] *= sc[u];
-      store8<T>(out + (first * row + i) * 8, v);
+      store8_wide<T>(out + (first * row + i) * 8, v, wide);
     }
   }
 }
