@@ -26,7 +26,7 @@ namespace {
 // requests that begin in or reach into its tokens leave an entry at their first token there, and
 // a running maximum over the tokens finds each token's entry. A page's table entry is written by
 // the token at its first position, so no two threads write one entry and none is read that
-// another writes.
+// another writes. Bound by latency: 256 requests of one token each take 3 us, 384 prompts with 393k tokens 5.
 constexpr int kPlanThreads = 256;
 constexpr int kPlanPer = 4;
 constexpr int kPlanTokens = kPlanThreads * kPlanPer;
@@ -167,7 +167,8 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(
 // flight together, and stay in registers as they came (the rows past the first kAppHeld passes
 // are read again); then the largest finite magnitude of each row, the segment's scale from its
 // rows and the page's old scale, and the codes of the rows and, where the scale grew, of the
-// page's older rows. Bound by reading x and writing the codes.
+// page's older rows. 16k tokens of 8 heads of 128 (fp16 to e4m3, K and V) take 50 us, bound by instructions
+// (about 300 for 16 elements of a warp's two rows) between the barriers; their 63 MB alone would take 10.
 constexpr int kAppThreads = 256;
 constexpr int kAppRows = 256;  // rows of one CTA: per + page - 1 <= 255
 constexpr int kAppHeld = 8;
@@ -359,7 +360,8 @@ __global__ void __launch_bounds__(kAppThreads) paged_append_kernel(
 
 // ---------------------------------------------------------------------------
 // read: values of the given slots, (N, H, D) for K and V; slots outside the cache give zeros.
-// One thread reads 8 codes and writes 8 values; bound by writing them.
+// One thread reads 8 codes and writes 8 values, fp32 as a whole 32-byte sector. Bound by writing them: 16k slots
+// of 8 heads of 128 (33 MB read, 132 MB written) take 23 us, the copy rate's time.
 // ---------------------------------------------------------------------------
 constexpr int kReadThreads = 256;
 constexpr int kReadItems = 4;  // of a thread, their codes all in flight
@@ -413,7 +415,7 @@ template <typename T, typename C>
 cudaError_t append_t(const PagedCache& c, const void* k, const void* v, const float* gate, const long long* slots,
                      long long n, long long k_ts, long long k_hs, long long v_ts, long long v_hs, cudaStream_t s) {
   // Few tokens: small blocks, so that many CTAs share them. Many: 128 tokens, which a CTA's threads hold
-  // in registers for head_dim 128 (a page each: 64 us instead of 59 for 16k tokens of 8 heads).
+  // in registers for head_dim 128 (a page of 64 each: 63 us instead of 59 for 16k tokens of 8 heads, events included).
   const int per = n * c.nkv <= 2048 ? 4 : 128;
   const bool vec = (reinterpret_cast<uintptr_t>(k) % 16 == 0) && (reinterpret_cast<uintptr_t>(v) % 16 == 0) &&
                    (k_ts * sizeof(T)) % 16 == 0 && (k_hs * sizeof(T)) % 16 == 0 && (v_ts * sizeof(T)) % 16 == 0 &&
