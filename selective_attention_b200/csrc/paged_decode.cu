@@ -52,6 +52,7 @@ constexpr int kMinTiles = 8;                        // 16-token tiles that a CTA
 constexpr int kEachTiles = 32;                      // see decode_launch
 constexpr int kStart = 8;                           // a row group's start and join, in tiles' time (see below)
 constexpr unsigned int kSiteDecLoad = 0x401, kSiteDecUse = 0x402;
+constexpr int kS64 = 2;
 constexpr float kDecLog2e = 1.4426950408889634f;
 constexpr float kGrow = 8.0f;      // log2: O is rescaled when a row's maximum grows by more
 constexpr float kOffset = 7.0f;    // log2: P = 2^(s - m + 7) <= 2^15
@@ -106,13 +107,18 @@ template <int D> __device__ __forceinline__ int tile_at(int row, int ch) {
   return row * 32 + ((ch ^ ((row >> 2) & 1)) << 4);
 }
 
-template <int D> constexpr int dec_stages() { return D == 256 ? 2 : (D == 128 ? 3 : 4); }
-template <int D> constexpr int dec_stage_bytes() { return kDecWarps * 32 * D; }  // K tiles, V tiles
+// 16-token tiles that a warp takes in one step.
+template <int D, int NG> constexpr int dec_unroll() { return D <= 64 && NG == 1 ? 2 : 1; }
+template <int D, int NG> constexpr int dec_stage_tiles() { return kDecWarps * dec_unroll<D, NG>(); }
+template <int D, int NG> constexpr int dec_stages() {
+  return D == 256 ? 2 : (D == 128 ? 3 : (D == 64 && NG == 1 ? kS64 : 4));
+}
+template <int D, int NG> constexpr int dec_stage_bytes() { return dec_stage_tiles<D, NG>() * 32 * D; }  // K, V tiles
 constexpr int kInfoFloats = 24;                                                  // 16 gates, k_scale, v_scale, live
 // Results of two warps on their way to two others: m, l and O of a lane.
 template <int D, int NG> constexpr int dec_xchg_words() { return NG * (D / 16 * 4 + 4); }
 template <int D, int NG> constexpr size_t dec_smem() {
-  return 1024 + (size_t)dec_stages<D>() * (dec_stage_bytes<D>() + kDecWarps * kInfoFloats * 4) +
+  return 1024 + (size_t)dec_stages<D, NG>() * (dec_stage_bytes<D, NG>() + dec_stage_tiles<D, NG>() * kInfoFloats * 4) +
          2 * 32 * dec_xchg_words<D, NG>() * 4 + 128;
 }
 
@@ -219,7 +225,8 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas_per_sm<D, NG>())
     paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                         const DecodeArgs a) {
   constexpr bool SPLIT = std::is_same<T, float>::value;
-  constexpr int NST = dec_stages<D>(), STAGE = dec_stage_bytes<D>(), TILE = 16 * D;
+  constexpr int NST = dec_stages<D, NG>(), STAGE = dec_stage_bytes<D, NG>(), TILE = 16 * D;
+  constexpr int U = dec_unroll<D, NG>(), GT = dec_stage_tiles<D, NG>();  // tiles of a warp's step and of a stage
   constexpr int KW = D / 16;                 // K words of a lane and row = k-steps
   constexpr int MT = D / 16;                 // 16-row tiles of O^T
   constexpr int VWORDS = D / 32;             // V words of a lane and token
@@ -229,7 +236,7 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas_per_sm<D, NG>())
   __shared__ long long s_at;
   uint8_t* ring = align1024_shared(dsm_raw);
   float* infos = reinterpret_cast<float*>(ring + NST * STAGE);
-  float* xchg = infos + NST * kDecWarps * kInfoFloats;
+  float* xchg = infos + NST * GT * kInfoFloats;
   uint64_t* bars = reinterpret_cast<uint64_t*>(xchg + 2 * 32 * dec_xchg_words<D, NG>());
   auto full = [&](int s) { return smem_u32(&bars[s]); };
   auto empty = [&](int s) { return smem_u32(&bars[NST + s]); };
@@ -290,8 +297,8 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas_per_sm<D, NG>())
 
   if (warp == kDecWarps) {
     // ---------------------------------------------------------------- fetch
-    // Lanes take the four tiles of a stage in turn: lanes 0-3 their K, 4-7 V, 8-11 gates, 12-15 scales,
-    // 16-23 the second column halves of head_dim 256. Page numbers and scales come 32 tiles at a time,
+    // Lanes take the GT tiles of a stage in turn: the first GT lanes their K, then V, gates, scales, and
+    // the second column halves of head_dim 256. Page numbers and scales come 32 tiles at a time,
     // one batch ahead.
     bool dead = false;
     for (long long at = begin; at < end;) {
@@ -304,38 +311,38 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas_per_sm<D, NG>())
       int id = page_of(sg.first + lane), id_next = -1;
       float ksc = 0.f, vsc = 0.f, ksc_next = 0.f, vsc_next = 0.f;
       if (valid(id)) ksc = a.ks[(long long)id * a.Hk + hk], vsc = a.vs[(long long)id * a.Hk + hk];
-      for (int t = sg.first, i = 0; t < sg.last; t += kDecWarps, ++i, ++step) {
-        const int in = i & 7;  // eight steps a batch
+      for (int t = sg.first, i = 0; t < sg.last; t += GT, ++i, ++step) {
+        const int in = i & (32 / GT - 1);  // step of the batch
         if (in == 0) {
           if (i > 0) id = id_next, ksc = ksc_next, vsc = vsc_next;
           id_next = page_of(t + 32 + lane);
-        } else if (in == 4) {
+        } else if (in == 16 / GT) {
           ksc_next = vsc_next = 0.f;
           if (valid(id_next))
             ksc_next = a.ks[(long long)id_next * a.Hk + hk], vsc_next = a.vs[(long long)id_next * a.Hk + hk];
         }
-        const int st = step % NST, w = lane & 3, mt = t + w;
+        const int st = step % NST, w = lane & (GT - 1), mt = t + w;
         if (step >= NST && !dead) dead = !mbar_wait_sleep(empty(st), ((step / NST) - 1) & 1, kSiteDecLoad);
         dead = __any_sync(0xffffffffu, dead);
-        const int my = __shfl_sync(0xffffffffu, id, 4 * in + w);
+        const int my = __shfl_sync(0xffffffffu, id, GT * in + w);
         const bool live = mt < sg.last && valid(my) && !dead;
         const long long ph = live ? (long long)my * a.Hk + hk : 0;
         const int row0 = (mt & ((1 << tiles_page) - 1)) << 4;
-        float* info = infos + (st * kDecWarps + w) * kInfoFloats;
-        const int role = lane >> 2;
-        const int n_live = __popc(__ballot_sync(0xffffffffu, live) & 0xfu);
+        float* info = infos + (st * GT + w) * kInfoFloats;
+        const int role = lane / GT;
+        const int n_live = __popc(__ballot_sync(0xffffffffu, live) & ((1u << GT) - 1u));
         // the bytes are announced and asked for; the stage is handed over below, with the scales
         if (lane == 0) mbar_announce(full(st), (uint32_t)(n_live * (2 * TILE + (a.gc ? 64 : 0))));
         __syncwarp();
         if (live) {
-          const uint32_t kd = smem_u32(ring + st * STAGE + w * TILE), vd = kd + kDecWarps * TILE;
+          const uint32_t kd = smem_u32(ring + st * STAGE + w * TILE), vd = kd + GT * TILE;
           if (role == 0) tma_load_3d(kd, &tm_k, 0, row0, (int)ph, full(st));
           if (role == 1) tma_load_3d(vd, &tm_v, 0, row0, (int)ph, full(st));
           if (role == 2 && a.gc) bulk_load(smem_u32(info), a.gc + (ph << a.page_shift) + row0, 64, full(st));
           if (D == 256 && role == 4) tma_load_3d(kd + 2048, &tm_k, 128, row0, (int)ph, full(st));
           if (D == 256 && role == 5) tma_load_3d(vd + 2048, &tm_v, 128, row0, (int)ph, full(st));
         }
-        const float mk = __shfl_sync(0xffffffffu, ksc, 4 * in + w), mv = __shfl_sync(0xffffffffu, vsc, 4 * in + w);
+        const float mk = __shfl_sync(0xffffffffu, ksc, GT * in + w), mv = __shfl_sync(0xffffffffu, vsc, GT * in + w);
         if (role == 3) info[16] = mk, info[17] = mv, info[18] = live ? 1.f : 0.f;
         __syncwarp();
         if (lane == 0) mbar_arrive(full(st));
@@ -411,73 +418,84 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas_per_sm<D, NG>())
 #pragma unroll
       for (int i = 0; i < MT; ++i) o[x][i][0] = o[x][i][1] = o[x][i][2] = o[x][i][3] = 0.f;
     }
-    for (int t = sg.first; t < sg.last; t += kDecWarps, ++step) {
+    for (int t = sg.first; t < sg.last; t += GT, ++step) {
       const int st = step % NST;
       if (!dead) dead = !__all_sync(0xffffffffu, mbar_wait_sleep(full(st), (step / NST) & 1, kSiteDecUse));
-      if (t + warp < sg.last) {
-      const uint8_t* kt = ring + st * STAGE + warp * TILE;
-      const uint8_t* vt = kt + kDecWarps * TILE;
-      const float* info = infos + (st * kDecWarps + warp) * kInfoFloats;
-      const int t0 = (t + warp) * 16 + lr, t1 = t0 + 8;
+      const int mine = warp * U;  // the warp's first tile of the stage
+      if (t + mine < sg.last) {  // (a tile past the last holds nothing that counts: its `live` is 0)
+      const uint8_t* kt = ring + st * STAGE + mine * TILE;
+      const uint8_t* vt = kt + GT * TILE;
+      const float* info = infos + (st * GT + mine) * kInfoFloats;
       // ---- S^T = K Q^T
-      float s[NG][4], s2[NG][4];
+      float s[U][NG][4], s2[U][NG][4];
 #pragma unroll
-      for (int x = 0; x < NG; ++x)
+      for (int u = 0; u < U; ++u) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[x][e] = s2[x][e] = 0.f;
-      uint32_t kw[2][KW];
+        for (int x = 0; x < NG; ++x)
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        if constexpr (D == 32) {
-          const uint2 w = *reinterpret_cast<const uint2*>(kt + tile_at<D>(lr + 8 * b, lc >> 1) + (lc & 1) * 8);
-          kw[b][0] = w.x, kw[b][1] = w.y;
-        } else {
+          for (int e = 0; e < 4; ++e) s[u][x][e] = s2[u][x][e] = 0.f;
+        const uint8_t* ku = kt + u * TILE;
+        uint32_t kw[2][KW];
 #pragma unroll
-          for (int j = 0; j < D / 64; ++j) {
-            const uint4 w = *reinterpret_cast<const uint4*>(kt + tile_at<D>(lr + 8 * b, lc + 4 * j));
-            kw[b][4 * j] = w.x, kw[b][4 * j + 1] = w.y, kw[b][4 * j + 2] = w.z, kw[b][4 * j + 3] = w.w;
+        for (int b = 0; b < 2; ++b) {
+          if constexpr (D == 32) {
+            const uint2 w = *reinterpret_cast<const uint2*>(ku + tile_at<D>(lr + 8 * b, lc >> 1) + (lc & 1) * 8);
+            kw[b][0] = w.x, kw[b][1] = w.y;
+          } else {
+#pragma unroll
+            for (int j = 0; j < D / 64; ++j) {
+              const uint4 w = *reinterpret_cast<const uint4*>(ku + tile_at<D>(lr + 8 * b, lc + 4 * j));
+              kw[b][4 * j] = w.x, kw[b][4 * j + 1] = w.y, kw[b][4 * j + 2] = w.z, kw[b][4 * j + 3] = w.w;
+            }
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < KW; ++k) {
+          uint32_t a0, a1, a2, a3;
+          expand4<C>(kw[0][k], a0, a2);
+          expand4<C>(kw[1][k], a1, a3);
+#pragma unroll
+          for (int x = 0; x < NG; ++x) {
+            mma16816(k & 1 ? s2[u][x] : s[u][x], a0, a1, a2, a3, qb[x][k][0], qb[x][k][1]);
+            if constexpr (SPLIT) mma16816(k & 1 ? s[u][x] : s2[u][x], a0, a1, a2, a3, ql[x][k][0], ql[x][k][1]);
           }
         }
       }
-#pragma unroll
-      for (int k = 0; k < KW; ++k) {
-        uint32_t a0, a1, a2, a3;
-        expand4<C>(kw[0][k], a0, a2);
-        expand4<C>(kw[1][k], a1, a3);
-#pragma unroll
-        for (int x = 0; x < NG; ++x) {
-          mma16816(k & 1 ? s2[x] : s[x], a0, a1, a2, a3, qb[x][k][0], qb[x][k][1]);
-          if constexpr (SPLIT) mma16816(k & 1 ? s[x] : s2[x], a0, a1, a2, a3, ql[x][k][0], ql[x][k][1]);
-        }
-      }
       // ---- scores in log2 units
-      const float ksc = info[16], vsc = info[17];
-      bool in0 = t0 < n, in1 = t1 < n;
-      float g0 = 0.f, g1 = 0.f;
-      if (a.gc) {
-        g0 = t0 < n - 1 ? info[lr] * kDecLog2e : 0.f;
-        g1 = t1 < n - 1 ? info[lr + 8] * kDecLog2e : 0.f;
-        in0 = in0 && g0 != -INFINITY;
-        in1 = in1 && g1 != -INFINITY;
-      }
-      const bool live = info[18] != 0.f;
-      in0 = in0 && live;
-      in1 = in1 && live;
-      bool grow = false;
+      bool in0[U], in1[U], grow = false;
+      float top = unit;
 #pragma unroll
-      for (int x = 0; x < NG; ++x)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float y = fmaf(s[x][e] + s2[x][e], qf[x][e & 1] * ksc, e < 2 ? g0 : g1);
-          s[x][e] = (e < 2 ? in0 : in1) ? y : -INFINITY;
-          grow |= s[x][e] > m[x][e & 1] + kGrow;
+      for (int u = 0; u < U; ++u) {
+        const float* iu = info + u * kInfoFloats;
+        const int t0 = (t + mine + u) * 16 + lr, t1 = t0 + 8;
+        const float ksc = iu[16];
+        top = fmaxf(top, iu[17]);
+        const bool live = iu[18] != 0.f;
+        in0[u] = live && t0 < n, in1[u] = live && t1 < n;
+        float g0 = 0.f, g1 = 0.f;
+        if (a.gc) {
+          g0 = t0 < n - 1 ? iu[lr] * kDecLog2e : 0.f;
+          g1 = t1 < n - 1 ? iu[lr + 8] * kDecLog2e : 0.f;
+          in0[u] = in0[u] && g0 != -INFINITY;
+          in1[u] = in1[u] && g1 != -INFINITY;
         }
+#pragma unroll
+        for (int x = 0; x < NG; ++x)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float y = fmaf(s[u][x][e] + s2[u][x][e], qf[x][e & 1] * ksc, e < 2 ? g0 : g1);
+            s[u][x][e] = (e < 2 ? in0[u] : in1[u]) ? y : -INFINITY;
+            grow |= s[u][x][e] > m[x][e & 1] + kGrow;
+          }
+      }
       if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
         for (int x = 0; x < NG; ++x)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float t = fmaxf(s[x][e], s[x][e + 2]);
+            float t = fmaxf(s[0][x][e], s[0][x][e + 2]);
+#pragma unroll
+            for (int u = 1; u < U; ++u) t = fmaxf(t, fmaxf(s[u][x][e], s[u][x][e + 2]));
             t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 4));
             t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 8));
             t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 16));
@@ -490,9 +508,9 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas_per_sm<D, NG>())
             for (int i = 0; i < MT; ++i) o[x][i][e] *= f, o[x][i][e + 2] *= f;
           }
       }
-      if (vsc > unit) {
-        const float f = unit / vsc;
-        unit = vsc;
+      if (top > unit) {
+        const float f = unit / top;
+        unit = top;
 #pragma unroll
         for (int x = 0; x < NG; ++x)
 #pragma unroll
@@ -500,71 +518,78 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas_per_sm<D, NG>())
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[x][i][e] *= f;
       }
-      const float ratio = unit > 0.f ? __fdividef(vsc, unit) : 0.f;
-      // ---- P, as the B operand of O^T (heads as columns, tokens as the contraction)
-      uint32_t pb[NG][2], pl[SPLIT ? NG : 1][2];
+      float m_of[NG][2];
 #pragma unroll
-      for (int x = 0; x < NG; ++x) {
-        const float m0 = m[x][0] == -INFINITY ? 0.f : m[x][0] - kOffset;
-        const float m1 = m[x][1] == -INFINITY ? 0.f : m[x][1] - kOffset;
-        float p[4];
+      for (int x = 0; x < NG; ++x)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) p[e] = dec_ex2(s[x][e] - (e & 1 ? m1 : m0));
-        l[x][0] += p[0] + p[2];
-        l[x][1] += p[1] + p[3];
+        for (int e = 0; e < 2; ++e) m_of[x][e] = m[x][e] == -INFINITY ? 0.f : m[x][e] - kOffset;
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
-          const float p0 = p[2 * b] * ratio, p1 = p[2 * b + 1] * ratio;
-          const uint32_t w = half2_bits(p0, p1);
-          pb[x][b] = transpose8x8(w);
-          if constexpr (SPLIT) {
-            const float2 hi = __half22float2(*reinterpret_cast<const __half2*>(&w));
-            pl[x][b] = transpose8x8(half2_bits(p0 - hi.x, p1 - hi.y));
+      for (int u = 0; u < U; ++u) {
+        const uint8_t* vu = vt + u * TILE;
+        const float ratio = unit > 0.f ? __fdividef(info[u * kInfoFloats + 17], unit) : 0.f;
+        // ---- P, as the B operand of O^T (heads as columns, tokens as the contraction)
+        uint32_t pb[NG][2], pl[SPLIT ? NG : 1][2];
+#pragma unroll
+        for (int x = 0; x < NG; ++x) {
+          float p[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) p[e] = dec_ex2(s[u][x][e] - m_of[x][e & 1]);
+          l[x][0] += p[0] + p[2];
+          l[x][1] += p[1] + p[3];
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+            const float p0 = p[2 * b] * ratio, p1 = p[2 * b + 1] * ratio;
+            const uint32_t w = half2_bits(p0, p1);
+            pb[x][b] = transpose8x8(w);
+            if constexpr (SPLIT) {
+              const float2 hi = __half22float2(*reinterpret_cast<const __half2*>(&w));
+              pl[x][b] = transpose8x8(half2_bits(p0 - hi.x, p1 - hi.y));
+            }
           }
         }
-      }
-      // ---- O^T += V^T P^T
-      uint32_t vw[4][VWORDS];  // tokens 2 lc, 2 lc + 1, 2 lc + 8, 2 lc + 9
+        // ---- O^T += V^T P^T
+        uint32_t vw[4][VWORDS];  // tokens 2 lc, 2 lc + 1, 2 lc + 8, 2 lc + 9
 #pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        const int row = 2 * lc + (b & 1) + (b >> 1) * 8;
-        if constexpr (D == 32) {
-          vw[b][0] = *reinterpret_cast<const uint32_t*>(vt + tile_at<D>(row, lr >> 2) + (lr & 3) * 4);
-        } else if constexpr (D == 64) {
-          const uint2 w = *reinterpret_cast<const uint2*>(vt + tile_at<D>(row, lr >> 1) + (lr & 1) * 8);
-          vw[b][0] = w.x, vw[b][1] = w.y;
-        } else {
+        for (int b = 0; b < 4; ++b) {
+          const int row = 2 * lc + (b & 1) + (b >> 1) * 8;
+          if constexpr (D == 32) {
+            vw[b][0] = *reinterpret_cast<const uint32_t*>(vu + tile_at<D>(row, lr >> 2) + (lr & 3) * 4);
+          } else if constexpr (D == 64) {
+            const uint2 w = *reinterpret_cast<const uint2*>(vu + tile_at<D>(row, lr >> 1) + (lr & 1) * 8);
+            vw[b][0] = w.x, vw[b][1] = w.y;
+          } else {
 #pragma unroll
-          for (int j = 0; j < D / 128; ++j) {
-            const uint4 w = *reinterpret_cast<const uint4*>(vt + tile_at<D>(row, lr + 8 * j));
-            vw[b][4 * j] = w.x, vw[b][4 * j + 1] = w.y, vw[b][4 * j + 2] = w.z, vw[b][4 * j + 3] = w.w;
+            for (int j = 0; j < D / 128; ++j) {
+              const uint4 w = *reinterpret_cast<const uint4*>(vu + tile_at<D>(row, lr + 8 * j));
+              vw[b][4 * j] = w.x, vw[b][4 * j + 1] = w.y, vw[b][4 * j + 2] = w.z, vw[b][4 * j + 3] = w.w;
+            }
           }
         }
-      }
-      if constexpr (std::is_same<C, E4M3>::value) {
-        // a NaN code of a token that does not count must not meet its zero weight
-        const unsigned b0 = __ballot_sync(0xffffffffu, in0), b1 = __ballot_sync(0xffffffffu, in1);
-        if ((b0 & b1) != 0xffffffffu) {
+        if constexpr (std::is_same<C, E4M3>::value) {
+          // a NaN code of a token that does not count must not meet its zero weight
+          const unsigned b0 = __ballot_sync(0xffffffffu, in0[u]), b1 = __ballot_sync(0xffffffffu, in1[u]);
+          if ((b0 & b1) != 0xffffffffu) {
 #pragma unroll
-          for (int b = 0; b < 4; ++b) {
-            const bool in = ((b < 2 ? b0 : b1) >> (4 * (2 * lc + (b & 1)))) & 1u;
+            for (int b = 0; b < 4; ++b) {
+              const bool in = ((b < 2 ? b0 : b1) >> (4 * (2 * lc + (b & 1)))) & 1u;
 #pragma unroll
-            for (int j = 0; j < VWORDS; ++j) vw[b][j] = in ? vw[b][j] : 0u;
+              for (int j = 0; j < VWORDS; ++j) vw[b][j] = in ? vw[b][j] : 0u;
+            }
           }
         }
-      }
 #pragma unroll
-      for (int j = 0; j < VWORDS; ++j) {
+        for (int j = 0; j < VWORDS; ++j) {
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const uint32_t sel = half ? 0x7362 : 0x5140;
-          uint32_t a0, a1, a2, a3;
-          expand4<C>(__byte_perm(vw[0][j], vw[1][j], sel), a0, a1);
-          expand4<C>(__byte_perm(vw[2][j], vw[3][j], sel), a2, a3);
+          for (int half = 0; half < 2; ++half) {
+            const uint32_t sel = half ? 0x7362 : 0x5140;
+            uint32_t a0, a1, a2, a3;
+            expand4<C>(__byte_perm(vw[0][j], vw[1][j], sel), a0, a1);
+            expand4<C>(__byte_perm(vw[2][j], vw[3][j], sel), a2, a3);
 #pragma unroll
-          for (int x = 0; x < NG; ++x) {
-            mma16816(o[x][2 * j + half], a0, a1, a2, a3, pb[x][0], pb[x][1]);
-            if constexpr (SPLIT) mma16816(o[x][2 * j + half], a0, a1, a2, a3, pl[x][0], pl[x][1]);
+            for (int x = 0; x < NG; ++x) {
+              mma16816(o[x][2 * j + half], a0, a1, a2, a3, pb[x][0], pb[x][1]);
+              if constexpr (SPLIT) mma16816(o[x][2 * j + half], a0, a1, a2, a3, pl[x][0], pl[x][1]);
+            }
           }
         }
       }
