@@ -9,8 +9,8 @@
 // query heads that share it, so it should run at the memory's rate. What decides that is the
 // work between a code's arrival and its product; this layout keeps it low:
 //   - one warp of a CTA fetches (TMA, 16 tokens of K or V a box, a ring of stages of 64 tokens), four
-//     warps compute, 16 tokens of a stage each; the fetching warp runs ahead from one request to the
-//     next, so that memory stays busy where the others join their results;
+//     warps compute, 16 tokens of a stage each (32 of 128 for head_dim up to 64); the fetching warp runs
+//     ahead from one request to the next, so that memory stays busy where the others join their results;
 //   - both products are m16n8k16 tensor-core products with the codes as the 16-row operand A and
 //     up to 8 query heads as the 8 columns: S^T = K Q^T has tokens as rows, O^T = V^T P^T has
 //     dimensions as rows, so heads pad to 8 and not to 16 (tcgen05 would pad them to 16 columns too,
@@ -25,7 +25,7 @@
 //     P relative to the largest one the warp has met (O is rescaled when that grows).
 // Measured: 64 requests of 1 to 8192 tokens (int8, 32 heads on 8 of 128, 547 MB) 106 us a step, 5.1 TB/s, of which 6.2
 // in the steady state; one of 131071 tokens (e4m3, 32 heads on 4, 134 MB) 34 us; 24 of 1 to 4097 tokens (fp32
-// queries, 24 heads of 64 with gates, 165 MB) 55 us, there bound by instructions: one query head fills an
+// queries, 24 heads of 64 with gates, 165 MB) 51 us, there bound by instructions: one query head fills an
 // eighth of each product.
 // Roundings: fp32 accumulation, softmax statistics and O. P is rounded to fp16 (2^-11 of itself),
 // offset by 2^7 so that products down to 2^-21 of the row's largest keep all bits. q enters
@@ -52,7 +52,6 @@ constexpr int kMinTiles = 8;                        // 16-token tiles that a CTA
 constexpr int kEachTiles = 32;                      // see decode_launch
 constexpr int kStart = 8;                           // a row group's start and join, in tiles' time (see below)
 constexpr unsigned int kSiteDecLoad = 0x401, kSiteDecUse = 0x402;
-constexpr int kS64 = 2;
 constexpr float kDecLog2e = 1.4426950408889634f;
 constexpr float kGrow = 8.0f;      // log2: O is rescaled when a row's maximum grows by more
 constexpr float kOffset = 7.0f;    // log2: P = 2^(s - m + 7) <= 2^15
@@ -107,11 +106,13 @@ template <int D> __device__ __forceinline__ int tile_at(int row, int ch) {
   return row * 32 + ((ch ^ ((row >> 2) & 1)) << 4);
 }
 
-// 16-token tiles that a warp takes in one step.
+// 16-token tiles that a warp takes in one step: two where a tile's work is short next to what a step costs
+// anyway (24 requests of up to 4097 tokens, 24 heads of 64: 53 us instead of 59 with cold caches; four stages
+// at three CTAs an SM instead of two at four: 55).
 template <int D, int NG> constexpr int dec_unroll() { return D <= 64 && NG == 1 ? 2 : 1; }
 template <int D, int NG> constexpr int dec_stage_tiles() { return kDecWarps * dec_unroll<D, NG>(); }
 template <int D, int NG> constexpr int dec_stages() {
-  return D == 256 ? 2 : (D == 128 ? 3 : (D == 64 && NG == 1 ? kS64 : 4));
+  return D == 256 ? 2 : (D == 128 ? 3 : (D == 64 && NG == 1 ? 2 : 4));
 }
 template <int D, int NG> constexpr int dec_stage_bytes() { return dec_stage_tiles<D, NG>() * 32 * D; }  // K, V tiles
 constexpr int kInfoFloats = 24;                                                  // 16 gates, k_scale, v_scale, live
