@@ -697,7 +697,7 @@ int paged_cache(const sattn_cache* c, PagedCache* o) {
 
 bool decode_geometry_ok(const PagedCache& c, int64_t requests, int64_t width, int64_t nheads) {
   return requests > 0 && requests <= 0x7fffffffll && width > 0 && nheads > 0 && nheads <= 65535 &&
-         nheads % c.nkv == 0 && width * c.page <= 0x7fffffffll;
+         nheads % c.nkv == 0 && width <= 0x7fffffffll / c.page;
 }
 
 }  // namespace
@@ -709,9 +709,10 @@ int sattn_paged_plan(const int32_t* lengths, const int32_t* new_lengths, int32_t
                      int64_t* slots, int32_t* positions, int64_t* free_state_out, int64_t requests,
                      int64_t table_width, int64_t num_free, int64_t num_tokens, int64_t page_size, void* stream) {
   if (requests < 0 || table_width < 0 || num_free < 0 || num_tokens < 0 || requests > 0x7fffffffll ||
-      num_tokens > 0x7fffffffll || table_width * page_size > 0x7fffffffll || num_free > 0x7fffffffll)
+      num_tokens > 0x7fffffffll || num_free > 0x7fffffffll)
     return SSD_ERR_INVALID_ARGUMENT;
   if (page_size != 16 && page_size != 32 && page_size != 64 && page_size != 128) return SSD_ERR_INVALID_ARGUMENT;
+  if (table_width > 0x7fffffffll / page_size) return SSD_ERR_INVALID_ARGUMENT;
   if (!free_state || !free_state_out || !cu_new || (num_tokens && (!slots || !positions)) ||
       (requests && (!lengths || !new_lengths || !lengths_out || (table_width && !block_table))) ||
       (num_free && !free_pages))

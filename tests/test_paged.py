@@ -96,6 +96,18 @@ def test_structs_match_the_header():
             assert getattr(cls, f).offset == off, f
 
 
+def test_widths_whose_product_with_the_page_wraps_are_refused():
+    from selective_attention_b200 import _lib
+
+    L, bad = _lib.lib(), _lib.SSD_ERR_INVALID_ARGUMENT
+    c = ctypes.byref(_lib.SattnCache(num_pages=4, nkv=2, page_size=16, head_dim=64, code=0, k_codes=4096, v_codes=4096,
+                                     k_scale=4096, v_scale=4096, log_gate=None))
+    for width in (1 << 31, 1 << 60, (1 << 62) + 1):
+        assert L.sattn_paged_plan(*[4096] * 10, 1, width, 4, 1, 16, None) == bad, width
+        assert L.sattn_paged_decode(c, 4096, 4096, 4096, 4096, 1, width, 2, 1.0, 1, 4096, 1 << 40, None) == bad, width
+        assert L.sattn_paged_decode_workspace_size(c, 1, width, 2) == 0, width
+
+
 def test_cpu_tensors_are_refused():
     import selective_attention_b200 as sab
 
