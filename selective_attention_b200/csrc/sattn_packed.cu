@@ -19,11 +19,34 @@
 namespace ssdb200 {
 namespace {
 
+// Packed fp32 pairs.
+__device__ __forceinline__ uint64_t pk2(float a, float b) {
+  return (uint64_t)__float_as_uint(a) | ((uint64_t)__float_as_uint(b) << 32);
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ float lo2(uint64_t x) { return __uint_as_float((uint32_t)x); }
+__device__ __forceinline__ float hi2(uint64_t x) { return __uint_as_float((uint32_t)(x >> 32)); }
+
 // ===========================================================================
 // CUDA-core kernel (fp32, and head_dim 16 or 32): CTA = (query head, 64-query tile of a sequence),
 // 64-key tiles of K and V staged in shared memory as fp32; thread (tr, tc) owns rows tr + 16 i
-// (i < 4), score columns tc + 16 j, output columns 4 tc + 64 g (g < 2). Bound by FFMA.
+// (i < 4), score columns tc + 16 j, output columns 4 tc + 64 g (g < D / 64). Two products an
+// instruction (fp32 pairs). Bound by those and by the shared-memory reads that feed them. At head_dim 128
+// V takes K's place once the scores are there, so that two CTAs fit an SM.
 // ===========================================================================
+template <int D> constexpr bool simt_share() { return D == 128; }
+template <int D> constexpr size_t simt_smem() {
+  return (size_t)((simt_share<D>() ? 2 : 3) * kPT * (D + 4) + kPT * (kPT + 4) + kPT) * sizeof(float);
+}
 template <typename T>
 __device__ __forceinline__ void stage64(float* dst, int ld, const T* src, long long stride, int rows, int D) {
   const int vpr = D >> 3, nv = kPT * vpr;
@@ -41,26 +64,26 @@ __device__ __forceinline__ void stage64(float* dst, int ld, const T* src, long l
   }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(256) sattn_packed_kernel(const T* __restrict__ q, const T* __restrict__ k,
+template <typename T, int D>
+__global__ void __launch_bounds__(256, 2) sattn_packed_kernel(const T* __restrict__ q, const T* __restrict__ k,
                                                            const T* __restrict__ v, const float* __restrict__ lg,
                                                            const int* __restrict__ cu, T* __restrict__ out, int R,
-                                                           int Tn, int Hq, int Hk, int D, PackedStrides st,
+                                                           int Tn, int Hq, int Hk, PackedStrides st,
                                                            float scale) {
   extern __shared__ float4 smem4[];
   __shared__ PackedTile s_tile;
   float* sm = reinterpret_cast<float*>(smem4);
-  const int LD = D + 4, LDP = kPT + 4;
+  constexpr int LD = D + 4, LDP = kPT + 4, G = D > 64 ? 2 : 1;
   float* Qs = sm;
   float* Ks = Qs + kPT * LD;
-  float* Vs = Ks + kPT * LD;
+  float* Vs = simt_share<D>() ? Ks : Ks + kPT * LD;
   float* Ps = Vs + kPT * LD;
   float* gs = Ps + kPT * LDP;
   const int tid = threadIdx.x, tr = tid >> 4, tc = tid & 15;
   if (tid < 32) {
     PackedFinder<6> finder;
     finder.init(cu, R, Tn);
-    const PackedTile t = finder.find((int)blockIdx.y);
+    const PackedTile t = finder.find((int)(gridDim.y - 1 - blockIdx.y));  // the last tiles of a sequence have most keys
     if (tid == 0) s_tile = t;
   }
   __syncthreads();
@@ -75,47 +98,49 @@ __global__ void __launch_bounds__(256) sattn_packed_kernel(const T* __restrict__
   const int q0 = tile.q0, n = tile.n;
   const long long base = tile.tok0 - q0;  // the sequence's first token
   stage64<T>(Qs, LD, q + (long long)tile.tok0 * st.q_ts + hq * st.q_hs, st.q_ts, tile.rows, D);
-  float o[4][8], m[4], l[4];
+  uint64_t o[4][2 * G];
+  float m[4], l[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     m[i] = -INFINITY;
     l[i] = 0.f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) o[i][e] = 0.f;
+    for (int e = 0; e < 2 * G; ++e) o[i][e] = 0;
   }
-  int dcol[2];
+  int dcol[G];
 #pragma unroll
-  for (int g = 0; g < 2; ++g) dcol[g] = min(4 * tc + 64 * g, D - 4);
+  for (int g = 0; g < G; ++g) dcol[g] = min(4 * tc + 64 * g, D - 4);
   const int qt = q0 / kPT;
   for (int kt = 0; kt <= qt; ++kt) {
     const int k0 = kt * kPT;
     __syncthreads();  // previous tile's K, V, P consumed
     stage64<T>(Ks, LD, k + (base + k0) * st.k_ts + hk * st.k_hs, st.k_ts, min(kPT, n - k0), D);
-    stage64<T>(Vs, LD, v + (base + k0) * st.v_ts + hk * st.v_hs, st.v_ts, min(kPT, n - k0), D);
+    if constexpr (!simt_share<D>())
+      stage64<T>(Vs, LD, v + (base + k0) * st.v_ts + hk * st.v_hs, st.v_ts, min(kPT, n - k0), D);
     if (tid < kPT) gs[tid] = lg && k0 + tid < n ? lg[(base + k0 + tid) * Hk + hk] : 0.f;
     __syncthreads();
+    uint64_t s2[4][4];  // sums over even and over odd dimensions
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s2[i][j] = 0;
+#pragma unroll 4
+    for (int d = 0; d < D; d += 4) {
+      ulonglong2 a[4], b[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) a[i] = *reinterpret_cast<const ulonglong2*>(Qs + (tr + 16 * i) * LD + d);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) b[j] = *reinterpret_cast<const ulonglong2*>(Ks + (tc + 16 * j) * LD + d);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s2[i][j] = fma2(a[i].y, b[j].y, fma2(a[i].x, b[j].x, s2[i][j]));
+    }
     float sc[4][4];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) sc[i][j] = 0.f;
-    for (int d = 0; d < D; d += 4) {
-      float4 a[4], b[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) a[i] = *reinterpret_cast<const float4*>(Qs + (tr + 16 * i) * LD + d);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) b[j] = *reinterpret_cast<const float4*>(Ks + (tc + 16 * j) * LD + d);
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          float t = sc[i][j];
-          t = fmaf(a[i].x, b[j].x, t);
-          t = fmaf(a[i].y, b[j].y, t);
-          t = fmaf(a[i].z, b[j].z, t);
-          sc[i][j] = fmaf(a[i].w, b[j].w, t);
-        }
-    }
+      for (int j = 0; j < 4; ++j) sc[i][j] = lo2(s2[i][j]) + hi2(s2[i][j]);
     bool skip = false;  // some row of this thread's half warp does not see some key of the tile
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -143,35 +168,44 @@ __global__ void __launch_bounds__(256) sattn_packed_kernel(const T* __restrict__
       }
       l[i] = l[i] * corr + hw_sum(rs);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) o[i][e] *= corr;
+      for (int e = 0; e < 2 * G; ++e) o[i][e] = pk2(lo2(o[i][e]) * corr, hi2(o[i][e]) * corr);
       m[i] = mn;
     }
     // a key that a row does not see is left out of its product, not multiplied by zero
     skip = __syncthreads_or(skip);
+    if constexpr (simt_share<D>()) {  // (every score has been computed)
+      stage64<T>(Vs, LD, v + (base + k0) * st.v_ts + hk * st.v_hs, st.v_ts, min(kPT, n - k0), D);
+      __syncthreads();
+    }
+    auto pv = [&](auto leave_out) {
 #pragma unroll 2
-    for (int j = 0; j < kPT; j += 4) {
-      float4 pa[4];
+      for (int j = 0; j < kPT; j += 4) {
+        float4 pa[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) pa[i] = *reinterpret_cast<const float4*>(Ps + (tr + 16 * i) * LDP + j);
+        for (int i = 0; i < 4; ++i) pa[i] = *reinterpret_cast<const float4*>(Ps + (tr + 16 * i) * LDP + j);
 #pragma unroll
-      for (int qq = 0; qq < 4; ++qq) {
-        float4 vv[2];
+        for (int qq = 0; qq < 4; ++qq) {
+          ulonglong2 vv[G];
 #pragma unroll
-        for (int g = 0; g < 2; ++g) vv[g] = *reinterpret_cast<const float4*>(Vs + (j + qq) * LD + dcol[g]);
+          for (int g = 0; g < G; ++g) vv[g] = *reinterpret_cast<const ulonglong2*>(Vs + (j + qq) * LD + dcol[g]);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float p = qq == 0 ? pa[i].x : (qq == 1 ? pa[i].y : (qq == 2 ? pa[i].z : pa[i].w));
-          if (skip && p == 0.f) continue;
+          for (int i = 0; i < 4; ++i) {
+            const float p = qq == 0 ? pa[i].x : (qq == 1 ? pa[i].y : (qq == 2 ? pa[i].z : pa[i].w));
+            const uint64_t pp = pk2(p, p);
+            const bool out = decltype(leave_out)::value && p == 0.f;
 #pragma unroll
-          for (int g = 0; g < 2; ++g) {
-            o[i][4 * g] = fmaf(p, vv[g].x, o[i][4 * g]);
-            o[i][4 * g + 1] = fmaf(p, vv[g].y, o[i][4 * g + 1]);
-            o[i][4 * g + 2] = fmaf(p, vv[g].z, o[i][4 * g + 2]);
-            o[i][4 * g + 3] = fmaf(p, vv[g].w, o[i][4 * g + 3]);
+            for (int g = 0; g < G; ++g) {
+              o[i][2 * g] = fma2(pp, out ? 0 : vv[g].x, o[i][2 * g]);
+              o[i][2 * g + 1] = fma2(pp, out ? 0 : vv[g].y, o[i][2 * g + 1]);
+            }
           }
         }
       }
-    }
+    };
+    if (skip)
+      pv(std::true_type{});
+    else
+      pv(std::false_type{});
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -179,27 +213,39 @@ __global__ void __launch_bounds__(256) sattn_packed_kernel(const T* __restrict__
     if (ri >= tile.rows) continue;
     const float inv = 1.0f / l[i];
 #pragma unroll
-    for (int g = 0; g < 2; ++g) {
+    for (int g = 0; g < G; ++g) {
       const int d = 4 * tc + 64 * g;
       if (d >= D) continue;
       T* op = ob + (long long)ri * Hq * D + d;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) op[e] = from_f32<T>(o[i][4 * g + e] * inv);
+      for (int e = 0; e < 4; ++e) op[e] = from_f32<T>((e & 1 ? hi2(o[i][2 * g + (e >> 1)]) : lo2(o[i][2 * g + (e >> 1)])) * inv);
     }
   }
 }
 
-template <typename T>
-cudaError_t packed_simt_t(const PackedArgs& a, cudaStream_t s) {
-  const size_t smem = (size_t)(3 * kPT * (a.D + 4) + kPT * (kPT + 4) + kPT) * sizeof(float);
-  cudaError_t e = cudaFuncSetAttribute(sattn_packed_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+template <typename T, int D>
+cudaError_t packed_simt_d(const PackedArgs& a, cudaStream_t s) {
+  constexpr size_t smem = simt_smem<D>();
+  static unsigned long long allowed = 0;
+  cudaError_t e = allow_smem(sattn_packed_kernel<T, D>, smem, allowed);
   if (e != cudaSuccess) return e;
   const long long tiles = packed_tile_bound(a.T, a.R, kPT);
   if (tiles > 65535) return cudaErrorInvalidValue;
   dim3 grid((unsigned)a.Hq, (unsigned)tiles);
-  sattn_packed_kernel<T><<<grid, 256, smem, s>>>((const T*)a.q, (const T*)a.k, (const T*)a.v, a.log_gate, a.cu,
-                                                 (T*)a.out, a.R, a.T, a.Hq, a.Hk, a.D, a.st, a.scale);
+  sattn_packed_kernel<T, D><<<grid, 256, smem, s>>>((const T*)a.q, (const T*)a.k, (const T*)a.v, a.log_gate, a.cu,
+                                                    (T*)a.out, a.R, a.T, a.Hq, a.Hk, a.st, a.scale);
   return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t packed_simt_t(const PackedArgs& a, cudaStream_t s) {
+  switch (a.D) {
+    case 16: return packed_simt_d<T, 16>(a, s);
+    case 32: return packed_simt_d<T, 32>(a, s);
+    case 64: return packed_simt_d<T, 64>(a, s);
+    case 128: return packed_simt_d<T, 128>(a, s);
+  }
+  return cudaErrorInvalidValue;
 }
 
 // ===========================================================================
@@ -256,22 +302,6 @@ __device__ __forceinline__ float pk_ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// Packed fp32 pairs.
-__device__ __forceinline__ uint64_t pk2(float a, float b) {
-  return (uint64_t)__float_as_uint(a) | ((uint64_t)__float_as_uint(b) << 32);
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ float lo2(uint64_t x) { return __uint_as_float((uint32_t)x); }
-__device__ __forceinline__ float hi2(uint64_t x) { return __uint_as_float((uint32_t)(x >> 32)); }
 // A wait for warps that mostly wait: suspended in the barrier, so that they take neither issue slots nor
 // power from the others. Bounded by the number of waits, each of at most about 10 us.
 __device__ __forceinline__ bool idle_wait(uint32_t bar, uint32_t parity, unsigned int site) {
