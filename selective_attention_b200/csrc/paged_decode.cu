@@ -22,13 +22,15 @@
 //     consecutive dimensions of V for eight row pairs: shared memory is read with 16-byte loads,
 //     K never needs a transposition and V needs one byte permute for each four codes;
 //   - the page scales stay outside the products: k_scale multiplies the fp32 scores; v_scale enters
-//     P relative to the largest one the warp has met (O is rescaled when that grows).
+//     P. What P must not exceed is therefore 2^s v_scale, whose largest power of two a warp follows for each
+//     head apart from that of 2^s: a page whose values are large takes no bits from the others where
+//     its keys have no weight or are dropped.
 // Measured: 64 requests of 1 to 8192 tokens (int8, 32 heads on 8 of 128, 547 MB) 106 us a step, 5.1 TB/s, of which 6.2
 // in the steady state; one of 131071 tokens (e4m3, 32 heads on 4, 134 MB) 34 us; 24 of 1 to 4097 tokens (fp32
 // queries, 24 heads of 64 with gates, 165 MB) 51 us, there bound by instructions: one query head fills an
 // eighth of each product.
 // Roundings: fp32 accumulation, softmax statistics and O. P is rounded to fp16 (2^-11 of itself),
-// offset by 2^7 so that products down to 2^-21 of the row's largest keep all bits. q enters
+// offset by 2^7 so that 2^s v_scale down to 2^-21 of the head's largest keeps all bits. q enters
 // as fp16 after scaling its row by a power of two, which is exact for fp16 and for bf16 (8 bits)
 // down to 2^-29 of the row's largest element; an fp32 q and its P are split into two fp16 parts (22 bits).
 #include <math.h>
@@ -53,8 +55,9 @@ constexpr int kEachTiles = 32;                      // see decode_launch
 constexpr int kStart = 8;                           // a row group's start and join, in tiles' time (see below)
 constexpr unsigned int kSiteDecLoad = 0x401, kSiteDecUse = 0x402;
 constexpr float kDecLog2e = 1.4426950408889634f;
-constexpr float kGrow = 8.0f;      // log2: O is rescaled when a row's maximum grows by more
-constexpr float kOffset = 7.0f;    // log2: P = 2^(s - m + 7) <= 2^15
+constexpr float kGrow = 8.0f;      // log2: a head's maxima are followed when one grows by more
+constexpr float kOffset = 7.0f;    // log2: P = 2^(s - mv + 7) * v_scale <= 2^15
+constexpr float kNone = -3e38f;    // a maximum before the first key (finite: 2^(kNone - kNone) is 1, of nothing)
 
 __device__ __forceinline__ float dec_ex2(float x) {
   float y;
@@ -69,6 +72,14 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// The smaller one; NaN if either is.
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float y;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+// The exponent of the power of two above |x| (finite, whatever x is).
+__device__ __forceinline__ float above(float x) { return (float)((int)((__float_as_uint(x) >> 23) & 0xffu) - 126); }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t y;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -411,10 +422,12 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas_per_sm<D, NG>())
       qf[x][1] = __shfl_sync(0xffffffffu, f, (2 * lc + 1) * 4);
     }
 
-    float o[NG][MT][4], m[NG][2], l[NG][2], unit = 0.f;  // O in units of the v_scale `unit`
+    // By head, in log2: m, the largest s, l in units of 2^m; mv, the largest s + log2(v_scale) (rounded up), O in units
+    // of 2^mv.
+    float o[NG][MT][4], m[NG][2], l[NG][2], mv[NG][2];
 #pragma unroll
     for (int x = 0; x < NG; ++x) {
-      m[x][0] = m[x][1] = -INFINITY;
+      m[x][0] = m[x][1] = mv[x][0] = mv[x][1] = kNone;
       l[x][0] = l[x][1] = 0.f;
 #pragma unroll
       for (int i = 0; i < MT; ++i) o[x][i][0] = o[x][i][1] = o[x][i][2] = o[x][i][3] = 0.f;
@@ -464,13 +477,11 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas_per_sm<D, NG>())
       }
       // ---- scores in log2 units
       bool in0[U], in1[U], grow = false;
-      float top = unit;
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const float* iu = info + u * kInfoFloats;
         const int t0 = (t + mine + u) * 16 + lr, t1 = t0 + 8;
         const float ksc = iu[16];
-        top = fmaxf(top, iu[17]);
         const bool live = iu[18] != 0.f;
         in0[u] = live && t0 < n, in1[u] = live && t1 < n;
         float g0 = 0.f, g1 = 0.f;
@@ -480,13 +491,14 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas_per_sm<D, NG>())
           in0[u] = in0[u] && g0 != -INFINITY;
           in1[u] = in1[u] && g1 != -INFINITY;
         }
+        const float lv = above(iu[17]);
 #pragma unroll
         for (int x = 0; x < NG; ++x)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const float y = fmaf(s[u][x][e] + s2[u][x][e], qf[x][e & 1] * ksc, e < 2 ? g0 : g1);
             s[u][x][e] = (e < 2 ? in0[u] : in1[u]) ? y : -INFINITY;
-            grow |= s[u][x][e] > m[x][e & 1] + kGrow;
+            grow |= s[u][x][e] > fminf(m[x][e & 1], mv[x][e & 1] - lv) + kGrow;
           }
       }
       if (__any_sync(0xffffffffu, grow)) {
@@ -494,52 +506,49 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas_per_sm<D, NG>())
         for (int x = 0; x < NG; ++x)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float t = fmaxf(s[0][x][e], s[0][x][e + 2]);
+            float t = fmaxf(s[0][x][e], s[0][x][e + 2]), y = t + above(info[17]);
 #pragma unroll
-            for (int u = 1; u < U; ++u) t = fmaxf(t, fmaxf(s[u][x][e], s[u][x][e + 2]));
-            t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 4));
-            t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 8));
-            t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 16));
-            const float mn = fmaxf(m[x][e], t);
-            const float f = m[x][e] == -INFINITY ? 0.f : dec_ex2(m[x][e] - mn);
-            if (mn == m[x][e]) continue;  // (uniform over the lanes of a column: no collective below)
-            m[x][e] = mn;
-            l[x][e] *= f;
+            for (int u = 1; u < U; ++u) {
+              const float tu = fmaxf(s[u][x][e], s[u][x][e + 2]);
+              t = fmaxf(t, tu);
+              y = fmaxf(y, tu + above(info[u * kInfoFloats + 17]));
+            }
+#pragma unroll
+            for (int off = 4; off < 32; off <<= 1) {
+              t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, off));
+              y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, off));
+            }
+            t = fmaxf(t, m[x][e]);
+            y = fmaxf(y, mv[x][e]);
+            l[x][e] *= dec_ex2(m[x][e] - t);
+            const float f = dec_ex2(mv[x][e] - y);
+            m[x][e] = t;
+            mv[x][e] = y;
 #pragma unroll
             for (int i = 0; i < MT; ++i) o[x][i][e] *= f, o[x][i][e + 2] *= f;
           }
       }
-      if (top > unit) {
-        const float f = unit / top;
-        unit = top;
-#pragma unroll
-        for (int x = 0; x < NG; ++x)
-#pragma unroll
-          for (int i = 0; i < MT; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[x][i][e] *= f;
-      }
-      float m_of[NG][2];
-#pragma unroll
-      for (int x = 0; x < NG; ++x)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) m_of[x][e] = m[x][e] == -INFINITY ? 0.f : m[x][e] - kOffset;
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const uint8_t* vu = vt + u * TILE;
-        const float ratio = unit > 0.f ? __fdividef(info[u * kInfoFloats + 17], unit) : 0.f;
-        // ---- P, as the B operand of O^T (heads as columns, tokens as the contraction)
+        // ---- P, as the B operand of O^T (heads as columns, tokens as the contraction). The scale of a tile
+        // without a key that counts is nothing's (and may be an infinity or NaN); where r is past
+        // the range, P is next to nothing.
+        const unsigned b0 = __ballot_sync(0xffffffffu, in0[u]), b1 = __ballot_sync(0xffffffffu, in1[u]);
+        const float vs = (b0 | b1) != 0u ? info[u * kInfoFloats + 17] : 0.f;
         uint32_t pb[NG][2], pl[SPLIT ? NG : 1][2];
 #pragma unroll
         for (int x = 0; x < NG; ++x) {
+          const float r0 = min_nan(vs * dec_ex2(m[x][0] - mv[x][0]), 3e38f);
+          const float r1 = min_nan(vs * dec_ex2(m[x][1] - mv[x][1]), 3e38f);
           float p[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) p[e] = dec_ex2(s[u][x][e] - m_of[x][e & 1]);
+          for (int e = 0; e < 4; ++e) p[e] = dec_ex2(s[u][x][e] - (m[x][e & 1] - kOffset));
           l[x][0] += p[0] + p[2];
           l[x][1] += p[1] + p[3];
 #pragma unroll
           for (int b = 0; b < 2; ++b) {
-            const float p0 = p[2 * b] * ratio, p1 = p[2 * b + 1] * ratio;
+            const float p0 = p[2 * b] * r0, p1 = p[2 * b + 1] * r1;
             const uint32_t w = half2_bits(p0, p1);
             pb[x][b] = transpose8x8(w);
             if constexpr (SPLIT) {
@@ -568,7 +577,6 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas_per_sm<D, NG>())
         }
         if constexpr (std::is_same<C, E4M3>::value) {
           // a NaN code of a token that does not count must not meet its zero weight
-          const unsigned b0 = __ballot_sync(0xffffffffu, in0[u]), b1 = __ballot_sync(0xffffffffu, in1[u]);
           if ((b0 & b1) != 0xffffffffu) {
 #pragma unroll
             for (int b = 0; b < 4; ++b) {
@@ -607,8 +615,9 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas_per_sm<D, NG>())
         l[x][e] += __shfl_xor_sync(0xffffffffu, l[x][e], 4);
         l[x][e] += __shfl_xor_sync(0xffffffffu, l[x][e], 8);
         l[x][e] += __shfl_xor_sync(0xffffffffu, l[x][e], 16);
+        const float f = dec_ex2(mv[x][e] - m[x][e]);
 #pragma unroll
-        for (int i = 0; i < MT; ++i) o[x][i][e] *= unit, o[x][i][e + 2] *= unit;
+        for (int i = 0; i < MT; ++i) o[x][i][e] *= f, o[x][i][e + 2] *= f;
       }
     auto put = [&](float* to) {
       float4* p = reinterpret_cast<float4*>(to) + lane;
@@ -627,8 +636,8 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas_per_sm<D, NG>())
         const float4 ml = *p;
         p += 32;
         const float n0 = fmaxf(m[x][0], ml.x), n1 = fmaxf(m[x][1], ml.y);
-        const float f0 = m[x][0] == -INFINITY ? 0.f : dec_ex2(m[x][0] - n0), g0 = ml.x == -INFINITY ? 0.f : dec_ex2(ml.x - n0);
-        const float f1 = m[x][1] == -INFINITY ? 0.f : dec_ex2(m[x][1] - n1), g1 = ml.y == -INFINITY ? 0.f : dec_ex2(ml.y - n1);
+        const float f0 = dec_ex2(m[x][0] - n0), g0 = dec_ex2(ml.x - n0);
+        const float f1 = dec_ex2(m[x][1] - n1), g1 = dec_ex2(ml.y - n1);
         m[x][0] = n0, m[x][1] = n1;
         l[x][0] = l[x][0] * f0 + ml.z * g0;  // (a NaN stays one, also times 0)
         l[x][1] = l[x][1] * f1 + ml.w * g1;

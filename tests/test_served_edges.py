@@ -1,0 +1,94 @@
+"""Served selective attention where values, weights or lengths are far from ordinary, against
+``oracle/paged_ref.py``: page scales many orders apart.
+
+Tolerances are those of ``test_paged.py``: a share of the result for its own rounding
+and a share of the weighted magnitudes sum_j w_j |v_j| that the row adds up for the rounding of its weights, each of
+which is relative. Where one group of keys holds all the weight, that sum is at most the group's largest |v|.
+"""
+import math
+
+import pytest
+import torch
+
+from oracle import paged_ref
+
+INF = float("inf")
+NAN = float("nan")
+DECODE_TOL = {torch.bfloat16: (2 ** -8, 2 ** -10), torch.float16: (2 ** -10, 2 ** -10), torch.float32: (1e-5, 3e-5)}
+
+
+def close(got, ref, vmax, tol, what=""):
+    rel, p = tol[got.dtype]
+    got, ref = got.double().cpu(), ref.double().cpu()
+    assert torch.equal(got.isnan(), ref.isnan()), f"{what}: NaN in other places"
+    fine = ref.isfinite()
+    assert torch.equal(got[ref.isinf()], ref[ref.isinf()]), f"{what}: infinities"
+    err = (got - ref).abs()[fine]
+    bound = rel * ref.abs()[fine] + p * vmax
+    assert bool((err <= bound).all()), f"{what}: {int((err > bound).sum())} outside, max err {err.max().item():.3e}"
+
+
+# ----------------------------------------------------------------------------- decode: page scales
+def _two_kinds_of_pages(kind, high, pages=24, page=16, D=64, seed=0):
+    """A request whose pages are of two kinds in mixed order: first element of every key +1 or -1 (so that a
+    query along it weighs one kind e^(2 |q|) times the other), values of scale ``high`` where it is -1."""
+    g = torch.Generator().manual_seed(seed)
+    minus = torch.arange(pages) % 3 == 1
+    kc = torch.zeros(pages, 1, page, D)
+    kc[..., 0] = torch.where(minus, -64.0, 64.0)[:, None, None]
+    vc = (torch.rand(pages, 1, page, D, generator=g) * 2 - 1) * 96
+    if kind == torch.int8:
+        vc = vc.round()
+    vs = torch.where(minus, high, 1.0 / 96)[:, None].float()
+    c = dict(k_cache=kc.to(kind), v_cache=vc.to(kind), k_scale=torch.full((pages, 1), 1.0 / 64), v_scale=vs)
+    return c, torch.arange(pages, dtype=torch.int32)[None], minus
+
+
+def _decode(c, q, table, lengths, gate, scale):
+    import selective_attention_b200 as sab
+
+    dev = {n: t.cuda() for n, t in c.items()}
+    got = sab.sattn_paged_decode(q.cuda(), block_table=table.cuda(), lengths=lengths.cuda(), scale=scale,
+                                 log_gate_cache=None if gate is None else gate.cuda(), **dev)
+    ref = paged_ref.decode(q, c["k_cache"], c["v_cache"], c["k_scale"], c["v_scale"], table, lengths, gate, scale)
+    return got, ref
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", [torch.int8, torch.float8_e4m3fn])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("high", [1e4, 1e9, 1e20, INF, NAN])
+def test_scales_of_dropped_pages_do_not_matter(kind, dtype, high):
+    c, table, minus = _two_kinds_of_pages(kind, high)
+    gate = torch.zeros(len(minus), 1, 16)
+    gate[minus] = -INF
+    q = torch.randn(1, 3, 64, generator=torch.Generator().manual_seed(3)).to(dtype)
+    got, ref = _decode(c, q, table, torch.tensor([len(minus) * 16 - 3], dtype=torch.int32), gate, 0.5)
+    close(got, ref, 1.0, DECODE_TOL)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", [torch.int8, torch.float8_e4m3fn])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("high", [1e4, 1e9, 1e15])
+@pytest.mark.parametrize("heads", [2, 12])
+def test_scales_of_pages_without_weight_do_not_matter_to_a_head(kind, dtype, high, heads):
+    """Every second head weighs the other kind of pages: each has the bits that its own pages' values need."""
+    c, table, minus = _two_kinds_of_pages(kind, high)
+    q = torch.zeros(1, heads, 64)
+    q[0, :, 0] = torch.where(torch.arange(heads) % 2 == 0, 40.0, -40.0)  # weights e^-80 of the other kind
+    got, ref = _decode(c, q.to(dtype), table, torch.tensor([len(minus) * 16], dtype=torch.int32), None, 1.0)
+    close(got[:, ::2], ref[:, ::2], 1.0 + math.exp(-80) * 96 * high, DECODE_TOL, "ordinary pages")
+    if dtype != torch.float16:  # (whose range ends before these values)
+        close(got[:, 1::2], ref[:, 1::2], 96.0 * high, DECODE_TOL, "pages of large values")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("scale", [0.0, 1e-38, 1e-30, 1e30])
+def test_values_near_the_ends_of_the_range(dtype, scale):
+    c, table, minus = _two_kinds_of_pages(torch.int8, scale)
+    c["v_scale"][:] = scale
+    q = torch.randn(1, 2, 64, generator=torch.Generator().manual_seed(3)).to(dtype)
+    got, ref = _decode(c, q, table, torch.tensor([len(minus) * 16], dtype=torch.int32), None, 0.5)
+    close(got, ref, 96.0 * scale + 1e-38, DECODE_TOL)
