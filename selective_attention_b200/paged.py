@@ -277,8 +277,8 @@ def sattn_paged_decode(q, k_cache, v_cache, k_scale, v_scale, block_table, lengt
     appended before): the pos-mode gated softmax of :func:`~.kernels.sattn_decode_step`
     (``modules/selective_attention.py:399-404``), in which every key but the own one adds its log-gate
     and a log-gate of ``-inf`` drops the key. A length of 0 gives zeros. ``scale`` defaults to
-    ``D ** -0.5``. Returns ``(R, Hq, D)`` in ``q``'s dtype. ``workspace`` (uint8) is allocated when it
-    is ``None`` or too small; calls that overlap on the GPU need one each.
+    ``D ** -0.5``. Returns ``(R, Hq, D)`` in ``q``'s dtype. ``workspace`` (contiguous uint8) is
+    allocated when it is ``None`` or does not do; calls that overlap on the GPU need one each.
     """
     c, H, page, D, d = _cache(k_cache, v_cache, k_scale, v_scale, log_gate_cache)
     shape = q.shape
@@ -305,7 +305,8 @@ def sattn_paged_decode(q, k_cache, v_cache, k_scale, v_scale, block_table, lengt
     if W == 0:
         return out.zero_()
     need = _decode_workspace(H, page, D, Hq)
-    if workspace is None or workspace.numel() * workspace.element_size() < need or workspace.data_ptr() % 16:
+    if (workspace is None or workspace.numel() * workspace.element_size() < need or workspace.data_ptr() % 16
+            or not workspace.is_contiguous()):
         workspace = torch.empty(need, device=dev, dtype=torch.uint8)
     _call("sattn_paged_decode", d, c, q.data_ptr(), block_table.data_ptr(), lengths.data_ptr(), out.data_ptr(), R, W, Hq,
           D ** -0.5 if scale is None else float(scale), code, workspace.data_ptr(), need)

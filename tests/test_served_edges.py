@@ -92,3 +92,23 @@ def test_values_near_the_ends_of_the_range(dtype, scale):
     q = torch.randn(1, 2, 64, generator=torch.Generator().manual_seed(3)).to(dtype)
     got, ref = _decode(c, q, table, torch.tensor([len(minus) * 16], dtype=torch.int32), None, 0.5)
     close(got, ref, 96.0 * scale + 1e-38, DECODE_TOL)
+
+
+# ----------------------------------------------------------------------------- decode: workspace
+@pytest.mark.gpu
+@pytest.mark.parametrize("how", ["expanded", "strided", "short", "unaligned"])
+def test_a_workspace_that_is_not_one_piece_of_memory_is_not_written(how):
+    """Its numel says nothing of the bytes behind it: the call takes one of its own."""
+    import selective_attention_b200 as sab
+
+    c, table, _ = _two_kinds_of_pages(torch.int8, 0.01, pages=120)
+    dev = {n: t.cuda() for n, t in c.items()}
+    args = dict(block_table=table.cuda(), lengths=torch.tensor([1900], dtype=torch.int32, device="cuda"), **dev)
+    q = torch.randn(1, 2, 64, generator=torch.Generator().manual_seed(3)).cuda()
+    want = sab.sattn_paged_decode(q, **args)
+    held = torch.zeros(1 << 23, dtype=torch.uint8, device="cuda")
+    work = {"expanded": held[:1].expand(1 << 22), "strided": held[::2], "short": held[:64],
+            "unaligned": held[8:]}[how]
+    assert torch.equal(sab.sattn_paged_decode(q, workspace=work, **args), want) and not held.any()
+    good = held[:1 << 22]
+    assert torch.equal(sab.sattn_paged_decode(q, workspace=good, **args), want) and bool(held.any())
