@@ -165,7 +165,7 @@ __global__ void __launch_bounds__(256, 2) sattn_packed_kernel(const T* __restric
       float rs = 0.f;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float p = sc[i][j] == -INFINITY ? 0.f : expf(sc[i][j] - mn);
+        const float p = sc[i][j] == -INFINITY ? -0.f : expf(sc[i][j] - mn);  // (a weight is never -0)
         rs += p;
         Ps[(tr + 16 * i) * LDP + tc + 16 * j] = p;
       }
@@ -174,7 +174,8 @@ __global__ void __launch_bounds__(256, 2) sattn_packed_kernel(const T* __restric
       for (int e = 0; e < 2 * G; ++e) o[i][e] = pk2(lo2(o[i][e]) * corr, hi2(o[i][e]) * corr);
       m[i] = mn;
     }
-    // a key that a row does not see is left out of its product, not multiplied by zero
+    // a key that a row does not see is left out of its product, not multiplied by zero; one that it sees is
+    // multiplied also where its weight has underflowed
     skip = __syncthreads_or(skip);
     if constexpr (simt_share<D>()) {  // (every score has been computed)
       stage64<T>(Vs, LD, v + (base + k0) * st.v_ts + hk * st.v_hs, st.v_ts, min(kPT, n - k0), D);
@@ -195,7 +196,7 @@ __global__ void __launch_bounds__(256, 2) sattn_packed_kernel(const T* __restric
           for (int i = 0; i < 4; ++i) {
             const float p = qq == 0 ? pa[i].x : (qq == 1 ? pa[i].y : (qq == 2 ? pa[i].z : pa[i].w));
             const uint64_t pp = pk2(p, p);
-            const bool out = decltype(leave_out)::value && p == 0.f;
+            const bool out = decltype(leave_out)::value && __float_as_uint(p) == 0x80000000u;
 #pragma unroll
             for (int g = 0; g < G; ++g) {
               o[i][2 * g] = fma2(pp, out ? 0 : vv[g].x, o[i][2 * g]);

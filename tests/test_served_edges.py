@@ -1,7 +1,7 @@
 """Served selective attention where values, weights or lengths are far from ordinary, against
-``oracle/paged_ref.py``: page scales many orders apart.
+``oracle/paged_ref.py``: page scales many orders apart, weights that underflow.
 
-Tolerances are those of ``test_paged.py``: a share of the result for its own rounding
+Tolerances are those of ``test_paged.py`` and ``test_sattn_packed.py``: a share of the result for its own rounding
 and a share of the weighted magnitudes sum_j w_j |v_j| that the row adds up for the rounding of its weights, each of
 which is relative. Where one group of keys holds all the weight, that sum is at most the group's largest |v|.
 """
@@ -14,6 +14,7 @@ from oracle import paged_ref
 
 INF = float("inf")
 NAN = float("nan")
+PROMPT_TOL = {torch.bfloat16: (2 ** -8, 2 ** -8), torch.float16: (2 ** -10, 2 ** -10), torch.float32: (1e-5, 3e-5)}
 DECODE_TOL = {torch.bfloat16: (2 ** -8, 2 ** -10), torch.float16: (2 ** -10, 2 ** -10), torch.float32: (1e-5, 3e-5)}
 
 
@@ -112,3 +113,32 @@ def test_a_workspace_that_is_not_one_piece_of_memory_is_not_written(how):
     assert torch.equal(sab.sattn_paged_decode(q, workspace=work, **args), want) and not held.any()
     good = held[:1 << 22]
     assert torch.equal(sab.sattn_paged_decode(q, workspace=good, **args), want) and bool(held.any())
+
+
+# ----------------------------------------------------------------------------- packed prompts
+def _prompt(q, k, v, gate=None, scale=None, impl="auto"):
+    import selective_attention_b200 as sab
+
+    cu = torch.tensor([0, q.shape[0]], dtype=torch.int32)
+    got = sab.sattn_prefill_packed(q.cuda(), k.cuda(), v.cuda(), cu.cuda(), None if gate is None else gate.cuda(), scale,
+                                   impl=impl)
+    sab.check_device_error()
+    return got, paged_ref.prefill_packed(q, k, v, cu, gate, scale)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("D", [32, 64, 128])
+@pytest.mark.parametrize("T", [20, 150])
+def test_a_nan_under_a_weight_that_underflows_is_seen(dtype, D, T):
+    """A key's value is NaN and its score 400 below the others: rows from its position on see it."""
+    g = torch.Generator().manual_seed(T + D)
+    q, k, v = (torch.randn(T, 1, D, generator=g) * 0.1 for _ in range(3))
+    q[..., 0], k[..., 0] = 20.0, 10.0
+    at = T - 9
+    k[at, 0, 0] = -10.0
+    v[at, 0, 3] = NAN
+    q, k, v = (x.to(dtype) for x in (q, k, v))
+    got, ref = _prompt(q, k, v, scale=1.0)
+    assert bool(ref[at:, 0, 3].isnan().all()) and not bool(ref[:at].isnan().any())
+    close(got, ref, v[v.isfinite()].float().abs().max().item(), PROMPT_TOL)
