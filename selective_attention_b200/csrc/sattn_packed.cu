@@ -41,10 +41,10 @@ __device__ __forceinline__ float hi2(uint64_t x) { return __uint_as_float((uint3
 // 64-key tiles of K and V staged in shared memory as fp32; thread (tr, tc) owns rows tr + 16 i
 // (i < 4), score columns tc + 16 j, output columns 4 tc + 64 g (g < D / 64). Two products an
 // instruction (fp32 pairs). At head_dim 128 V takes K's place once the scores are there, so that two CTAs fit
-// an SM. Bound by the latency of a key tile (load, scores, softmax, products, three barriers in a row)
-// in the longest sequence's last tiles: three CTAs an SM instead of two change nothing. 8 prompts of up
-// to 1024 tokens: fp32, 16 heads on 4 of 128, 563 us (25 TFLOP/s); bf16, the same heads of 32, 262 us; fp32, 24
-// heads of 64 with gates, 578 us.
+// an SM. A CTA takes the tile of its rank, so that the tiles with most keys start first (the other way round the
+// longest ones ended alone: 564 us instead of 488 in the first case below). Bound by reading shared
+// memory, whose pipe is 78 % busy (the FMA units 54 %). 8 prompts of up to 1024 tokens: fp32, 16 heads on 4 of 128,
+// 488 us (29 TFLOP/s); bf16, the same heads of 32, 222 us; fp32, 24 heads of 64 with gates, 501 us.
 // ===========================================================================
 template <int D> constexpr bool simt_share() { return D == 128; }
 template <int D> constexpr size_t simt_smem() {
@@ -86,7 +86,7 @@ __global__ void __launch_bounds__(256, 2) sattn_packed_kernel(const T* __restric
   if (tid < 32) {
     PackedFinder<6> finder;
     finder.init(cu, R, Tn);
-    const PackedTile t = finder.find((int)(gridDim.y - 1 - blockIdx.y));  // the last tiles of a sequence have most keys
+    const PackedTile t = finder.find((int)blockIdx.y);
     if (tid == 0) s_tile = t;
   }
   __syncthreads();
