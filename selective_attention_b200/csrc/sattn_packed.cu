@@ -262,8 +262,8 @@ cudaError_t packed_simt_t(const PackedArgs& a, cudaStream_t s) {
 //                     S_w(j): O_w += P_w V_j (A from TMEM), then S_w(j + 1). The tiles alternate, so
 //                     that the tensor core works on one while the other's softmax runs;
 //   warps 4-7, 8-11   softmax of tile w, thread = query row = TMEM lane, a tile's 128 scores in
-//                     registers: running maximum in log2 units (O is rescaled only when it grows
-//                     by more than e^8), P = 2^(s - m) rounded to the type, fp32 sums;
+//                     registers: running maximum in log2 units (O is rescaled only when it grows by
+//                     more than 2^kRescale), P = 2^(s - m + kOffset) rounded to the type, fp32 sums;
 //   warps 2-3         what no query may meet: a product multiplies by zero where it should leave
 //                     out, which is wrong for infinities and NaN. In the last key tiles (own, later
 //                     and other sequences' positions) they set non-finite elements of V to zero, and
@@ -286,7 +286,11 @@ using namespace sm100;
 constexpr int kPkThreads = 384;
 constexpr int kCleanSlots = 4;
 constexpr float kPkLog2e = 1.4426950408889634f;
-constexpr float kPkRescale = 8.0f * kPkLog2e;
+// P in bfloat16 has fp32's exponents. In fp16 it would lose bits below 2^-14 and end at 2^-25, while the sums go on:
+// 131000 keys of weight e^-16.2, 1 % of a row, came out 29 % too heavy. Up to 2^15 it keeps all bits
+// down to 2^-21 of the largest weight, and no weight is off by more than 2^-32 of it.
+template <typename T> struct PkRange { static constexpr float kRescale = 8.0f * kPkLog2e, kOffset = 0.0f; };
+template <> struct PkRange<__half> { static constexpr float kRescale = 8.0f, kOffset = 7.0f; };
 constexpr unsigned int kSitePkLoad = 0x411, kSitePkMma = 0x412, kSitePkSoft = 0x413, kSitePkClean = 0x414;
 template <int D> constexpr int pk_tile_bytes() { return 128 * D * 2; }
 // One ring for the tiles of K and V in the order of their use, K_0 V_0 K_1 V_1 ...: what shared memory
@@ -827,7 +831,7 @@ __global__ void __launch_bounds__(kPkThreads, 1)
         const float mt = fmaxf(fmaxf(mp[0], mp[1]), fmaxf(mp[2], mp[3])) * mul;
         float f = 1.f;
         bool resc = false;
-        if (mt < INFINITY && mt > m_used + kPkRescale) {
+        if (mt < INFINITY && mt > m_used + PkRange<T>::kRescale) {
           if (m_used != -INFINITY) {  // O and the sum hold earlier tiles: rescale them
             f = pk_ex2(m_used - mt);
             lsum *= f;
@@ -847,7 +851,7 @@ __global__ void __launch_bounds__(kPkThreads, 1)
             tmem_st16(to + 16 * c, o);
           }
         }
-        const float mb = m_used == -INFINITY ? 0.f : -m_used;
+        const float mb = m_used == -INFINITY ? 0.f : PkRange<T>::kOffset - m_used;
         const uint64_t mul2 = pk2(mul, mul), mb2 = pk2(mb, mb);
         uint64_t ls[2] = {0ull, 0ull};
 #pragma unroll

@@ -142,3 +142,32 @@ def test_a_nan_under_a_weight_that_underflows_is_seen(dtype, D, T):
     got, ref = _prompt(q, k, v, scale=1.0)
     assert bool(ref[at:, 0, 3].isnan().all()) and not bool(ref[:at].isnan().any())
     close(got, ref, v[v.isfinite()].float().abs().max().item(), PROMPT_TOL)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D", [64, 128])
+def test_many_keys_of_small_weight_add_up(dtype, D):
+    """One key of weight 1 and value 0, and 131000 keys of weight e^-16.2 (1.55 steps of fp16's smallest number) and value 1:
+    together they are 1 % of the sum. The last rows are compared; q and k are exact, so the oracle is their sum."""
+    import selective_attention_b200 as sab
+
+    T, gap = 131000, 16.2
+    q, k, v = (torch.zeros(T, 1, D, dtype=dtype) for _ in range(3))
+    q[:, 0, 0] = 1.0
+    k[0, 0, 0] = 8.0
+    k[1:, 0, 0] = 8.0 - 16.0
+    v[1:] = 1.0
+    scale = gap / 16
+    cu = torch.tensor([0, T], dtype=torch.int32)
+    got = sab.sattn_prefill_packed(q.cuda(), k.cuda(), v.cuda(), cu.cuda(), None, scale)[-300:]
+    sab.check_device_error()
+    n = torch.arange(T - 300, T, dtype=torch.float64)
+    w = n * math.exp(-gap)
+    ref = (w / (1 + w))[:, None, None].expand(-1, 1, D)
+    # a weight's rounding is relative (the weighted magnitudes are the result itself), but half a step of 2^-31 of the
+    # largest weight where float16 has no exponent left; the scores' own roundings in 32 bits move a weight by 1e-4 at most
+    rel, least = {torch.bfloat16: (2 ** -7, 0.0), torch.float16: (2 ** -9, 2 ** -32)}[dtype]
+    err = (got.double().cpu() - ref).abs()
+    bound = (rel + 1e-4) * ref + T * least
+    assert bool((err <= bound).all()), f"max relative err {(err / ref).max().item():.3e}"
