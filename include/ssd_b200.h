@@ -399,15 +399,17 @@ typedef struct sattn_cache {
  * synchronisation). Request r holds lengths[r] tokens in the pages block_table[r, 0 ..
  * ceil(lengths[r] / page_size)) and is to take new_lengths[r] more. Free pages are a ring:
  * free_pages[i % num_free] for i in [free_state[0], free_state[1]) are free, handed out in that
- * order to the requests in order. A request whose pages do not fit the table's width, or that
- * asks for more than is left for it, is not served: its length stays, its slots are -1, and it
- * and later ones that need a page get none (a request that needs no page is served).
+ * order to the requests in order. A request is not served, that is its length stays, its slots are -1 and it
+ * gets no page, in three cases:
+ *   - its pages do not fit the table's width: this request alone;
+ *   - too few pages are left for it: it and every later one that needs a page (one that needs none is served);
+ *   - its tokens do not all lie within num_tokens: it and every later one with new tokens.
  *   lengths, new_lengths  (requests,)              int32
  *   block_table           (requests, table_width)  int32, new entries written in place
  *   free_pages            (num_free,)              int32
  *   free_state            (2,)                     int64: handed out, returned (running counts)
  *   lengths_out           (requests,)              int32: lengths after the tokens are written
- *   cu_new                (requests + 1,)          int32: offsets of the requests' tokens
+ *   cu_new                (requests + 1,)          int32: offsets of the requests' tokens, served or not (at most 2^31 - 1)
  *   slots, positions      (num_tokens,)            int64, int32: of each token; -1 and 0 past cu_new's end
  *   free_state_out        (2,)                     int64
  * Outputs other than block_table do not overlap inputs.

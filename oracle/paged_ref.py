@@ -25,12 +25,13 @@ def plan(lengths, new_lengths, block_table, free_pages, free_state, num_tokens, 
         if served:
             upto += end - has
             served = end == has or upto <= min(tail - head, free_pages.numel())
+        served = served and (add == 0 or cu[-1] + add <= num_tokens)
         if served and end > has:
             for i in range(end - has):
                 at = head + upto - (end - has) + i
                 table[r, has + i] = free_pages[at % free_pages.numel()]
             given = upto
-        for i in range(add):
+        for i in range(min(add, num_tokens - len(slots))):
             p = n + i
             slots.append(int(table[r, p // page]) * page + p % page if served else -1)
             pos.append(p)
@@ -38,7 +39,7 @@ def plan(lengths, new_lengths, block_table, free_pages, free_state, num_tokens, 
         cu.append(cu[-1] + add)
     slots = (slots + [-1] * num_tokens)[:num_tokens]
     pos = (pos + [0] * num_tokens)[:num_tokens]
-    return (table, torch.tensor(out, dtype=torch.int32), torch.tensor(cu, dtype=torch.int32),
+    return (table, torch.tensor(out, dtype=torch.int32), torch.tensor(cu).clamp(max=2 ** 31 - 1).to(torch.int32),
             torch.tensor(slots, dtype=torch.int64), torch.tensor(pos, dtype=torch.int32),
             torch.tensor([head + given, tail], dtype=torch.int64))
 

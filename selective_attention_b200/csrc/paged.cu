@@ -21,12 +21,14 @@ namespace {
 // plan
 // ---------------------------------------------------------------------------
 // One launch; a CTA writes the slots and positions of kPlanTokens new tokens. Each CTA sums all
-// requests' new tokens and pages by itself (a block scan over pairs packed in 64 bits), which
+// requests' new tokens and pages by itself (a block scan over pairs, which stop at 2^31), which
 // for some hundred requests costs less than a second launch or a wait between CTAs would; the
 // requests that begin in or reach into its tokens leave an entry at their first token there, and
 // a running maximum over the tokens finds each token's entry. A page's table entry is written by
 // the token at its first position, so no two threads write one entry and none is read that
-// another writes. Bound by latency: 256 requests of one token each take 3 us, 384 prompts with 393k tokens 5.
+// another writes; so only a request whose tokens are all among the T that are planned is served, or it
+// would hold pages that its table does not name. Those that are come first, so that a sum that has stopped
+// is never theirs. Bound by latency: 256 requests of one token each take 3 us, 384 prompts with 393k tokens 5.
 constexpr int kPlanThreads = 256;
 constexpr int kPlanPer = 4;
 constexpr int kPlanTokens = kPlanThreads * kPlanPer;
@@ -36,13 +38,19 @@ struct PlanEntry {
   int served;
 };
 
-__device__ __forceinline__ unsigned long long warp_scan_add(unsigned long long v, int lane) {
-#pragma unroll
-  for (int off = 1; off < 32; off <<= 1) {
-    const unsigned long long o = __shfl_up_sync(0xffffffffu, v, off);
-    if (lane >= off) v += o;
-  }
-  return v;
+// New tokens and pages, each at most 2^31.
+struct PlanSum {
+  unsigned tokens, pages;
+};
+__device__ __forceinline__ unsigned add_up_to(unsigned a, unsigned b) {
+  const unsigned c = a + b;
+  return c < a ? 0x80000000u : min(c, 0x80000000u);
+}
+__device__ __forceinline__ PlanSum operator+(PlanSum a, PlanSum b) {
+  return PlanSum{add_up_to(a.tokens, b.tokens), add_up_to(a.pages, b.pages)};
+}
+__device__ __forceinline__ PlanSum shfl_up(PlanSum v, int off) {
+  return PlanSum{__shfl_up_sync(0xffffffffu, v.tokens, off), __shfl_up_sync(0xffffffffu, v.pages, off)};
 }
 
 __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(
@@ -52,7 +60,7 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(
     long long F, long long T, int page_shift) {
   __shared__ PlanEntry ent[kPlanTokens];
   __shared__ short start[kPlanTokens];
-  __shared__ unsigned long long wsum[kPlanThreads / 32];
+  __shared__ PlanSum wsum[kPlanThreads / 32];
   __shared__ int wmax[kPlanThreads / 32];
   __shared__ long long s_given;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -65,7 +73,7 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(
   for (int i = 0; i < kPlanPer; ++i) start[tid + i * kPlanThreads] = -1;
   if (tid == 0) s_given = 0;
   __syncthreads();
-  unsigned long long carry = 0;  // low word: new tokens, high word: pages
+  PlanSum carry{0u, 0u};
   for (int r0 = 0; r0 < R; r0 += kPlanThreads) {
     const int r = r0 + tid;
     int len = 0, add = 0, need = 0;
@@ -77,31 +85,36 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(
       fits = end <= W;
       need = fits ? (int)(end - (((long long)len + page - 1) >> page_shift)) : 0;
     }
-    const unsigned long long mine = ((unsigned long long)(unsigned)need << 32) | (unsigned)add;
-    unsigned long long incl = warp_scan_add(mine, lane);
+    PlanSum incl{(unsigned)add, (unsigned)need};
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const PlanSum o = shfl_up(incl, off);
+      if (lane >= off) incl = o + incl;
+    }
     if (lane == 31) wsum[warp] = incl;
+    PlanSum excl = shfl_up(incl, 1);
+    if (lane == 0) excl = PlanSum{0u, 0u};
     __syncthreads();
-    unsigned long long before = carry, all = carry;
+    PlanSum before = carry, all = carry;
 #pragma unroll
     for (int w = 0; w < kPlanThreads / 32; ++w) {
-      const unsigned long long x = wsum[w];
-      if (w < warp) before += x;
-      all += x;
+      const PlanSum x = wsum[w];
+      if (w < warp) before = before + x;
+      all = all + x;
     }
     carry = all;
-    incl += before;
-    const long long upto = (long long)(incl >> 32);
-    const int cu = (int)((unsigned)incl - (unsigned)add);
-    const bool served = r < R && fits && (need == 0 || upto <= avail);
+    incl = before + incl;
+    const long long upto = incl.pages, cu = (before + excl).tokens;
+    const bool served = r < R && fits && (need == 0 || upto <= avail) && (add == 0 || cu + add <= T);
     if (r < R) {
-      if (add > 0 && cu < t1 && cu + (long long)add > t0) {
-        const int at = (int)(max((long long)cu, t0) - t0);
-        ent[at] = PlanEntry{r, len, cu, (int)(upto - need), served};
+      if (add > 0 && cu < t1 && cu + add > t0) {
+        const int at = (int)(max(cu, t0) - t0);
+        ent[at] = PlanEntry{r, len, (int)cu, (int)(upto - need), served};
         start[at] = (short)at;
       }
       if (blockIdx.x == 0) {
         lengths_out[r] = served ? len + add : lengths[r];
-        cu_new[r + 1] = cu + add;
+        cu_new[r + 1] = (int)min(incl.tokens, 0x7fffffffu);
         if (served && need > 0) atomicMax((unsigned long long*)&s_given, (unsigned long long)upto);
       }
     }
@@ -130,7 +143,7 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(
   int prev = __shfl_up_sync(0xffffffffu, incl, 1);
   if (lane == 0) prev = -1;
   for (int w = 0; w < warp; ++w) prev = max(prev, wmax[w]);
-  const long long total = (long long)(unsigned)carry;
+  const long long total = carry.tokens;
 #pragma unroll
   for (int i = 0; i < kPlanPer; ++i) {
     const long long t = t0 + tid * kPlanPer + i;

@@ -87,13 +87,14 @@ def sattn_paged_plan(lengths, new_lengths, block_table, free_pages, free_state, 
     ``new_lengths[r]`` more; pages come from the ring ``free_pages``, of which those counted
     ``free_state[0]`` to ``free_state[1]`` (int64; handed out, returned) are free. ``lengths``,
     ``new_lengths`` ``(R,)``, ``block_table`` ``(R, W)`` and ``free_pages`` ``(F,)`` are int32;
-    ``num_tokens`` is the number of rows to plan (the new tokens, or more: padding). New entries of
+    ``num_tokens`` is the number of rows to plan: the new tokens, or more (padding). New entries of
     ``block_table`` are written in place; nothing else of the inputs changes.
 
     Returns ``(lengths_out, cu_new, slots, positions, free_state_out)``: ``(R,)`` int32 lengths
     with the new tokens, ``(R + 1,)`` int32 offsets of each request's tokens, ``(num_tokens,)`` int64
     slots (page * page_size + place) and int32 positions, and the ring's new state. A request whose
-    pages are not to be had keeps its length and gets slots of -1.
+    pages are not to be had, or whose tokens do not all lie within ``num_tokens``, keeps its length and gets
+    slots of -1.
     """
     d = lengths.get_device()
     shape = block_table.shape
@@ -424,7 +425,7 @@ class PagedSelectiveCache:
 
     def plan(self, new_lengths: torch.Tensor, num_tokens: int):
         """Pages for ``new_lengths`` ``(requests,)`` int32 more tokens (0: the request takes no part);
-        ``num_tokens`` is their sum, or more. Returns ``(cu_seqlens, slots, positions)``."""
+        ``num_tokens`` is their sum, or more (requests past it are not served). Returns ``(cu_seqlens, slots, positions)``."""
         self.lengths, cu, slots, positions, self.free_state = sattn_paged_plan(
             self.lengths, new_lengths, self.block_table, self.free_pages, self.free_state, num_tokens, self.page_size)
         return cu, slots, positions

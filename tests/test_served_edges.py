@@ -171,3 +171,61 @@ def test_many_keys_of_small_weight_add_up(dtype, D):
     err = (got.double().cpu() - ref).abs()
     bound = (rel + 1e-4) * ref + T * least
     assert bool((err <= bound).all()), f"max relative err {(err / ref).max().item():.3e}"
+
+
+# ----------------------------------------------------------------------------- plan: tokens past the planned ones
+MANY = 2 ** 31 - 1
+
+
+def _plan(lengths, new, width, num_tokens, page=16, free=64):
+    args = (torch.tensor(lengths, dtype=torch.int32), torch.tensor(new, dtype=torch.int32),
+            torch.full((len(lengths), width), -1, dtype=torch.int32), torch.arange(free, dtype=torch.int32).flip(0).contiguous(),
+            torch.tensor([0, free]))
+    for r, n in enumerate(lengths):
+        args[2][r, :-(-n // page)] = 100 + r
+    return args, num_tokens, page
+
+
+PAST = [_plan([0, 0, 0], [20, 30, 5], 4, 54), _plan([0, 0, 0], [20, 30, 5], 4, 20), _plan([0, 0], [20, 30], 4, 19),
+        _plan([3, 40, 0, 9], [2, 0, 60, 0], 4, 10), _plan([5], [3], 2, 0), _plan([0] * 300, [7] * 300, 1, 1500, free=300),
+        _plan([0, 0, 0, 0], [5, MANY, MANY, 6], 4, 12), _plan([0] * 600, [9] + [MANY] * 598 + [5], 4, 1100),
+        # sums that pass 2^32 by a little
+        _plan([0, 0, 0, 0], [MANY, MANY, 2, 9], 4, 100), _plan([0] * 34, [5] + [MANY] * 32 + [50], 4, 60)]
+
+
+@pytest.mark.parametrize("case", PAST)
+def test_plan_oracle_serves_no_request_past_the_planned_tokens(case):
+    (lengths, new, table, free, state), T, page = case
+    got, n, cu, slots, _, st = paged_ref.plan(lengths, new, table, free, state, T, page)
+    assert slots.numel() == T and st[0] - state[0] == ((got >= 0) & (table < 0)).sum()
+    for r in range(len(n)):
+        pages = -(-int(n[r]) // page)
+        assert bool((got[r, :pages] >= 0).all()) and bool((got[r, pages:] == -1).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", PAST)
+def test_plan_serves_no_request_past_the_planned_tokens(case):
+    """Every request holds just the pages that its table names, whatever its new length."""
+    import selective_attention_b200 as sab
+
+    args, T, page = case
+    ref = paged_ref.plan(*args, T, page)
+    dev = [a.cuda() for a in args]
+    got = sab.sattn_paged_plan(*dev, T, page)
+    assert torch.equal(dev[2].cpu(), ref[0])
+    for g, r, n in zip(got, ref[1:], ("lengths", "cu", "slots", "positions", "free_state")):
+        assert torch.equal(g.cpu(), r), n
+
+
+@pytest.mark.gpu
+def test_pages_come_back_whole_after_a_plan_for_too_few_tokens():
+    import selective_attention_b200 as sab
+
+    c = sab.PagedSelectiveCache(1, 2, 64, 6, 1, 64, 16)
+    c.plan(torch.tensor([20, 20], dtype=torch.int32, device="cuda"), 39)
+    assert c.lengths.tolist() == [20, 0]
+    c.release(torch.tensor([0, 1], device="cuda"))
+    head, tail = c.free_state.tolist()
+    ring = c.free_pages.tolist()
+    assert sorted(ring[i % 6] for i in range(head, tail)) == list(range(6))
