@@ -445,9 +445,11 @@ int sattn_paged_read(const sattn_cache* cache, const int64_t* slots, int64_t num
  * One decode step's attention: for request r with n = lengths[r] cached tokens (its own last),
  *   s_j = scale * q . k_j + (j < n-1 ? log_gate_j : 0),   out = softmax(s) . v
  * (the pos-mode gated softmax of sattn_decode_step). A key with log-gate -inf drops out; n = 0 gives
- * zeros; n is cut to the table's width.
+ * zeros; n is cut to the table's width. A table entry that is no page of the cache drops its keys; a request
+ * of whose keys none is left gets NaN.
  *   q, out       (requests, nheads, D)    dtype, 16-byte aligned; nheads a multiple of Hkv
  *   block_table  (requests, table_width)  int32        lengths  (requests,)  int32
+ * At most 65535 requests, and num_pages * Hkv and table_width * page_size below 2^31.
  * workspace: sattn_paged_decode_workspace_size() bytes (may be 0), 16-byte aligned; nothing in it
  * needs to start at zero or outlives the call.
  */
@@ -471,6 +473,8 @@ int sattn_paged_decode(const sattn_cache* cache, const void* q, const int32_t* b
  * All base addresses 16-byte aligned, all strides multiples of 16 bytes; D in {16, 32, 64, 128}.
  * impl: SSD_IMPL_AUTO takes the tcgen05 kernel for 16-bit types with D 64 or 128 and the
  * CUDA-core kernel otherwise; SSD_IMPL_TC requires the former, SSD_IMPL_SIMT forces the latter.
+ * num_tokens / tile + num_seqs is at most 65534, with tiles of 64 positions on CUDA cores, 128 on tensor cores,
+ * 256 there where nheads / nkv is odd.
  */
 typedef struct sattn_packed_params {
   int64_t num_tokens, num_seqs, nheads, nkv, head_dim;

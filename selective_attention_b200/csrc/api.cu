@@ -696,7 +696,8 @@ int paged_cache(const sattn_cache* c, PagedCache* o) {
 }
 
 bool decode_geometry_ok(const PagedCache& c, int64_t requests, int64_t width, int64_t nheads) {
-  return requests > 0 && requests <= 0x7fffffffll && width > 0 && nheads > 0 && nheads <= 65535 &&
+  // (requests: the join's grid; pages * nkv: the tensor maps' coordinate over both)
+  return requests > 0 && requests <= 65535 && c.pages * c.nkv <= 0x7fffffffll && width > 0 && nheads > 0 && nheads <= 65535 &&
          nheads % c.nkv == 0 && width <= 0x7fffffffll / c.page;
 }
 
@@ -813,6 +814,7 @@ int sattn_prefill_packed(const sattn_packed_params* p, void* stream) {
   a.st = PackedStrides{strides[0], strides[1], strides[2], strides[3], strides[4], strides[5]};
   a.scale = p->scale;
   a.use_tc = p->impl != SSD_IMPL_SIMT && tc_ok;
+  if (!sattn_packed_fits(a)) return SSD_ERR_INVALID_ARGUMENT;
   return cuda_status(launch_sattn_packed(a, reinterpret_cast<cudaStream_t>(stream)));
 }
 

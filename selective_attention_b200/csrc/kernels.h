@@ -149,6 +149,7 @@ struct PackedArgs {
   int use_tc;
 };
 bool sattn_packed_tc_supported(int D, int dtype);
+bool sattn_packed_fits(const PackedArgs& a);  // in a grid
 cudaError_t launch_sattn_packed(const PackedArgs& a, cudaStream_t s);
 unsigned int fetch_error_packed(cudaStream_t s);
 

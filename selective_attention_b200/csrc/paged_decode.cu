@@ -846,8 +846,6 @@ size_t paged_decode_workspace(int Hq, int Hk, int D) {
 
 cudaError_t launch_paged_decode(const PagedCache& c, const void* q, const int* table, const int* lengths, void* out,
                                 int R, int W, int Hq, float scale, int dtype, void* workspace, cudaStream_t s) {
-  // the join's grid, and the tensor maps' coordinate over (page, head)
-  if (R > 65535 || c.pages * c.nkv > 0x7fffffffll) return cudaErrorInvalidValue;
   DecodeArgs a{};
   a.q = q;
   a.ks = c.ks, a.vs = c.vs, a.gc = c.gate;

@@ -233,9 +233,7 @@ cudaError_t packed_simt_d(const PackedArgs& a, cudaStream_t s) {
   static unsigned long long allowed = 0;
   cudaError_t e = allow_smem(sattn_packed_kernel<T, D>, smem, allowed);
   if (e != cudaSuccess) return e;
-  const long long tiles = packed_tile_bound(a.T, a.R, kPT);
-  if (tiles > 65535) return cudaErrorInvalidValue;
-  dim3 grid((unsigned)a.Hq, (unsigned)tiles);
+  dim3 grid((unsigned)a.Hq, (unsigned)packed_tile_bound(a.T, a.R, kPT));
   sattn_packed_kernel<T, D><<<grid, 256, smem, s>>>((const T*)a.q, (const T*)a.k, (const T*)a.v, a.log_gate, a.cu,
                                                     (T*)a.out, a.R, a.T, a.Hq, a.Hk, a.st, a.scale);
   return cudaGetLastError();
@@ -950,7 +948,6 @@ cudaError_t packed_tc_t(const PackedArgs& a, cudaStream_t s) {
   k.v_ts = a.st.v_ts, k.v_hs = a.st.v_hs;
   k.scale = a.scale;
   const long long tiles = packed_tile_bound(a.T, a.R, PAIR ? 128 : 256);
-  if (tiles > 65535) return cudaErrorInvalidValue;
   auto fn = sattn_packed_tc_kernel<T, D, GATED, PAIR>;
   static unsigned long long allowed = 0;
   cudaError_t e = allow_smem(fn, pk_smem<D, GATED>(), allowed);
@@ -959,9 +956,11 @@ cudaError_t packed_tc_t(const PackedArgs& a, cudaStream_t s) {
   return cudaGetLastError();
 }
 
+bool packed_pair(const PackedArgs& a) { return (a.Hq / a.Hk) % 2 == 0; }
+
 template <typename T>
 cudaError_t packed_tc(const PackedArgs& a, cudaStream_t s) {
-  const bool pair = (a.Hq / a.Hk) % 2 == 0;
+  const bool pair = packed_pair(a);
   if (a.D == 64) {
     if (a.log_gate) return pair ? packed_tc_t<T, 64, true, true>(a, s) : packed_tc_t<T, 64, true, false>(a, s);
     return pair ? packed_tc_t<T, 64, false, true>(a, s) : packed_tc_t<T, 64, false, false>(a, s);
@@ -971,6 +970,10 @@ cudaError_t packed_tc(const PackedArgs& a, cudaStream_t s) {
 }
 
 }  // namespace
+
+bool sattn_packed_fits(const PackedArgs& a) {
+  return packed_tile_bound(a.T, a.R, !a.use_tc ? kPT : (packed_pair(a) ? 128 : 256)) <= 65535;
+}
 
 bool sattn_packed_tc_supported(int D, int dtype) { return (D == 64 || D == 128) && dtype != SSD_F32; }
 

@@ -277,8 +277,8 @@ def sattn_paged_decode(q, k_cache, v_cache, k_scale, v_scale, block_table, lengt
     ``lengths`` ``(R,)`` int32. Request ``r``'s own token is the last of its ``lengths[r]`` (it was
     appended before): the pos-mode gated softmax of :func:`~.kernels.sattn_decode_step`
     (``modules/selective_attention.py:399-404``), in which every key but the own one adds its log-gate
-    and a log-gate of ``-inf`` drops the key. A length of 0 gives zeros. ``scale`` defaults to
-    ``D ** -0.5``. Returns ``(R, Hq, D)`` in ``q``'s dtype. ``workspace`` (contiguous uint8) is
+    and a log-gate of ``-inf`` drops the key. A length of 0 gives zeros. At most 65535
+    requests. ``scale`` defaults to ``D ** -0.5``. Returns ``(R, Hq, D)`` in ``q``'s dtype. ``workspace`` (contiguous uint8) is
     allocated when it is ``None`` or does not do; calls that overlap on the GPU need one each.
     """
     c, H, page, D, d = _cache(k_cache, v_cache, k_scale, v_scale, log_gate_cache)

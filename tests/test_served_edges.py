@@ -5,6 +5,7 @@ Tolerances are those of ``test_paged.py`` and ``test_sattn_packed.py``: a share 
 and a share of the weighted magnitudes sum_j w_j |v_j| that the row adds up for the rounding of its weights, each of
 which is relative. Where one group of keys holds all the weight, that sum is at most the group's largest |v|.
 """
+import ctypes
 import math
 
 import pytest
@@ -27,6 +28,28 @@ def close(got, ref, vmax, tol, what=""):
     err = (got - ref).abs()[fine]
     bound = rel * ref.abs()[fine] + p * vmax
     assert bool((err <= bound).all()), f"{what}: {int((err > bound).sum())} outside, max err {err.max().item():.3e}"
+
+
+# ----------------------------------------------------------------------------- refusals (CPU)
+def test_sizes_past_the_grids_are_invalid_arguments():
+    from selective_attention_b200 import _lib
+
+    L, bad = _lib.lib(), _lib.SSD_ERR_INVALID_ARGUMENT
+
+    def cache(**kw):
+        return ctypes.byref(_lib.SattnCache(**{**dict(num_pages=4, nkv=2, page_size=16, head_dim=64, code=0, k_codes=4096,
+                                                      v_codes=4096, k_scale=4096, v_scale=4096, log_gate=None), **kw}))
+
+    for c, requests in ((cache(), 65536), (cache(num_pages=2 ** 30), 1)):
+        assert L.sattn_paged_decode(c, 4096, 4096, 4096, 4096, requests, 1, 2, 1.0, 1, 4096, 1 << 40, None) == bad
+        assert L.sattn_paged_decode_workspace_size(c, requests, 1, 2) == 0
+    for kw in (dict(num_seqs=65535), dict(num_tokens=256 * 65535, nkv=2), dict(num_tokens=128 * 65535),
+               dict(num_tokens=64 * 65535, dtype=0), dict(num_tokens=64 * 65000, num_seqs=535, impl=_lib.IMPL_SIMT)):
+        p = _lib.SattnPackedParams(**{**dict(
+            num_tokens=4, num_seqs=1, nheads=2, nkv=1, head_dim=64, q_token_stride=128, q_head_stride=64,
+            k_token_stride=64, k_head_stride=64, v_token_stride=64, v_head_stride=64, dtype=1, impl=0, scale=1.0, q=4096,
+            k=4096, v=4096, log_gate=None, cu_seqlens=4096, out=4096), **kw})
+        assert L.sattn_prefill_packed(ctypes.byref(p), None) == bad, kw
 
 
 # ----------------------------------------------------------------------------- decode: page scales
