@@ -783,6 +783,7 @@ int sattn_prefill_packed(const sattn_packed_params* p, void* stream) {
   if (p->num_tokens < 0 || p->num_tokens > 0x7fffffffll || p->num_seqs < 0 || p->num_seqs > 0x7fffffffll ||
       p->nheads <= 0 || p->nkv <= 0 || p->nheads > 0x7fffffffll || p->nheads % p->nkv != 0)
     return SSD_ERR_INVALID_ARGUMENT;
+  if (p->impl != SSD_IMPL_AUTO && p->impl != SSD_IMPL_TC && p->impl != SSD_IMPL_SIMT) return SSD_ERR_INVALID_ARGUMENT;
   const int64_t D = p->head_dim;
   if (D != 16 && D != 32 && D != 64 && D != 128) return SSD_ERR_INVALID_ARGUMENT;
   if (!dtype_ok(p->dtype)) return SSD_ERR_UNSUPPORTED_DTYPE;

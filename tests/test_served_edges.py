@@ -52,6 +52,14 @@ def test_sizes_past_the_grids_are_invalid_arguments():
         assert L.sattn_prefill_packed(ctypes.byref(p), None) == bad, kw
 
 
+def test_an_impl_that_is_not_of_packed_prompts_is_refused():
+    from selective_attention_b200 import _lib
+
+    for impl in (_lib.IMPL_TC_STAGED, -1, 9):
+        p = _lib.SattnPackedParams(num_tokens=0, num_seqs=1, nheads=2, nkv=1, head_dim=64, dtype=1, impl=impl)
+        assert _lib.lib().sattn_prefill_packed(ctypes.byref(p), None) == _lib.SSD_ERR_INVALID_ARGUMENT
+
+
 # ----------------------------------------------------------------------------- decode: page scales
 def _two_kinds_of_pages(kind, high, pages=24, page=16, D=64, seed=0):
     """A request whose pages are of two kinds in mixed order: first element of every key +1 or -1 (so that a
