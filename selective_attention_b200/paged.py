@@ -215,8 +215,9 @@ def sattn_paged_append(k, v, slots, k_cache, v_cache, k_scale, v_scale, log_gate
     earlier codes are rounded anew.
     """
     c, H, _, D, d = _cache(k_cache, v_cache, k_scale, v_scale, log_gate_cache)
-    T = k.shape[0]
-    if not (k.shape == v.shape == (T, H, D) and k.dtype == v.dtype and k.dtype in _lib.DTYPE_CODES
+    shape = k.shape
+    T = shape[0] if len(shape) == 3 else -1
+    if not (shape == v.shape == (T, H, D) and k.dtype == v.dtype and k.dtype in _lib.DTYPE_CODES
             and slots.dtype == _I64 and slots.shape == (T,)
             and k.get_device() == v.get_device() == slots.get_device() == d
             and (log_gate is None) == (log_gate_cache is None)
@@ -282,11 +283,11 @@ def sattn_paged_decode(q, k_cache, v_cache, k_scale, v_scale, block_table, lengt
     allocated when it is ``None`` or does not do; calls that overlap on the GPU need one each.
     """
     c, H, page, D, d = _cache(k_cache, v_cache, k_scale, v_scale, log_gate_cache)
-    shape = q.shape
-    R, Hq = shape[0], shape[1]
-    W = block_table.shape[-1]
-    if not (len(shape) == 3 and shape[2] == D and Hq and Hq % H == 0 and q.dtype in _lib.DTYPE_CODES
-            and block_table.shape == (R, W) and lengths.shape == (R,) and block_table.dtype == lengths.dtype == _I32
+    shape, table = q.shape, block_table.shape
+    R, Hq = shape[:2] if len(shape) == 3 else (-1, 0)
+    W = table[1] if len(table) == 2 else -1
+    if not (Hq and shape[2] == D and Hq % H == 0 and q.dtype in _lib.DTYPE_CODES
+            and table == (R, W) and lengths.shape == (R,) and block_table.dtype == lengths.dtype == _I32
             and block_table.is_contiguous() and lengths.is_contiguous()
             and q.get_device() == block_table.get_device() == lengths.get_device() == d):
         _decode_faults(q, k_cache, block_table, lengths, H, D)

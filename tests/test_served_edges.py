@@ -60,6 +60,34 @@ def test_an_impl_that_is_not_of_packed_prompts_is_refused():
         assert _lib.lib().sattn_prefill_packed(ctypes.byref(p), None) == _lib.SSD_ERR_INVALID_ARGUMENT
 
 
+@pytest.mark.gpu
+def test_tensors_of_other_ranks_are_refused():
+    import selective_attention_b200 as sab
+
+    c = {n: t.cuda() for n, t in _two_kinds_of_pages(torch.int8, 1.0)[0].items()}
+    i32 = dict(dtype=torch.int32, device="cuda")
+    q, k, slots = torch.zeros(2, 4, 64, device="cuda"), torch.zeros(3, 1, 64, device="cuda"), torch.arange(3, device="cuda")
+    table, n, cu = torch.zeros(2, 3, **i32), torch.zeros(2, **i32), torch.zeros(2, **i32)
+    state = torch.zeros(2, dtype=torch.int64, device="cuda")
+    for bad in (dict(q=q[0, 0, 0]), dict(q=q[0, 0]), dict(q=q[0]), dict(q=q[None]), dict(block_table=table[0, 0]),
+                dict(block_table=table[0]), dict(block_table=table[None]), dict(lengths=n[0]), dict(lengths=table)):
+        with pytest.raises(ValueError):
+            sab.sattn_paged_decode(**{**dict(q=q, block_table=table, lengths=n), **c, **bad})
+    for bad in (dict(k=k[0, 0, 0]), dict(k=k[0]), dict(v=k[0, 0]), dict(slots=slots[0]), dict(slots=slots[None])):
+        with pytest.raises(ValueError):
+            sab.sattn_paged_append(**{**dict(k=k, v=k, slots=slots), **c, **bad})
+    for bad in (dict(q=k[0, 0, 0]), dict(k=k[0]), dict(v=k[0, 0]), dict(cu_seqlens=cu[0]), dict(cu_seqlens=cu[None])):
+        with pytest.raises(ValueError):
+            sab.sattn_prefill_packed(**{**dict(q=k, k=k, v=k, cu_seqlens=cu), **bad})
+    for bad in (dict(lengths=n[0]), dict(new_lengths=n[None]), dict(block_table=table[0]), dict(free_pages=n[0]),
+                dict(free_state=state[0])):
+        with pytest.raises(ValueError):
+            sab.sattn_paged_plan(**{**dict(lengths=n, new_lengths=n, block_table=table, free_pages=n, free_state=state,
+                                           num_tokens=0, page_size=16), **bad})
+    with pytest.raises(ValueError):
+        sab.sattn_paged_read(slots[0], *(c[x] for x in ("k_cache", "v_cache", "k_scale", "v_scale")))
+
+
 # ----------------------------------------------------------------------------- decode: page scales
 def _two_kinds_of_pages(kind, high, pages=24, page=16, D=64, seed=0):
     """A request whose pages are of two kinds in mixed order: first element of every key +1 or -1 (so that a
