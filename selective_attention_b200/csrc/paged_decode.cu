@@ -486,10 +486,11 @@ __global__ void __launch_bounds__(kDecThreads, dec_ctas_per_sm<D, NG>())
         in0[u] = live && t0 < n, in1[u] = live && t1 < n;
         float g0 = 0.f, g1 = 0.f;
         if (a.gc) {
-          g0 = t0 < n - 1 ? iu[lr] * kDecLog2e : 0.f;
-          g1 = t1 < n - 1 ? iu[lr + 8] * kDecLog2e : 0.f;
+          g0 = t0 < n - 1 ? iu[lr] : 0.f;
+          g1 = t1 < n - 1 ? iu[lr + 8] : 0.f;
           in0[u] = in0[u] && g0 != -INFINITY;
           in1[u] = in1[u] && g1 != -INFINITY;
+          g0 *= kDecLog2e, g1 *= kDecLog2e;
         }
         const float lv = above(iu[17]);
 #pragma unroll

@@ -5,6 +5,7 @@
 // Query head h reads key head h / (Hq / Hk). A key whose log-gate is -inf drops out for every later
 // query, whatever it holds, and so does every key that a query does not see: a NaN or an infinity
 // there changes nothing. Rows past the last sequence are written as zeros.
+#include <float.h>
 #include <math.h>
 
 #include <type_traits>
@@ -659,7 +660,11 @@ __global__ void __launch_bounds__(kPkThreads, 1)
       const int care = work.tiles0() - 1, nk = max(work.tiles0(), work.tiles1(PAIR)), hk = work.head / group;
       auto gate_at = [&](int key) {
         if constexpr (!GATED) return 0.f;
-        return key < work.n ? a.lg[(long long)(work.seq0 + key) * a.Hk + hk] * kPkLog2e : 0.f;
+        return key < work.n ? a.lg[(long long)(work.seq0 + key) * a.Hk + hk] : 0.f;
+      };
+      auto in_log2 = [](float x) {  // (only -inf itself drops a key)
+        const float y = x * kPkLog2e;
+        return y == -INFINITY && x != -INFINITY ? -FLT_MAX : y;
       };
       int j = GATED ? 0 : care;
       float g0 = gate_at(128 * j + t), g1 = gate_at(128 * j + t + 64);
@@ -675,8 +680,8 @@ __global__ void __launch_bounds__(kPkThreads, 1)
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         if constexpr (GATED) {
-          gates[((tiles + j) % GS) * 128 + t] = g0;
-          gates[((tiles + j) % GS) * 128 + t + 64] = g1;
+          gates[((tiles + j) % GS) * 128 + t] = in_log2(g0);
+          gates[((tiles + j) % GS) * 128 + t + 64] = in_log2(g1);
           if (j < care) {
 #pragma unroll
             for (int half = 0; half < 2; ++half) {

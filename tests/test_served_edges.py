@@ -288,3 +288,45 @@ def test_pages_come_back_whole_after_a_plan_for_too_few_tokens():
     head, tail = c.free_state.tolist()
     ring = c.free_pages.tolist()
     assert sorted(ring[i % 6] for i in range(head, tail)) == list(range(6))
+
+
+# ----------------------------------------------------------------------------- gates of the type's lowest value
+LOWEST = torch.finfo(torch.float32).min
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("D", [64, 128])
+def test_a_gate_of_the_lowest_value_does_not_drop_its_key_from_prompts(dtype, D):
+    """Only -inf drops a key. One with the lowest finite gate has no weight, but a NaN there is seen."""
+    g = torch.Generator().manual_seed(D)
+    T = 300
+    q, k, v = (torch.randn(T, 2, D, generator=g).to(dtype) for _ in range(3))
+    gate = torch.nn.functional.logsigmoid(torch.randn(T, 2, generator=g))
+    gate[torch.rand(T, 2, generator=g) < 0.5] = LOWEST
+    vmax = v.float().abs().max().item()
+    got, ref = _prompt(q, k, v, gate)
+    close(got, ref, vmax, PROMPT_TOL, "no weight")
+    gate[:, 1] = LOWEST
+    got, ref = _prompt(q, k, v, gate)
+    close(got, ref, vmax, PROMPT_TOL, "no weight for any earlier key")
+    gate[[5, 270]], v[5, 0, 2], v[270, 1, 7] = LOWEST, NAN, NAN
+    gate[[9, 280]], v[9, 0, 3], v[280, 1, 4] = -INF, NAN, NAN  # these rows alone
+    got, ref = _prompt(q, k, v, gate)
+    assert bool(ref[5:, 0, 2].isnan().all()) and bool(ref[270:, 1, 7].isnan().all())
+    assert int(ref[:, 0, 3].isnan().sum()) == 1 and int(ref[:, 1, 4].isnan().sum()) == 1
+    close(got, ref, vmax, PROMPT_TOL, "NaN")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_a_gate_of_the_lowest_value_does_not_drop_its_key_from_a_decode(dtype):
+    c, table, _ = _two_kinds_of_pages(torch.float8_e4m3fn, 1.0 / 96)
+    gate = torch.full((24, 1, 16), LOWEST)
+    gate[7] = -INF
+    c["v_cache"].view(torch.uint8)[4, 0, 3, 5] = 0x7f  # seen
+    c["v_cache"].view(torch.uint8)[7, 0, 3, 6] = 0x7f  # dropped
+    q = torch.randn(1, 2, 64, generator=torch.Generator().manual_seed(3)).to(dtype)
+    got, ref = _decode(c, q, table, torch.tensor([24 * 16], dtype=torch.int32), gate, 0.5)
+    assert bool(ref[..., 5].isnan().all()) and not bool(ref[..., 6].isnan().any())
+    close(got, ref, 1.0, DECODE_TOL)
