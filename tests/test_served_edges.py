@@ -330,3 +330,51 @@ def test_a_gate_of_the_lowest_value_does_not_drop_its_key_from_a_decode(dtype):
     got, ref = _decode(c, q, table, torch.tensor([24 * 16], dtype=torch.int32), gate, 0.5)
     assert bool(ref[..., 5].isnan().all()) and not bool(ref[..., 6].isnan().any())
     close(got, ref, 1.0, DECODE_TOL)
+
+
+# ----------------------------------------------------------------------------- decode: many rows to join
+@pytest.mark.gpu
+@pytest.mark.parametrize("Hq,Hk,D,gated", [(16, 2, 64, True), (20, 2, 128, False), (16, 4, 256, False), (16, 1, 32, True)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_many_rows_that_several_ctas_share(Hq, Hk, D, gated, dtype):
+    """From 592 requests x query heads on a row's parts are joined by four warps instead of sixteen."""
+    from test_paged import _check_decode, _filled
+
+    lens = [(97 * i) % 331 for i in range(39)] + [620]
+    c, table, n = _filled(lens, Hk, D, 16, torch.int8, gated)
+    q = torch.randn(len(lens), Hq, D, generator=torch.Generator().manual_seed(3)).to(dtype)
+    got = _check_decode(c, table, n, q)
+    assert torch.equal(got, _check_decode(c, table, n, q))
+
+
+# ----------------------------------------------------------------------------- captured calls
+@pytest.mark.gpu
+def test_captured_append_decode_and_prompts_replay():
+    """The functions' launches in a graph, on inputs that change between replays; the calls' own tensors are the state."""
+    import selective_attention_b200 as sab
+
+    g = torch.Generator().manual_seed(1)
+    c = sab.PagedSelectiveCache(1, 3, 1024, 200, 2, 64)
+    lens = [700, 33, 300]
+    cu, slots, _ = c.plan(torch.tensor(lens, dtype=torch.int32, device="cuda"), sum(lens))
+    k, v = (torch.randn(sum(lens), 2, 64, generator=g).bfloat16().cuda() for _ in range(2))
+    q = torch.randn(sum(lens), 4, 64, generator=g).bfloat16().cuda()
+    gate = torch.nn.functional.logsigmoid(torch.randn(sum(lens), 2, generator=g)).cuda()
+
+    def step():
+        c.append(0, k, v, slots, gate)
+        return sab.sattn_prefill_packed(q, k, v, cu, gate), c.decode(0, q[:3])
+
+    step()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        outs = step()
+    for _ in range(2):
+        for t in (k, v, q):
+            t.copy_(torch.randn(t.shape, generator=g).bfloat16())
+        graph.replay()
+        got = [o.clone() for o in outs]
+        for a, b in zip(got, step()):
+            assert torch.equal(a, b)
