@@ -426,7 +426,7 @@ int sattn_paged_plan(const int32_t* lengths, const int32_t* new_lengths, int32_t
  *   old = first > 0 ? scale : 0;  new = max(old, max|x| * (1 / largest code))   (fp32, finite x only)
  *   codes of the call's tokens = round(x / new) (ties to even, saturated); the page's earlier codes
  *   become round(code * (old / new)) where new > old.
- * A NaN is held as 0 (int8) or NaN (e4m3), an infinity as the largest code.
+ * A NaN is held as 0 (int8) or NaN (e4m3), an infinity as the largest code; where new is 0, all codes are 0.
  *   k, v      (num_tokens, Hkv, D)  dtype, with token and head strides in elements
  *   log_gate  (num_tokens, Hkv)     fp32; NULL exactly when the cache has none
  */

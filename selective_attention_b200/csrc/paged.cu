@@ -28,7 +28,8 @@ namespace {
 // the token at its first position, so no two threads write one entry and none is read that
 // another writes; so only a request whose tokens are all among the T that are planned is served, or it
 // would hold pages that its table does not name. Those that are come first, so that a sum that has stopped
-// is never theirs. Bound by latency: 256 requests of one token each take 3 us, 384 prompts with 393k tokens 5.
+// is never theirs. Bound by latency and each CTA's scan: 256 requests
+// of one token each take 4.4 us (captured in a graph), 384 prompts with 393k tokens (386 CTAs) 8.9.
 constexpr int kPlanThreads = 256;
 constexpr int kPlanPer = 4;
 constexpr int kPlanTokens = kPlanThreads * kPlanPer;
@@ -180,8 +181,9 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(
 // flight together, and stay in registers as they came (the rows past the first kAppHeld passes
 // are read again); then the largest finite magnitude of each row, the segment's scale from its
 // rows and the page's old scale, and the codes of the rows and, where the scale grew, of the
-// page's older rows. 16k tokens of 8 heads of 128 (fp16 to e4m3, K and V) take 50 us, bound by instructions
-// (about 300 for 16 elements of a warp's two rows) between the barriers; their 63 MB alone would take 10.
+// page's older rows. 16k tokens of 8 heads of 128 (fp16 to e4m3, K and V) take 51 us back to back and 57 with cold
+// caches, bound by instructions (about 300 for 16 elements of a warp's two rows) between the barriers; the 65 MB
+// that they are and the 33 MB of codes would take 15 at the copy rate.
 constexpr int kAppThreads = 256;
 constexpr int kAppRows = 256;  // rows of one CTA: per + page - 1 <= 255
 constexpr int kAppHeld = 8;
@@ -374,7 +376,8 @@ __global__ void __launch_bounds__(kAppThreads) paged_append_kernel(
 // ---------------------------------------------------------------------------
 // read: values of the given slots, (N, H, D) for K and V; slots outside the cache give zeros.
 // One thread reads 8 codes and writes 8 values, fp32 as a whole 32-byte sector. Bound by writing them: 16k slots
-// of 8 heads of 128 (33 MB read, 132 MB written) take 23 us, the copy rate's time.
+// of 8 heads of 128 (33 MB read, 132 MB written) take 33 us with cold caches and 28 back to back, where half of what
+// is written stays in L2; at the copy rate they would take 25.
 // ---------------------------------------------------------------------------
 constexpr int kReadThreads = 256;
 constexpr int kReadItems = 4;  // of a thread, their codes all in flight

@@ -780,7 +780,10 @@ bool make_map_codes(CUtensorMap* map, const void* base, int D, int page, uint64_
 }
 
 // Query heads of one row group: 16 where more than 8 share a key head (one reading serves twice as
-// many; with head_dim 256 the registers hold 8), else 8.
+// many; with head_dim 256 the registers hold 8), else 8. With fp32 queries the registers do not quite hold
+// them: head_dim 128 with 16 heads spills 220 bytes a thread, head_dim 256 up to 194 (16-bit queries 60 and 24).
+// 32 requests of up to 4096 tokens with cold caches, fp32 and bf16 queries: 32 heads on 2 of 128 (36 MB) 37 and 30 us,
+// 16 heads on 2 of 256 (73 MB) 42 and 36.
 int dec_ng(int g, int D) { return g > 8 && D < 256 ? 2 : 1; }
 int dec_ctas(int g, int D) {
   const int per = D == 256 || dec_ng(g, D) == 2 ? 2 : (D == 128 ? 3 : 4);

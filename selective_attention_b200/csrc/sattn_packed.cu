@@ -272,7 +272,7 @@ cudaError_t packed_simt_t(const PackedArgs& a, cudaStream_t s) {
 // (one exponential a score: 16 a clock and SM, just as long as the products of head_dim 128).
 // Every second to eighth pair of exponentials on the FMA pipes instead (a cubic) gained 4 % on a cool card
 // and lost 1 to 7 % at the power limit, where such kernels run when there is more than one of them.
-// A prompt of 8192 tokens, 32 heads on 8 of 128, bf16: 477 us (1150 TFLOP/s) cool, 550 us (1000) back to
+// A prompt of 8192 tokens, 32 heads on 8 of 128, bf16: 471 us (1170 TFLOP/s) cool, 548 us (1000) back to
 // back; a pair of 128 x 128 tiles takes 3400 cycles, of which its products alone 2040.
 // TMEM columns: S_0 [0, 128) S_1 [128, 256) (P_w in the first 64 of S_w) O_0 [256, 256 + D) O_1 [384, 384 + D).
 // Every wait is bounded; a role that gives up records a site code and leaves its loop, and the others'

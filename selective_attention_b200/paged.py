@@ -393,7 +393,8 @@ class PagedSelectiveCache:
     either :func:`sattn_prefill_packed` (whole prompts, packed by the plan's ``cu_seqlens``) or
     :meth:`decode` (one token for each request); :meth:`release` gives a finished request's pages
     back. Nothing synchronizes: which requests a plan served is read from its ``lengths`` when the
-    host wants to know.
+    host wants to know. :meth:`plan` and :meth:`release` put new tensors in the place of ``lengths`` and
+    ``free_state``: what is captured in a graph once and replayed is a step's appends and its attention, not these.
     """
 
     def __init__(self, layers: int, requests: int, max_tokens: int, num_pages: int, heads: int, head_dim: int,
